@@ -336,6 +336,61 @@ int peer_select_noalloc(const peer_config_t* cfg, const float* queries, const vo
 int peer_usage_histogram(const int64_t* ids, int64_t n_ids, int64_t* counts, int64_t num_experts,
                          int64_t* dropped, void* stream);
 
+/* ---- Training operators around the layer -------------------------------------------------------------
+ * No handle: every buffer, workspaces included, is the caller's, so calls on different streams or in
+ * different captured graphs never share memory.  All are asynchronous on `stream` of the current device.
+ * Rows are `dim` consecutive values (1 <= dim <= PEER_ROW_DIM_MAX); inputs may have a row stride (in
+ * elements) of their own, outputs are contiguous.  dtype: F32, BF16 or F16; sums and statistics are fp32.
+ * Results do not vary from run to run (no accumulation in memory). */
+#define PEER_ROW_DIM_MAX (1 << 20)
+
+/* Layer norm, the block's ln_2 (llm/models/foundation.py:118, 196-199) as an operator with a gradient:
+ * y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps).  weight, bias (fp32 or dtype, said by
+ * param_dtype) may be NULL.  mean, rstd [rows] are for the backward pass (may be NULL); payload [rows, dim]
+ * bytes and scale [rows] (both or none) receive x in the form of peer_pack_rows. */
+int peer_layer_norm(const void* x, int64_t x_stride, int32_t dtype, const void* weight, const void* bias,
+                    int32_t param_dtype, float eps, int64_t rows, int64_t dim, void* y, float* mean, float* rstd,
+                    void* payload, float* scale, void* stream);
+
+/* Bytes of workspace the sums of grad_weight / grad_bias need. */
+int64_t peer_layer_norm_workspace(int64_t rows, int64_t dim);
+
+/* Gradients of peer_layer_norm from grad_y, x (or, when payload and scale are given, the values they stand
+ * for; x may then be NULL) and the forward pass's mean and rstd.  grad_x (dtype), grad_weight and grad_bias
+ * (param_dtype) are written; any of them may be NULL.  `add` (contiguous [rows, dim] or NULL) is added to
+ * grad_x before its rounding: the gradient of a residual branch around the norm.  grad_x may not alias an
+ * input.  workspace: peer_layer_norm_workspace bytes, 16-byte aligned (NULL when neither sum is wanted). */
+int peer_layer_norm_backward(const void* grad_y, int64_t grad_stride, const void* x, int64_t x_stride, const void* payload,
+                             const float* scale, const float* mean, const float* rstd, const void* weight, int32_t dtype,
+                             int32_t param_dtype, const void* add, int64_t rows, int64_t dim, void* grad_x,
+                             void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Activation checkpoints: rows as e4m3 bytes with one fp32 scale each, the smallest power of two that brings
+ * the row's largest finite magnitude to at most 448 (1 for a row of zeros, at least 2^-126).  Rounded to
+ * nearest even; infinite and NaN values become NaN. */
+int peer_pack_rows(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t dim, void* payload,
+                   float* scale, void* stream);
+
+/* The values packed rows stand for: payload * scale, clamped to dtype's finite range. */
+int peer_unpack_rows(const void* payload, const float* scale, int32_t dtype, int64_t rows, int64_t dim, void* out,
+                     void* stream);
+
+/* out[t] = scale * weight[ids[t]] (the model's token embedding, llm/models/foundation.py:338); ids int32 or
+ * int64 (id_bytes 4 or 8).  An id outside [0, vocab) reads nothing: its row is zero, and it is added to
+ * *dropped when that pointer is given. */
+int peer_embedding(const void* ids, int32_t id_bytes, int64_t n_ids, const void* weight, int32_t dtype, int64_t vocab,
+                   int64_t dim, float scale, void* out, int64_t* dropped, void* stream);
+
+/* Bytes of workspace peer_embedding_backward needs. */
+int64_t peer_embedding_workspace(int64_t n_ids, int64_t dim);
+
+/* grad_weight[v] = scale * sum of grad[t] over ids[t] = v: every row of grad_weight [vocab, dim] is written, the sums are
+ * in fp32 in the order of t and rounded once.  Ids outside the table, and padding_idx (-1: none), take no part.
+ * workspace: peer_embedding_workspace bytes, 16-byte aligned. */
+int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_t n_ids, const void* grad, int64_t grad_stride,
+                            int32_t dtype, int64_t vocab, int64_t dim, float scale, int64_t padding_idx, void* grad_weight,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Reads and clears the device status word (synchronises `stream`).  Returns
  * PEER_OK, PEER_ERR_DEVICE_TIMEOUT or PEER_ERR_BOUNDS.  The kernels never
  * trap: a bounded wait that runs out, or an expert id outside the table,

@@ -80,6 +80,19 @@ EXPORTS = {
     "peer_xchg_status": (C.c_int, [C.c_void_p, C.c_void_p]),
     "peer_xchg_destroy": (C.c_int, [C.c_void_p]),
     "peer_usage_histogram": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "peer_layer_norm": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_float, C.c_int64,
+                                  C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "peer_layer_norm_workspace": (C.c_int64, [C.c_int64, C.c_int64]),
+    "peer_layer_norm_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                           C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int64,
+                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "peer_pack_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "peer_unpack_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
+    "peer_embedding": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_float,
+                                 C.c_void_p, C.c_void_p, C.c_void_p]),
+    "peer_embedding_workspace": (C.c_int64, [C.c_int64, C.c_int64]),
+    "peer_embedding_backward": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int64,
+                                          C.c_int64, C.c_float, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "peer_query_status": (C.c_int, [C.c_void_p, C.c_void_p]),
     "peer_launch_count": (C.c_int64, [C.c_void_p]),
     "peer_freeze_keys": (C.c_int, [C.c_void_p, C.c_int]),

@@ -206,6 +206,19 @@ cudaError_t launch_route_tuples(const int32_t* ids, const float* weights, int64_
 // LayerNorm over the model dimension, fp32 parameters (block_ln.cu)
 cudaError_t launch_block_ln(const void* x, int act_dtype, int64_t rows, int D, const float* w, const float* b, float eps,
                             void* out, cudaStream_t s);
+// Positions of ids in the order of the ids (row_sort.cu).  `row_sort_layout` cuts a workspace of `row_sort_bytes(n)`
+// bytes; after the launch `sorted_keys` / `order` point at the sorted ids (vocab for the skipped ones, at the end) and
+// their positions.
+struct RowSortArgs {
+    const void* ids; int id_bytes;        // int32 or int64
+    int64_t n, vocab, skip;               // ids outside [0, vocab) and the id `skip` are left out
+    uint32_t* keys[2]; uint32_t* pos[2]; uint32_t* counts; uint32_t* totals;
+    uint32_t* sorted_keys; uint32_t* order;
+};
+int64_t row_sort_bytes(int64_t n);
+void row_sort_layout(RowSortArgs& a, void* workspace);
+cudaError_t launch_row_sort(RowSortArgs& a, cudaStream_t s);
+
 // one-time per-process attribute set-up (dynamic shared memory opt-in)
 cudaError_t select_simt_setup();
 

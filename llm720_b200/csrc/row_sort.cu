@@ -1,0 +1,182 @@
+// Positions of table ids in the order of the ids: a stable sort of (id,
+// position) pairs by least-significant digits of at most 8 bits.  Equal ids keep
+// the order of their positions, so a sum over an id's positions has one fixed
+// order.  Ids outside [0, vocab), and the one id given as `skip`, get the key
+// `vocab` and end up behind all others.
+//
+// Per digit: (1) every tile of keys counts its digits, (2) every digit scans its
+// counts over the tiles, (3) every tile scatters its keys; the rank of a key
+// among its tile's equal digits comes from a vote over the warp
+// (match.any) on top of a running count per warp and digit.
+#include "kernels.h"
+#include "row_ops.cuh"
+
+namespace peer {
+
+namespace {
+
+constexpr int SORT_THREADS = 256;
+constexpr int SORT_WARPS = SORT_THREADS / 32;
+constexpr int MAX_DIGITS = 256;
+
+__device__ __forceinline__ uint32_t source_key(const RowSortArgs& a, int64_t i) {
+    const int64_t id = a.id_bytes == 8 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
+    return (id < 0 || id >= a.vocab || id == a.skip) ? static_cast<uint32_t>(a.vocab) : static_cast<uint32_t>(id);
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const RowSortArgs a, const uint32_t* __restrict__ keys, int shift,
+                                                                  int digits, int items, int tiles) {
+    __shared__ uint32_t hist[MAX_DIGITS];
+    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0u;
+    __syncthreads();
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * SORT_THREADS * items;
+    for (int i = 0; i < items; ++i) {
+        const int64_t j = t0 + static_cast<int64_t>(i) * SORT_THREADS + threadIdx.x;
+        if (j < a.n) {
+            const uint32_t key = FIRST ? source_key(a, j) : keys[j];
+            atomicAdd(&hist[(key >> shift) & (digits - 1)], 1u);
+        }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) a.counts[static_cast<int64_t>(d) * tiles + blockIdx.x] = hist[d];
+}
+
+// block d: exclusive scan of digit d's counts over the tiles, in place; the digit's total
+__global__ void __launch_bounds__(SORT_THREADS) sort_scan_kernel(const RowSortArgs a, int tiles) {
+    __shared__ uint32_t warp_total[SORT_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t* row = a.counts + static_cast<int64_t>(blockIdx.x) * tiles;
+    uint32_t carry = 0u;
+    for (int t0 = 0; t0 < tiles; t0 += SORT_THREADS) {
+        const int t = t0 + threadIdx.x;
+        const uint32_t v = t < tiles ? row[t] : 0u;
+        uint32_t inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(FULL_MASK, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) warp_total[warp] = inc;
+        __syncthreads();
+        uint32_t before = carry, all = 0u;
+#pragma unroll
+        for (int i = 0; i < SORT_WARPS; ++i) {
+            const uint32_t u = warp_total[i];
+            if (i < warp) before += u;
+            all += u;
+        }
+        if (t < tiles) row[t] = before + inc - v;
+        carry += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) a.totals[blockIdx.x] = carry;
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const RowSortArgs a, const uint32_t* __restrict__ keys,
+                                                                    const uint32_t* __restrict__ pos, uint32_t* __restrict__ keys_out,
+                                                                    uint32_t* __restrict__ pos_out, int shift, int digits, int items,
+                                                                    int tiles) {
+    __shared__ uint32_t seen[SORT_WARPS][MAX_DIGITS];       // running count per warp and digit, then the warp's first slot
+    __shared__ uint32_t warp_total[SORT_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int d = threadIdx.x; d < SORT_WARPS * MAX_DIGITS; d += SORT_THREADS) (&seen[0][0])[d] = 0u;
+    __syncthreads();
+    // a warp owns `items` consecutive groups of 32 keys, in order
+    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) * SORT_WARPS + warp) * items * 32;
+    uint32_t key[16], rank[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (i >= items) break;
+        const int64_t j = w0 + i * 32 + lane;
+        const bool in = j < a.n;
+        key[i] = in ? (FIRST ? source_key(a, j) : keys[j]) : 0u;
+        const uint32_t digit = (key[i] >> shift) & (digits - 1);
+        const unsigned same = __match_any_sync(FULL_MASK, in ? digit : 0xffffffffu);
+        const int leader = __ffs(same) - 1;
+        uint32_t before = 0u;
+        if (in && lane == leader) {
+            before = seen[warp][digit];
+            seen[warp][digit] = before + __popc(same);
+        }
+        before = __shfl_sync(FULL_MASK, before, leader);
+        rank[i] = before + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+    }
+    __syncthreads();
+    // first slot of digit d: all smaller digits' totals + this digit's earlier tiles + its earlier warps
+    {
+        const int d = threadIdx.x;
+        const uint32_t v = d < digits ? a.totals[d] : 0u;
+        uint32_t inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(FULL_MASK, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) warp_total[warp] = inc;
+        __syncthreads();
+        uint32_t first = inc - v;
+#pragma unroll
+        for (int i = 0; i < SORT_WARPS; ++i) if (i < warp) first += warp_total[i];
+        if (d < digits) {
+            first += a.counts[static_cast<int64_t>(d) * tiles + blockIdx.x];
+#pragma unroll
+            for (int i = 0; i < SORT_WARPS; ++i) { const uint32_t u = seen[i][d]; seen[i][d] = first; first += u; }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (i >= items) break;
+        const int64_t j = w0 + i * 32 + lane;
+        if (j < a.n) {
+            const uint32_t slot = seen[warp][(key[i] >> shift) & (digits - 1)] + rank[i];
+            keys_out[slot] = key[i];
+            pos_out[slot] = FIRST ? static_cast<uint32_t>(j) : pos[j];
+        }
+    }
+}
+
+int bit_length(int64_t v) { int b = 0; while (v > 0) { ++b; v >>= 1; } return b; }
+int items_for(int64_t n) { return n <= (1 << 16) ? 4 : 16; }
+int64_t round256(int64_t v) { return (v + 255) & ~static_cast<int64_t>(255); }
+int64_t tiles_for(int64_t n) { const int64_t t = SORT_THREADS * items_for(n); return (n + t - 1) / t; }
+
+}  // namespace
+
+int64_t row_sort_bytes(int64_t n) {
+    return 4 * round256(n * 4) + round256(tiles_for(n) * MAX_DIGITS * 4) + round256(MAX_DIGITS * 4);
+}
+
+void row_sort_layout(RowSortArgs& a, void* workspace) {
+    char* p = static_cast<char*>(workspace);
+    const int64_t each = round256(a.n * 4);
+    for (int i = 0; i < 2; ++i) { a.keys[i] = reinterpret_cast<uint32_t*>(p); p += each; a.pos[i] = reinterpret_cast<uint32_t*>(p); p += each; }
+    a.counts = reinterpret_cast<uint32_t*>(p);
+    p += round256(tiles_for(a.n) * MAX_DIGITS * 4);
+    a.totals = reinterpret_cast<uint32_t*>(p);
+}
+
+cudaError_t launch_row_sort(RowSortArgs& a, cudaStream_t s) {
+    const int bits = bit_length(a.vocab);                    // keys are 0 .. vocab
+    const int passes = (bits + 7) / 8, per = (bits + passes - 1) / passes;
+    const int items = items_for(a.n), tiles = static_cast<int>(tiles_for(a.n));
+    const int digits = 1 << per;
+    for (int p = 0; p < passes; ++p) {
+        const int in = (p + 1) & 1, out = p & 1, shift = p * per;
+        if (p == 0) sort_count_kernel<true><<<tiles, SORT_THREADS, 0, s>>>(a, nullptr, shift, digits, items, tiles);
+        else sort_count_kernel<false><<<tiles, SORT_THREADS, 0, s>>>(a, a.keys[in], shift, digits, items, tiles);
+        sort_scan_kernel<<<digits, SORT_THREADS, 0, s>>>(a, tiles);
+        if (p == 0)
+            sort_scatter_kernel<true><<<tiles, SORT_THREADS, 0, s>>>(a, nullptr, nullptr, a.keys[out], a.pos[out], shift, digits, items, tiles);
+        else
+            sort_scatter_kernel<false><<<tiles, SORT_THREADS, 0, s>>>(a, a.keys[in], a.pos[in], a.keys[out], a.pos[out], shift, digits, items, tiles);
+        a.sorted_keys = a.keys[out];
+        a.order = a.pos[out];
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace peer

@@ -30,5 +30,19 @@ def as_rows(t: torch.Tensor) -> torch.Tensor:
     return rows if D == 1 or rows.stride(1) == 1 else rows.contiguous()
 
 
-def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# torch.cuda.current_stream and torch.cuda.device cost 4 and 1.5 us a call, more than the launch they are for; the raw
+# accessors cost 0.2 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(entry, device: torch.device, *args) -> None:
+    """Call a C entry point with the current stream of ``device`` as its last argument; raise on an error code."""
+    index = device.index
+    if _current_device() == index:
+        rc = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)

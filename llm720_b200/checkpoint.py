@@ -19,7 +19,7 @@ from typing import Tuple
 import torch
 
 from . import _lib
-from ._rows import DTYPES, as_rows, require_cuda, require_dtype, stream_of
+from ._rows import DTYPES, as_rows, launch, require_cuda, require_dtype
 
 
 def pack_rows_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -32,9 +32,8 @@ def pack_rows_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     payload = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     rows = as_rows(x)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().peer_pack_rows(rows.data_ptr(), rows.stride(0), dt, rows.shape[0], rows.shape[1],
-                                              payload.data_ptr(), scale.data_ptr(), stream_of(x.device)))
+    launch(_lib.load().peer_pack_rows, x.device, rows.data_ptr(), rows.stride(0), dt, *rows.shape, payload.data_ptr(),
+           scale.data_ptr())
     return payload, scale
 
 
@@ -52,7 +51,6 @@ def unpack_rows_e4m3(payload: torch.Tensor, scale: torch.Tensor, dtype: torch.dt
     payload, scale = payload.contiguous(), scale.contiguous()
     out = torch.empty(payload.shape, dtype=dtype, device=payload.device)
     D = payload.shape[-1]
-    with torch.cuda.device(payload.device):
-        _lib.check(_lib.load().peer_unpack_rows(payload.data_ptr(), scale.data_ptr(), DTYPES[dtype], payload.numel() // D, D,
-                                                out.data_ptr(), stream_of(payload.device)))
+    launch(_lib.load().peer_unpack_rows, payload.device, payload.data_ptr(), scale.data_ptr(), DTYPES[dtype],
+           payload.numel() // D, D, out.data_ptr())
     return out

@@ -94,4 +94,199 @@ template <typename T> __device__ __forceinline__ float param_at(const void* p, b
     return f32 ? static_cast<const float*>(p)[i] : to_f32<T>(static_cast<const T*>(p)[i]);
 }
 
+
+// ---------------------------------------------------------------------------
+// Pieces of a row: what one thread loads at once.  Wide: 16 bytes (rows whose start, stride and width are multiples
+// of 16 bytes); narrow: one value.
+// ---------------------------------------------------------------------------
+template <typename T, bool WIDE> struct Piece;
+template <typename T> struct Piece<T, false> {
+    static constexpr int N = 1;
+    using Raw = T;
+    using Packed = uint8_t;
+    __device__ static __forceinline__ Raw zero() { return from_f32<T>(0.f); }
+    __device__ static __forceinline__ Raw load(const T* p) { return __ldg(p); }
+    __device__ static __forceinline__ void store(T* p, const Raw& r) { *p = r; }
+    __device__ static __forceinline__ void decode(const Raw& r, float (&f)[1]) { f[0] = to_f32<T>(r); }
+    __device__ static __forceinline__ Raw encode(const float (&f)[1]) { return from_f32<T>(f[0]); }
+    __device__ static __forceinline__ Packed load_packed(const uint8_t* p) { return __ldg(p); }
+    __device__ static __forceinline__ void decode_packed(const Packed& r, float s, float (&f)[1]) { f[0] = unpacked<T>(e4m3_value(r), s); }
+    __device__ static __forceinline__ Packed encode_packed(const float (&f)[1]) { return static_cast<uint8_t>(e4m3_pair(f[0], 0.f)); }
+};
+template <> struct Piece<float, true> {
+    static constexpr int N = 4;
+    using Raw = uint4;
+    using Packed = uint32_t;
+    __device__ static __forceinline__ Raw zero() { return make_uint4(0u, 0u, 0u, 0u); }
+    __device__ static __forceinline__ Raw load(const float* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ static __forceinline__ void store(float* p, const Raw& r) { *reinterpret_cast<uint4*>(p) = r; }
+    __device__ static __forceinline__ void decode(const Raw& r, float (&f)[4]) {
+        f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+    }
+    __device__ static __forceinline__ Raw encode(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    __device__ static __forceinline__ Packed load_packed(const uint8_t* p) { return __ldg(reinterpret_cast<const uint32_t*>(p)); }
+    __device__ static __forceinline__ void decode_packed(const Packed& r, float s, float (&f)[4]) {
+        const float2 a = e4m3_pair_values(static_cast<uint16_t>(r)), b = e4m3_pair_values(static_cast<uint16_t>(r >> 16));
+        f[0] = unpacked<float>(a.x, s); f[1] = unpacked<float>(a.y, s); f[2] = unpacked<float>(b.x, s); f[3] = unpacked<float>(b.y, s);
+    }
+    __device__ static __forceinline__ Packed encode_packed(const float (&f)[4]) {
+        return e4m3_pair(f[0], f[1]) | (static_cast<uint32_t>(e4m3_pair(f[2], f[3])) << 16);
+    }
+};
+template <typename T> struct Piece<T, true> {
+    static constexpr int N = 8;
+    using Raw = uint4;
+    using Packed = uint2;
+    __device__ static __forceinline__ Raw zero() { return make_uint4(0u, 0u, 0u, 0u); }
+    __device__ static __forceinline__ Raw load(const T* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ static __forceinline__ void store(T* p, const Raw& r) { *reinterpret_cast<uint4*>(p) = r; }
+    __device__ static __forceinline__ void decode(const Raw& r, float (&f)[8]) {
+        const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] = to_f32<T>(e[q]);
+    }
+    __device__ static __forceinline__ Raw encode(const float (&f)[8]) {
+        uint4 r;
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) e[q] = from_f32<T>(f[q]);
+        return r;
+    }
+    __device__ static __forceinline__ Packed load_packed(const uint8_t* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
+    __device__ static __forceinline__ void decode_packed(const Packed& r, float s, float (&f)[8]) {
+        const uint32_t h[2] = {r.x, r.y};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float2 a = e4m3_pair_values(static_cast<uint16_t>(h[q >> 1] >> (16 * (q & 1))));
+            f[2 * q] = unpacked<T>(a.x, s);
+            f[2 * q + 1] = unpacked<T>(a.y, s);
+        }
+    }
+    __device__ static __forceinline__ Packed encode_packed(const float (&f)[8]) {
+        return make_uint2(e4m3_pair(f[0], f[1]) | (static_cast<uint32_t>(e4m3_pair(f[2], f[3])) << 16),
+                          e4m3_pair(f[4], f[5]) | (static_cast<uint32_t>(e4m3_pair(f[6], f[7])) << 16));
+    }
+};
+
+// Largest magnitude of raw pieces as an unsigned number in the storage type's own bit pattern (two 16-bit lanes per
+// word: `join` folds them), which orders like the magnitude itself; at `not_finite` or above it an infinity or NaN was
+// among them.  One logic and one maximum instruction per word instead of a conversion per value.
+template <typename T> struct Magnitude;
+template <> struct Magnitude<float> {
+    static constexpr uint32_t not_finite = F32_INF_BITS;
+    __device__ static __forceinline__ uint32_t fold(uint32_t m, const float& v) { return max(m, __float_as_uint(v) & 0x7fffffffu); }
+    __device__ static __forceinline__ uint32_t fold(uint32_t m, const uint4& v) {
+        return max(max(max(m, v.x & 0x7fffffffu), v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+    }
+    __device__ static __forceinline__ uint32_t join(uint32_t m) { return m; }
+    __device__ static __forceinline__ uint32_t f32_bits(uint32_t m) { return m; }
+};
+template <typename T> struct Magnitude16 {
+    __device__ static __forceinline__ uint32_t fold(uint32_t m, const T& v) { return __vmaxu2(m, *reinterpret_cast<const uint16_t*>(&v) & 0x7fffu); }
+    __device__ static __forceinline__ uint32_t fold(uint32_t m, const uint4& v) {
+        m = __vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+        return __vmaxu2(m, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    }
+    __device__ static __forceinline__ uint32_t join(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+};
+template <> struct Magnitude<__nv_bfloat16> : Magnitude16<__nv_bfloat16> {
+    static constexpr uint32_t not_finite = 0x7f80u;
+    __device__ static __forceinline__ uint32_t f32_bits(uint32_t m) { return m << 16; }
+};
+template <> struct Magnitude<__half> : Magnitude16<__half> {
+    static constexpr uint32_t not_finite = 0x7c00u;
+    __device__ static __forceinline__ uint32_t f32_bits(uint32_t m) {
+        return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+    }
+};
+// Largest finite magnitude (fp32 bits) over the warp's pieces; `odd`: the warp holds an infinity or NaN somewhere.
+template <typename T, bool WIDE, int NV>
+__device__ __forceinline__ uint32_t warp_top(const typename Piece<T, WIDE>::Raw (&x)[NV], bool& odd) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) m = Magnitude<T>::fold(m, x[i]);
+    m = warp_max_u32(Magnitude<T>::join(m));
+    odd = m >= Magnitude<T>::not_finite;
+    if (!odd) return Magnitude<T>::f32_bits(m);
+    m = 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[Piece<T, WIDE>::N];
+        Piece<T, WIDE>::decode(x[i], f);
+#pragma unroll
+        for (int q = 0; q < Piece<T, WIDE>::N; ++q) m = max(m, finite_abs_bits(f[q]));
+    }
+    return warp_max_u32(m);
+}
+// a piece in 8 bits; infinities and NaN are looked for only where the warp has some
+template <typename T, bool WIDE>
+__device__ __forceinline__ typename Piece<T, WIDE>::Packed pack_piece(const typename Piece<T, WIDE>::Raw& x, float inv, bool odd) {
+    constexpr int N = Piece<T, WIDE>::N;
+    float f[N];
+    Piece<T, WIDE>::decode(x, f);
+    if (odd) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) f[q] = e4m3_operand(f[q], inv);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) f[q] *= inv;
+    }
+    return Piece<T, WIDE>::encode_packed(f);
+}
+
+// Sums of K values (a power of two) over the warp in K - 1 + 5 - log2(K) shuffles: each step halves the values a lane
+// carries.  On return lane k * (32 / K) (and its neighbours up to the next) holds the sum of v[k] as the result.
+template <int K>
+__device__ __forceinline__ float warp_sums(float (&v)[K]) {
+    const int lane = threadIdx.x & 31;
+    int o = 16;
+#pragma unroll
+    for (int half = K / 2; half >= 1; half >>= 1) {
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float give = up ? v[i] : v[i + half];
+            const float keep = up ? v[i + half] : v[i];
+            v[i] = keep + __shfl_xor_sync(FULL_MASK, give, o);
+        }
+        o >>= 1;
+    }
+    float r = v[0];
+#pragma unroll
+    for (; o > 0; o >>= 1) r += __shfl_xor_sync(FULL_MASK, r, o);
+    return r;
+}
+
+// barrier of one of several row groups of a block (ids 1 .. groups); one group: the block's
+__device__ __forceinline__ void group_sync(int group, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+}
+
+
+// ---------------------------------------------------------------------------
+// How a row is spread over threads: `warps` warps per row, `groups` rows' worth of warps per block, nv pieces per
+// thread, u_rows rows at a time per group.  warps == 0: the row is longer than MAX_ROW_WARPS warps take.
+// ---------------------------------------------------------------------------
+constexpr int MAX_ROW_WARPS = 16;
+constexpr int GRID_SMS = 148;
+struct RowShape { int warps, groups, nv, u_rows; };
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Many rows: nv_max pieces per thread, so that a row needs few warps and few exchanges between them.  Fewer than 1024
+// rows (under seven per SM): nv_min, a row is then spread wider and finished sooner.
+inline RowShape row_shape(int64_t rows, int64_t pieces, int nv_min, int nv_max, int block_warps, int u_max) {
+    RowShape s{};
+    s.nv = ((rows < 1024 && pieces <= 32 * MAX_ROW_WARPS * nv_min) || pieces <= 32 * nv_min) ? nv_min : nv_max;
+    const int64_t warps = (pieces + 32 * s.nv - 1) / (32 * s.nv);
+    if (warps > MAX_ROW_WARPS) return s;
+    s.warps = static_cast<int>(warps);
+    s.groups = block_warps / s.warps < 1 ? 1 : block_warps / s.warps;
+    const int64_t ru = (rows + GRID_SMS * s.groups - 1) / (GRID_SMS * s.groups);      // all u_max only when every SM gets some
+    s.u_rows = static_cast<int>(ru < 1 ? 1 : (ru > u_max ? u_max : ru));
+    return s;
+}
+
 }  // namespace peer

@@ -38,16 +38,113 @@ __global__ void __launch_bounds__(256) unpack_rows_loop_kernel(const uint8_t* __
     }
 }
 
+// A group of `warps` warps per row, the row in registers: read once.  Rows are independent, so a group takes one at a
+// time and the SM's other groups cover its exchange.
+template <typename T, bool WIDE, int NV, bool MULTI>
+__global__ void __launch_bounds__(512) pack_rows_kernel(const T* __restrict__ x, int64_t x_stride, int64_t rows, int64_t D,
+                                                        uint8_t* __restrict__ payload, float* __restrict__ scale, int warps) {
+    using P = Piece<T, WIDE>;
+    constexpr int N = P::N;
+    __shared__ uint32_t part[MULTI ? 2 * MAX_ROW_WARPS : 1];
+    const int lane = threadIdx.x & 31, threads = warps * 32;
+    const int group = MULTI ? threadIdx.x / threads : threadIdx.x >> 5;
+    const int gt = threadIdx.x - group * threads;
+    const int groups = blockDim.x / threads;
+    const int64_t pieces = D / N;
+    int parity = 0;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * groups + group; r < rows; r += static_cast<int64_t>(gridDim.x) * groups) {
+        typename P::Raw v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = gt + static_cast<int64_t>(i) * threads;
+            v[i] = c < pieces ? P::load(x + r * x_stride + c * N) : P::zero();
+        }
+        bool odd;
+        uint32_t top = warp_top<T, WIDE, NV>(v, odd);
+        if constexpr (MULTI) {
+            uint32_t* slot = part + parity * MAX_ROW_WARPS + group * warps;
+            if (lane == 0) slot[gt >> 5] = top;
+            group_sync(group, threads);
+            for (int k = 0; k < warps; ++k) top = max(top, slot[k]);
+            parity ^= 1;                                   // the next row's exchange leaves these slots alone
+        }
+        const int e = e4m3_scale_exponent(top);
+        const float inv = exp2_int(-e);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = gt + static_cast<int64_t>(i) * threads;
+            if (c < pieces) *reinterpret_cast<typename P::Packed*>(payload + r * D + c * N) = pack_piece<T, WIDE>(v[i], inv, odd);
+        }
+        if (gt == 0) scale[r] = exp2_int(e);
+    }
+}
+
+// One warp per segment of 8 * 32 pieces of a row.
+constexpr int SEGMENT = 8;
 template <typename T>
-cudaError_t pack_t(const void* x, int64_t x_stride, int64_t rows, int64_t D, uint8_t* payload, float* scale, cudaStream_t s) {
-    const unsigned grid = static_cast<unsigned>(rows < 148 * 64 ? rows : 148 * 64);
-    pack_rows_loop_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(x), x_stride, rows, D, payload, scale);
+__global__ void __launch_bounds__(256) unpack_rows_kernel(const uint8_t* __restrict__ payload, const float* __restrict__ scale,
+                                                          int64_t rows, int64_t D, int segments, T* __restrict__ out) {
+    using P = Piece<T, true>;
+    constexpr int N = P::N;
+    const int lane = threadIdx.x & 31;
+    const int64_t pieces = D / N, jobs = rows * segments;
+    const int64_t stride = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
+    for (int64_t j = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; j < jobs; j += stride) {
+        const int64_t r = segments == 1 ? j : j / segments;
+        const int64_t c0 = (j - r * segments) * SEGMENT * 32 + lane;
+        const float s = __ldg(scale + r);
+        typename P::Packed v[SEGMENT];
+#pragma unroll
+        for (int i = 0; i < SEGMENT; ++i)
+            if (c0 + i * 32 < pieces) v[i] = P::load_packed(payload + r * D + (c0 + i * 32) * N);
+#pragma unroll
+        for (int i = 0; i < SEGMENT; ++i)
+            if (c0 + i * 32 < pieces) {
+                float f[N];
+                P::decode_packed(v[i], s, f);
+                P::store(out + r * D + (c0 + i * 32) * N, P::encode(f));
+            }
+    }
+}
+
+template <typename T, bool WIDE, int NV>
+cudaError_t pack_launch(const T* x, int64_t x_stride, int64_t rows, int64_t D, uint8_t* payload, float* scale, const RowShape& h,
+                        cudaStream_t s) {
+    const int64_t need = (rows + h.groups - 1) / h.groups;
+    const unsigned grid = static_cast<unsigned>(need < GRID_SMS * 16 ? need : GRID_SMS * 16), threads = h.warps * h.groups * 32;
+    if (h.warps > 1) pack_rows_kernel<T, WIDE, NV, true><<<grid, threads, 0, s>>>(x, x_stride, rows, D, payload, scale, h.warps);
+    else pack_rows_kernel<T, WIDE, NV, false><<<grid, threads, 0, s>>>(x, x_stride, rows, D, payload, scale, h.warps);
     return cudaGetLastError();
 }
 
 template <typename T>
+cudaError_t pack_t(const void* xv, int64_t x_stride, int64_t rows, int64_t D, uint8_t* payload, float* scale, cudaStream_t s) {
+    constexpr int N = 16 / sizeof(T);
+    const T* x = static_cast<const T*>(xv);
+    const bool wide = D % N == 0 && x_stride % N == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(payload) & (N - 1)) == 0;
+    const RowShape h = wide ? row_shape(rows, D / N, 2, 8, 8, 1) : row_shape(rows, D, 4, 16, 8, 1);
+    if (h.warps == 0) {
+        const unsigned grid = static_cast<unsigned>(rows < GRID_SMS * 64 ? rows : GRID_SMS * 64);
+        pack_rows_loop_kernel<T><<<grid, 256, 0, s>>>(x, x_stride, rows, D, payload, scale);
+        return cudaGetLastError();
+    }
+    if (!wide) return h.nv == 4 ? pack_launch<T, false, 4>(x, x_stride, rows, D, payload, scale, h, s)
+                                : pack_launch<T, false, 16>(x, x_stride, rows, D, payload, scale, h, s);
+    return h.nv == 2 ? pack_launch<T, true, 2>(x, x_stride, rows, D, payload, scale, h, s)
+                     : pack_launch<T, true, 8>(x, x_stride, rows, D, payload, scale, h, s);
+}
+
+template <typename T>
 cudaError_t unpack_t(const uint8_t* payload, const float* scale, int64_t rows, int64_t D, void* out, cudaStream_t s) {
-    const unsigned grid = static_cast<unsigned>(rows < 148 * 64 ? rows : 148 * 64);
+    constexpr int N = 16 / sizeof(T);
+    if (D % N == 0 && aligned16(out) && (reinterpret_cast<uintptr_t>(payload) & (N - 1)) == 0) {
+        const int segments = static_cast<int>((D / N + SEGMENT * 32 - 1) / (SEGMENT * 32));
+        const int64_t blocks = (rows * segments + 7) / 8;
+        const unsigned grid = static_cast<unsigned>(blocks < GRID_SMS * 64 ? blocks : GRID_SMS * 64);
+        unpack_rows_kernel<T><<<grid, 256, 0, s>>>(payload, scale, rows, D, segments, static_cast<T*>(out));
+        return cudaGetLastError();
+    }
+    const unsigned grid = static_cast<unsigned>(rows < GRID_SMS * 64 ? rows : GRID_SMS * 64);
     unpack_rows_loop_kernel<T><<<grid, 256, 0, s>>>(payload, scale, rows, D, static_cast<T*>(out));
     return cudaGetLastError();
 }

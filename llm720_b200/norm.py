@@ -15,71 +15,81 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import as_rows, require_cuda, require_dtype, stream_of
+from ._rows import as_rows, launch, require_cuda, require_dtype
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def norm_forward(rows: torch.Tensor, weight, bias, eps: float, dt: int, pdt: int, stats: bool, pack: bool):
-    """(y, mean, rstd, payload, scale) of a row matrix; the last four as asked for, else None."""
+def norm_forward(x: torch.Tensor, weight, bias, eps: float, dt: int, pdt: int, keep: bool, pack: bool):
+    """(y, stats, payload, scale): y of x's shape; with ``keep`` the rows' means and 1/deviations as stats [2, rows],
+    with ``pack`` x in 8 bits, else None."""
+    rows = as_rows(x)
     R, D = rows.shape
-    dev = rows.device
-    y = torch.empty(R, D, dtype=rows.dtype, device=dev)
-    mean = rstd = payload = scale = None
-    if stats:
-        mean, rstd = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
+    dev = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = payload = scale = mean = rstd = None
+    if keep:
+        stats = torch.empty(2, R, dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * R
     if pack:
         payload = torch.empty(R, D, dtype=torch.float8_e4m3fn, device=dev)
         scale = torch.empty(R, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().peer_layer_norm(
-            rows.data_ptr(), rows.stride(0), dt, _ptr(weight), _ptr(bias), pdt, eps, R, D, y.data_ptr(), _ptr(mean), _ptr(rstd),
-            _ptr(payload), _ptr(scale), stream_of(dev)))
-    return y, mean, rstd, payload, scale
+    launch(_lib.load().peer_layer_norm, dev, rows.data_ptr(), rows.stride(0), dt, _ptr(weight), _ptr(bias), pdt, eps, R, D,
+           y.data_ptr(), mean, rstd, _ptr(payload), _ptr(scale))
+    return y, stats, payload, scale
 
 
-def norm_backward(grad_rows: torch.Tensor, rows, payload, scale, mean, rstd, weight, dt: int, pdt: int, want_x: bool,
-                  weight_dtype, bias_dtype, add: Optional[torch.Tensor] = None):
-    """(dx, dweight, dbias) of a row matrix; ``weight_dtype`` / ``bias_dtype`` None: that sum is not wanted.
-    ``add`` (contiguous rows) is added to dx before its rounding."""
+def norm_backward(grad_y: torch.Tensor, x, payload, scale, stats, weight, dt: int, pdt: int, want_x: bool, weight_dtype,
+                  bias_dtype, add: Optional[torch.Tensor] = None):
+    """(dx, dweight, dbias); ``weight_dtype`` / ``bias_dtype`` None: that sum is not wanted.  x or its packed form.
+    ``add`` (contiguous, of x's shape) is added to dx before its rounding."""
+    grad_rows = as_rows(grad_y)
     R, D = grad_rows.shape
-    dev = grad_rows.device
+    dev = grad_y.device
     lib = _lib.load()
-    dx = torch.empty(R, D, dtype=grad_rows.dtype, device=dev) if want_x else None
+    rows = None if x is None else as_rows(x)
+    dx = torch.empty(grad_y.shape, dtype=grad_y.dtype, device=dev) if want_x else None
     dw = None if weight_dtype is None else torch.empty(D, dtype=weight_dtype, device=dev)
     db = None if bias_dtype is None else torch.empty(D, dtype=bias_dtype, device=dev)
-    nbytes = lib.peer_layer_norm_workspace(R, D) if (dw is not None or db is not None) else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        _lib.check(lib.peer_layer_norm_backward(
-            grad_rows.data_ptr(), grad_rows.stride(0), _ptr(rows), 0 if rows is None else rows.stride(0), _ptr(payload),
-            _ptr(scale), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dt, pdt, _ptr(add), R, D, _ptr(dx), _ptr(dw), _ptr(db),
-            _ptr(ws), nbytes, stream_of(dev)))
+    ws, nbytes = None, 0
+    if dw is not None or db is not None:
+        nbytes = lib.peer_layer_norm_workspace(R, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    mean = stats.data_ptr()
+    launch(lib.peer_layer_norm_backward, dev, grad_rows.data_ptr(), grad_rows.stride(0), _ptr(rows),
+           0 if rows is None else rows.stride(0), _ptr(payload), _ptr(scale), mean, mean + 4 * R, _ptr(weight), dt, pdt, _ptr(add),
+           R, D, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
     return dx, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, checkpoint, dt, pdt):
-        rows = as_rows(x)
         packed = checkpoint == "e4m3"
-        y, mean, rstd, payload, scale = norm_forward(rows, weight, bias, eps, dt, pdt, True, packed)
-        ctx.save_for_backward(None if packed else x, weight, payload, scale, mean, rstd)
+        y, stats, payload, scale = norm_forward(x, weight, bias, eps, dt, pdt, True, packed)
+        ctx.save_for_backward(None if packed else x, weight, payload, scale, stats)
         ctx.codes = (dt, pdt)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y.view(x.shape)
+        ctx.param_dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
-        x, weight, payload, scale, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = norm_backward(as_rows(grad_y), None if x is None else as_rows(x), payload, scale, mean, rstd, weight,
-                                   *ctx.codes, need[0], weight.dtype if need[1] else None,
-                                   ctx.bias_dtype if need[2] else None)
-        return None if dx is None else dx.view(grad_y.shape), dw, db, None, None, None, None
+        return _norm_grad_once(ctx, grad_y) if torch.is_grad_enabled() else _norm_grad(ctx, grad_y)
+
+
+def _norm_grad(ctx, grad_y):
+    x, weight, payload, scale, stats = ctx.saved_tensors
+    want_x, want_w, want_b = ctx.needs_input_grad[:3]
+    wdt, bdt = ctx.param_dtypes
+    dx, dw, db = norm_backward(grad_y, x, payload, scale, stats, weight, *ctx.codes, want_x, wdt if want_w else None,
+                               bdt if want_b else None)
+    return dx, dw, db, None, None, None, None
+
+
+_norm_grad_once = once_differentiable(_norm_grad)     # create_graph=True: a second derivative raises
 
 
 def check_norm_arguments(x, weight, bias, eps):
@@ -121,4 +131,4 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, checkpoint, dt, pdt)
-    return norm_forward(as_rows(x), weight, bias, eps, dt, pdt, False, False)[0].view(x.shape)
+    return norm_forward(x, weight, bias, eps, dt, pdt, False, False)[0]

@@ -14,17 +14,15 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import as_rows, require_cuda, require_dtype, stream_of
+from ._rows import as_rows, launch, require_cuda, require_dtype
 
 _MAX_ROWS = 2**31 - 2
 
 
 def _lookup(ids, weight, scale, dropped, dt):
     out = torch.empty(ids.shape + weight.shape[1:], dtype=weight.dtype, device=weight.device)
-    with torch.cuda.device(weight.device):
-        _lib.check(_lib.load().peer_embedding(
-            ids.data_ptr(), ids.element_size(), ids.numel(), weight.data_ptr(), dt, weight.shape[0], weight.shape[1], scale,
-            out.data_ptr(), None if dropped is None else dropped.data_ptr(), stream_of(weight.device)))
+    launch(_lib.load().peer_embedding, weight.device, ids.data_ptr(), ids.element_size(), ids.numel(), weight.data_ptr(), dt,
+           *weight.shape, scale, out.data_ptr(), None if dropped is None else dropped.data_ptr())
     return out
 
 
@@ -36,21 +34,26 @@ class _Embedding(torch.autograd.Function):
         return _lookup(ids, weight, scale, dropped, dt)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
-        ids, = ctx.saved_tensors
-        scale, padding_idx, dt, (V, D) = ctx.args
-        rows = as_rows(grad_out)
-        dev = grad_out.device
-        lib = _lib.load()
-        grad = torch.empty(V, D, dtype=grad_out.dtype, device=dev)
-        nbytes = lib.peer_embedding_workspace(ids.numel(), D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(lib.peer_embedding_backward(
-                ids.data_ptr(), ids.element_size(), ids.numel(), rows.data_ptr(), rows.stride(0), dt, V, D, scale,
-                -1 if padding_idx is None else padding_idx, grad.data_ptr(), ws.data_ptr(), nbytes, stream_of(dev)))
-        return grad, None, None, None, None, None
+        return _embedding_grad_once(ctx, grad_out) if torch.is_grad_enabled() else _embedding_grad(ctx, grad_out)
+
+
+def _embedding_grad(ctx, grad_out):
+    ids, = ctx.saved_tensors
+    scale, padding_idx, dt, (V, D) = ctx.args
+    rows = as_rows(grad_out)
+    dev = grad_out.device
+    lib = _lib.load()
+    n = ids.numel()
+    grad = torch.empty(V, D, dtype=grad_out.dtype, device=dev)
+    nbytes = lib.peer_embedding_workspace(n, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    launch(lib.peer_embedding_backward, dev, ids.data_ptr(), ids.element_size(), n, rows.data_ptr(), rows.stride(0), dt, V, D,
+           scale, -1 if padding_idx is None else padding_idx, grad.data_ptr(), ws.data_ptr(), nbytes)
+    return grad, None, None, None, None, None
+
+
+_embedding_grad_once = once_differentiable(_embedding_grad)     # create_graph=True: a second derivative raises
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, padding_idx: Optional[int] = None,

@@ -156,135 +156,126 @@ __device__ __forceinline__ void load_params(const void* p, bool f32, int64_t D, 
     }
 }
 
-template <typename T, bool WIDE, int NV, int U, bool MULTI, bool PACK>
-__global__ void __launch_bounds__(512) norm_kernel(const NormParams p, int warps, int ru) {
+template <typename T, int N>
+__device__ __forceinline__ void load_param_piece(const void* p, bool f32, int64_t c, float (&f)[N]) {
+    if constexpr (N == 1) {
+        f[0] = param_at<T>(p, f32, c);
+    } else if (f32) {
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + q));
+            f[q] = v.x; f[q + 1] = v.y; f[q + 2] = v.z; f[q + 3] = v.w;
+        }
+    } else {
+        Piece<T, true>::decode(Piece<T, true>::load(static_cast<const T*>(p) + c), f);
+    }
+}
+
+// Forward.  A row per group and at most 64 values per thread: with 2048 bf16 values a warp has its row to itself and
+// there is no exchange; the parameters come from L1.
+template <typename T, bool WIDE, int NV, bool MULTI, bool PACK>
+__global__ void __launch_bounds__(512, 2) norm_kernel(const NormParams p, int warps) {
     using P = Piece<T, WIDE>;
-    constexpr int N = P::N, E = NV * N;
-    __shared__ float2 part[MULTI ? 2 * MAX_WARPS * U : 1];
-    __shared__ uint32_t part_top[MULTI && PACK ? 2 * MAX_WARPS * U : 1];
+    constexpr int N = P::N;
+    __shared__ float2 part[MULTI ? 2 * MAX_WARPS : 1];
+    __shared__ uint32_t part_top[MULTI && PACK ? 2 * MAX_WARPS : 1];
     const int lane = threadIdx.x & 31, threads = warps * 32;
     const int group = MULTI ? threadIdx.x / threads : threadIdx.x >> 5;
     const int gt = threadIdx.x - group * threads, gw = gt >> 5;
     const int groups = blockDim.x / threads;
-    const int64_t pieces = p.D / N;
-    float w[E], b[E];
-    load_params<T, NV, N>(p.w, p.param_f32, p.D, gt, threads, 1.f, w);
-    load_params<T, NV, N>(p.b, p.param_f32, p.D, gt, threads, 0.f, b);
+    const int pieces = static_cast<int>(p.D / N);
     auto columns_of = [&](int wi) {                        // columns held by warp wi of the group
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t left = pieces - (static_cast<int64_t>(i) * threads + wi * 32);
-            n += static_cast<int>(left < 0 ? 0 : (left > 32 ? 32 : left)) * N;
-        }
-        return static_cast<float>(n);
+        for (int i = 0; i < NV; ++i) n += min(max(pieces - (i * threads + wi * 32), 0), 32);
+        return static_cast<float>(n * N);
     };
     const float mine = columns_of(gw), inv_mine = mine > 0.f ? 1.f / mine : 0.f;
     const float inv_d = 1.f / static_cast<float>(p.D);
     int parity = 0;
-    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * groups + group) * ru; r0 < p.rows;
-         r0 += static_cast<int64_t>(gridDim.x) * groups * ru) {
-        typename P::Raw x[U][NV];
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * groups + group; r < p.rows; r += static_cast<int64_t>(gridDim.x) * groups) {
+        const T* xr = static_cast<const T*>(p.x) + r * p.x_stride;
+        typename P::Raw x[NV];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int i = 0; i < NV; ++i) {
+            const int c = gt + i * threads;
+            x[i] = c < pieces ? P::load(xr + c * N) : P::zero();
+        }
+        float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int64_t c = gt + static_cast<int64_t>(i) * threads;
-                const bool in = u < ru && r0 + u < p.rows && c < pieces;
-                x[u][i] = in ? P::load(static_cast<const T*>(p.x) + (r0 + u) * p.x_stride + c * N) : P::zero();
-            }
-        float s[U], mean[U], rstd[U];
-        uint32_t top[U];
-        bool odd[U];                                        // the warp holds an infinity or NaN of row u
+        for (int i = 0; i < NV; ++i) {
+            float f[N];
+            P::decode(x[i], f);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = 0.f;
+            for (int q = 0; q < N; ++q) s += f[q];
+        }
+        bool odd = false;                                   // the warp holds an infinity or NaN of this row
+        uint32_t top = 0u;
+        if (PACK) top = warp_top<T, WIDE, NV>(x, odd);
+        float mean = warp_sum(s) * inv_mine, m2 = 0.f;      // of the warp's columns
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < NV; ++i) {
+            if (gt + i * threads < pieces) {
                 float f[N];
-                P::decode(x[u][i], f);
+                P::decode(x[i], f);
 #pragma unroll
-                for (int q = 0; q < N; ++q) s[u] += f[q];
-            }
-            if (PACK) top[u] = warp_top<T, WIDE, NV>(x[u], odd[u]);
-        }
-        const float wm = warp_sums<U>(s) * inv_mine;        // lane u * (32 / U): this warp's mean of row u
-        float m2[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            mean[u] = __shfl_sync(FULL_MASK, wm, u * (32 / U));
-            m2[u] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (gt + static_cast<int64_t>(i) * threads < pieces) {
-                    float f[N];
-                    P::decode(x[u][i], f);
-#pragma unroll
-                    for (int q = 0; q < N; ++q) { const float d = f[q] - mean[u]; m2[u] = fmaf(d, d, m2[u]); }
-                }
+                for (int q = 0; q < N; ++q) { const float d = f[q] - mean; m2 = fmaf(d, d, m2); }
             }
         }
-        const float wm2 = warp_sums<U>(m2);
-        if constexpr (!MULTI) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) rstd[u] = 1.f / sqrtf(__shfl_sync(FULL_MASK, wm2, u * (32 / U)) * inv_d + p.eps);
-        } else {
-            float2* slot = part + parity * MAX_WARPS * U + group * warps * U;
-            uint32_t* slot_top = part_top + (PACK ? parity * MAX_WARPS * U + group * warps * U : 0);
-            if (lane % (32 / U) == 0) slot[gw * U + lane / (32 / U)] = make_float2(wm, wm2);
-            if (PACK && lane == 0) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) slot_top[gw * U + u] = top[u];
+        m2 = warp_sum(m2);
+        if constexpr (MULTI) {
+            float2* slot = part + parity * MAX_WARPS + group * warps;
+            uint32_t* slot_top = part_top + (PACK ? parity * MAX_WARPS + group * warps : 0);
+            if (lane == 0) {
+                slot[gw] = make_float2(mean, m2);
+                if (PACK) slot_top[gw] = top;
             }
             group_sync(group, threads);
-#pragma unroll
-            for (int u = 0; u < U; ++u) mean[u] = 0.f;
+            mean = 0.f;
             for (int k = 0; k < warps; ++k) {
-                const float n = columns_of(k);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    mean[u] = fmaf(n, slot[k * U + u].x, mean[u]);
-                    if (PACK) top[u] = max(top[u], slot_top[k * U + u]);
-                }
+                mean = fmaf(columns_of(k), slot[k].x, mean);
+                if (PACK) top = max(top, slot_top[k]);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) { mean[u] *= inv_d; m2[u] = 0.f; }
+            mean *= inv_d;
+            m2 = 0.f;
             for (int k = 0; k < warps; ++k) {
-                const float n = columns_of(k);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float2 v = slot[k * U + u];
-                    const float d = v.x - mean[u];
-                    m2[u] += fmaf(n * d, d, v.y);
-                }
+                const float2 v = slot[k];
+                const float d = v.x - mean;
+                m2 += fmaf(columns_of(k) * d, d, v.y);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) rstd[u] = 1.f / sqrtf(m2[u] * inv_d + p.eps);
-            parity ^= 1;                                    // the next rows' exchange leaves these slots alone
+            parity ^= 1;                                    // the next row's exchange leaves these slots alone
         }
+        const float rstd = 1.f / sqrtf(m2 * inv_d + p.eps);
+        const int e = PACK ? e4m3_scale_exponent(top) : 0;
+        const float inv = exp2_int(-e);
+        T* yr = static_cast<T*>(p.y) + r * p.D;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t r = r0 + u;
-            if (u >= ru || r >= p.rows) break;
-            const int e = PACK ? e4m3_scale_exponent(top[u]) : 0;
-            const float inv = exp2_int(-e);
+        for (int i = 0; i < NV; ++i) {
+            const int c = gt + i * threads;
+            if (c < pieces) {
+                float f[N], v[N];
+                P::decode(x[i], f);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int64_t c = gt + static_cast<int64_t>(i) * threads;
-                if (c >= pieces) break;
-                float f[N], y[N];
-                P::decode(x[u][i], f);
+                for (int q = 0; q < N; ++q) f[q] = (f[q] - mean) * rstd;
+                if (p.w) {
+                    load_param_piece<T, N>(p.w, p.param_f32, c * N, v);
 #pragma unroll
-                for (int q = 0; q < N; ++q) y[q] = fmaf((f[q] - mean[u]) * rstd[u], w[i * N + q], b[i * N + q]);
-                P::store(static_cast<T*>(p.y) + r * p.D + c * N, P::encode(y));
+                    for (int q = 0; q < N; ++q) f[q] *= v[q];
+                }
+                if (p.b) {
+                    load_param_piece<T, N>(p.b, p.param_f32, c * N, v);
+#pragma unroll
+                    for (int q = 0; q < N; ++q) f[q] += v[q];
+                }
+                P::store(yr + c * N, P::encode(f));
                 if constexpr (PACK)
-                    *reinterpret_cast<typename P::Packed*>(p.payload + r * p.D + c * N) = pack_piece<T, WIDE>(x[u][i], inv, odd[u]);
+                    *reinterpret_cast<typename P::Packed*>(p.payload + r * p.D + c * N) = pack_piece<T, WIDE>(x[i], inv, odd);
             }
-            if (gt == 0) {
-                if (p.mean) p.mean[r] = mean[u];
-                if (p.rstd) p.rstd[r] = rstd[u];
-                if (PACK) p.scale[r] = exp2_int(e);
-            }
+        }
+        if (gt == 0) {
+            if (p.mean) p.mean[r] = mean;
+            if (p.rstd) p.rstd[r] = rstd;
+            if (PACK) p.scale[r] = exp2_int(e);
         }
     }
 }
@@ -434,28 +425,408 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
     }
 }
 
-// `splits` partial rows to the gradients: 32 columns by 8 lanes of partials per block
+// ---------------------------------------------------------------------------
+// ---------------------------------------------------------------------------
+// Many rows of whole 16-byte pieces.  A group of warps owns a row, 16 columns per thread, the same columns in every row,
+// so parameters and column sums stay in registers.  Every thread copies its own pieces of the group's next rows into
+// shared memory (cp.async) while it works on the current one; nobody else reads them, so the ring needs no barrier and
+// no registers, and what is left in a row's chain is one exchange between the group's warps.
+// With the loads covered the instruction count decides: values are decoded once, kept as fp32 pairs across the exchange
+// and go through the packed fp32 instructions, two columns each.  W > 0: the row is exactly W full warps (512 W
+// columns), which turns the addresses of a thread's pieces and the exchange into constants; W == 0 takes any other
+// width.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float2 splat(float a) { return make_float2(a, a); }
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
+// 1/sqrt(v): the hardware estimate and one Newton step (relative error below 2^-23); 0, infinite and NaN pass through
+__device__ __forceinline__ float inverse_sqrt(float v) {
+    const float r = rsqrtf(v);
+    return (v > 0.f && v < __uint_as_float(F32_INF_BITS)) ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+}
+
+constexpr int RING_COLUMNS = 16, RING_THREADS = 512;      // columns per thread; one block per SM
+
+template <typename T, int NV, int N>
+__device__ __forceinline__ void load_param_pairs(const void* p, bool f32, const bool (&in)[NV], int gt, int threads, float absent,
+                                                 float2 (&out)[NV][N / 2]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) f[q] = absent;
+        if (p && in[i]) load_param_piece<T, N>(p, f32, (gt + i * threads) * N, f);
+#pragma unroll
+        for (int h = 0; h < N / 2; ++h) out[i][h] = make_float2(f[2 * h], f[2 * h + 1]);
+    }
+}
+
+// 16, 8 or 4 bytes of this thread's shared memory
+template <typename V> __device__ __forceinline__ V shared_at(uint32_t at);
+template <> __device__ __forceinline__ uint4 shared_at<uint4>(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+template <> __device__ __forceinline__ uint2 shared_at<uint2>(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+template <> __device__ __forceinline__ uint32_t shared_at<uint32_t>(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <typename T, int W, bool PACK, int STAGES>
+__global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormParams p, int row_warps) {
+    using P = Piece<T, true>;
+    constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2;
+    constexpr int STAGE = NV * RING_THREADS * 16;           // bytes: [piece][thread]
+    extern __shared__ __align__(16) unsigned char ring_smem[];
+    __shared__ float2 part[2 * MAX_WARPS];
+    __shared__ uint32_t part_top[2 * MAX_WARPS];
+    __shared__ float held[MAX_WARPS];                       // columns of each of the group's warps
+    const int warps = W ? W : row_warps;
+    const int lane = threadIdx.x & 31, threads = warps * 32;
+    const int group = threadIdx.x / threads, gt = threadIdx.x - group * threads, gw = gt >> 5;
+    const int groups = blockDim.x / threads;
+    bool in[NV];
+    int mine = 0;
+    {
+        const int pieces = static_cast<int>(p.D / N);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            in[i] = W || gt + i * threads < pieces;
+            mine += min(max(pieces - (i * threads + gw * 32), 0), 32) * N;
+        }
+    }
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * groups + group, step = static_cast<int64_t>(gridDim.x) * groups;
+    int rows = first < p.rows ? static_cast<int>((p.rows - first + step - 1) / step) : 0;      // of this group
+    int to_fetch = rows;
+    const T* src = static_cast<const T*>(p.x) + first * p.x_stride + gt * N;      // this thread's pieces of the row fetched next
+    const int64_t src_step = step * p.x_stride;
+    const uint32_t slot0 = smem_u32(ring_smem) + threadIdx.x * 16, slot_end = slot0 + STAGES * STAGE;
+    uint32_t slot = slot0, fetch_slot = slot0;
+    auto fetch = [&]() {
+        if (to_fetch > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (in[i]) copy_async<16>(fetch_slot + i * RING_THREADS * 16, src + i * threads * N);
+        }
+        src += src_step;
+        --to_fetch;
+        fetch_slot += STAGE;
+        if (fetch_slot == slot_end) fetch_slot = slot0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    float2 w[NV][H], b[NV][H];                              // loaded while the first rows are on their way
+    load_param_pairs<T, NV, N>(p.w, p.param_f32, in, gt, threads, 1.f, w);
+    load_param_pairs<T, NV, N>(p.b, p.param_f32, in, gt, threads, 0.f, b);
+    if (group == 0 && lane == 0) held[gw] = static_cast<float>(mine);
+    __syncthreads();
+    const float inv_mine = mine > 0 ? 1.f / static_cast<float>(mine) : 0.f, inv_d = 1.f / static_cast<float>(p.D);
+    T* dst = static_cast<T*>(p.y) + first * p.D + gt * N;
+    uint8_t* dst8 = p.payload + first * p.D + gt * N;
+    const int64_t dst_step = step * p.D;
+    int64_t r = first;
+    int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
+    for (; rows > 0; --rows) {
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        typename P::Raw raw[NV];
+        float2 x[NV][H], s2 = splat(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            raw[i] = in[i] ? shared_at<uint4>(slot + i * RING_THREADS * 16) : P::zero();
+            float f[N];
+            P::decode(raw[i], f);
+#pragma unroll
+            for (int h = 0; h < H; ++h) { x[i][h] = make_float2(f[2 * h], f[2 * h + 1]); s2 = __fadd2_rn(s2, x[i][h]); }
+        }
+        slot += STAGE;
+        if (slot == slot_end) slot = slot0;
+        bool odd = false;
+        uint32_t top = 0u;
+        if (PACK) top = warp_top<T, true, NV>(raw, odd);
+        float mean = warp_sum(s2.x + s2.y) * inv_mine;
+        const float2 neg = splat(-mean);
+        s2 = splat(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (in[i]) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) { const float2 d = __fadd2_rn(x[i][h], neg); s2 = __ffma2_rn(d, d, s2); }
+            }
+        float m2 = warp_sum(s2.x + s2.y);
+        if (warps > 1) {
+            if (lane == 0) {
+                part[exchange + gw] = make_float2(mean, m2);
+                if (PACK) part_top[exchange + gw] = top;
+            }
+            group_sync(group, threads);
+            mean = 0.f;
+#pragma unroll
+            for (int k = 0; k < (W ? W : warps); ++k) {
+                mean = fmaf(W ? 1.f : held[k], part[exchange + k].x, mean);
+                if (PACK) top = max(top, part_top[exchange + k]);
+            }
+            mean *= W ? 1.f / (W ? W : 1) : inv_d;
+            m2 = 0.f;
+#pragma unroll
+            for (int k = 0; k < (W ? W : warps); ++k) {
+                const float2 v = part[exchange + k];
+                const float d = v.x - mean;
+                m2 += fmaf((W ? 32.f * RING_COLUMNS : held[k]) * d, d, v.y);
+            }
+            exchange += other;
+            other = -other;
+        }
+        const float rstd = inverse_sqrt(m2 * inv_d + p.eps);
+        const float2 r2 = splat(rstd), c2 = splat(-mean * rstd);
+        const int e = PACK ? e4m3_scale_exponent(top) : 0;
+        const float inv = exp2_int(-e);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (in[i]) {
+                float f[N];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const float2 v = __ffma2_rn(__ffma2_rn(x[i][h], r2, c2), w[i][h], b[i][h]);
+                    f[2 * h] = v.x;
+                    f[2 * h + 1] = v.y;
+                }
+                P::store(dst + i * threads * N, P::encode(f));
+                if constexpr (PACK)
+                    *reinterpret_cast<typename P::Packed*>(dst8 + i * threads * N) = pack_piece<T, true>(raw[i], inv, odd);
+            }
+        dst += dst_step;
+        if (PACK) dst8 += dst_step;
+        if (gt == 0) {
+            if (p.mean) p.mean[r] = mean;
+            if (p.rstd) p.rstd[r] = rstd;
+            if (PACK) p.scale[r] = exp2_int(e);
+        }
+        r += step;
+    }
+}
+
+template <typename T, int W, bool KEPT, int STAGES>
+__global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const NormGradParams p, int row_warps) {
+    using P = Piece<T, true>;
+    using X = typename std::conditional<KEPT, typename P::Packed, uint4>::type;
+    constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2, XB = static_cast<int>(sizeof(X));
+    // bytes of a stage: dy [piece][thread], x [piece][thread], {mean, 1/deviation, scale, -} [warp]
+    constexpr int X_AT = NV * RING_THREADS * 16, STAT_AT = X_AT + NV * RING_THREADS * XB, STAGE = STAT_AT + (RING_THREADS / 32) * 16;
+    extern __shared__ __align__(16) unsigned char ring_smem[];
+    __shared__ float2 part[2 * MAX_WARPS];
+    const int warps = W ? W : row_warps;
+    const int lane = threadIdx.x & 31, threads = warps * 32;
+    const int group = threadIdx.x / threads, gt = threadIdx.x - group * threads, gw = gt >> 5;
+    const int groups = blockDim.x / threads;
+    bool in[NV];
+    {
+        const int pieces = static_cast<int>(p.D / N);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) in[i] = W || gt + i * threads < pieces;
+    }
+    const float inv_d = 1.f / static_cast<float>(p.D);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * groups + group, step = static_cast<int64_t>(gridDim.x) * groups;
+    int rows = first < p.rows ? static_cast<int>((p.rows - first + step - 1) / step) : 0;      // of this group
+    int to_fetch = rows;
+    const T* src_dy = static_cast<const T*>(p.dy) + first * p.dy_stride + gt * N;
+    const T* src_x = static_cast<const T*>(p.x) + first * p.x_stride + gt * N;
+    const uint8_t* src_8 = p.payload + first * p.D + gt * N;
+    // lanes 0, 1 and (KEPT) 2 of every warp bring the row's mean, 1/deviation and scale into the warp's own slots
+    const float* src_stat = (lane == 0 ? p.mean : lane == 1 ? p.rstd : p.scale) + first;
+    const bool brings = lane < (KEPT ? 3 : 2);
+    const int64_t dy_step = step * p.dy_stride, x_step = step * (KEPT ? p.D : p.x_stride);
+    const uint32_t base = smem_u32(ring_smem);
+    const int dy_at = threadIdx.x * 16, x_at = X_AT + threadIdx.x * XB, stat_at = STAT_AT + (threadIdx.x >> 5) * 16;
+    uint32_t slot = base, fetch_slot = base;
+    auto fetch = [&]() {
+        if (to_fetch > 0) {
+            if (brings) copy_async<4>(fetch_slot + stat_at + lane * 4, src_stat);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (in[i]) {
+                    copy_async<16>(fetch_slot + dy_at + i * RING_THREADS * 16, src_dy + i * threads * N);
+                    if constexpr (KEPT) copy_async<XB>(fetch_slot + x_at + i * RING_THREADS * XB, src_8 + i * threads * N);
+                    else copy_async<16>(fetch_slot + x_at + i * RING_THREADS * XB, src_x + i * threads * N);
+                }
+        }
+        src_dy += dy_step;
+        if constexpr (KEPT) src_8 += x_step; else src_x += x_step;
+        src_stat += step;
+        --to_fetch;
+        fetch_slot += STAGE;
+        if (fetch_slot == base + STAGES * STAGE) fetch_slot = base;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    float2 w[NV][H], aw[NV][H], ab[NV][H];                  // w loaded while the first rows are on their way
+    load_param_pairs<T, NV, N>(p.w, p.param_f32, in, gt, threads, 1.f, w);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int h = 0; h < H; ++h) aw[i][h] = ab[i][h] = splat(0.f);
+    T* dst = static_cast<T*>(p.dx) + first * p.D + gt * N;
+    const T* add = static_cast<const T*>(p.add) + first * p.D + gt * N;
+    const int64_t dst_step = step * p.D;
+    int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
+    for (; rows > 0; --rows) {
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();                                       // the row's statistics came by other lanes
+        float mean, rstd, sc;
+        {
+            const uint4 v = shared_at<uint4>(slot + stat_at);
+            mean = __uint_as_float(v.x);
+            rstd = __uint_as_float(v.y);
+            sc = __uint_as_float(v.z);
+        }
+        const float2 r2 = splat(rstd), c2 = splat(-mean * rstd);
+        float2 n[NV][H], g[NV][H], s1 = splat(0.f), s2 = splat(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const X xr = in[i] ? shared_at<X>(slot + x_at + i * RING_THREADS * XB) : X{};
+            const uint4 dr = in[i] ? shared_at<uint4>(slot + dy_at + i * RING_THREADS * 16) : P::zero();
+            float f[N], d[N];
+            if constexpr (KEPT) P::decode_packed(xr, sc, f); else P::decode(xr, f);
+            P::decode(dr, d);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const float2 dv = make_float2(d[2 * h], d[2 * h + 1]);
+                n[i][h] = __ffma2_rn(make_float2(f[2 * h], f[2 * h + 1]), r2, c2);
+                g[i][h] = __fmul2_rn(dv, w[i][h]);
+                s1 = __fadd2_rn(s1, g[i][h]);
+                s2 = __ffma2_rn(g[i][h], n[i][h], s2);
+                aw[i][h] = __ffma2_rn(dv, n[i][h], aw[i][h]);
+                ab[i][h] = __fadd2_rn(ab[i][h], dv);
+            }
+        }
+        slot += STAGE;
+        if (slot == base + STAGES * STAGE) slot = base;
+        if (p.dx) {
+            float s[2] = {s1.x + s1.y, s2.x + s2.y};
+            const float total = warp_sums<2>(s);            // lane 0: the first sum, lane 16: the second
+            float m1 = 0.f, m2 = 0.f;
+            if (warps == 1) {
+                m1 = __shfl_sync(FULL_MASK, total, 0);
+                m2 = __shfl_sync(FULL_MASK, total, 16);
+            } else {
+                if ((lane & 15) == 0) reinterpret_cast<float*>(part + exchange + gw)[lane >> 4] = total;
+                group_sync(group, threads);
+#pragma unroll
+                for (int k = 0; k < (W ? W : warps); ++k) {
+                    const float2 v = part[exchange + k];
+                    m1 += v.x;
+                    m2 += v.y;
+                }
+                exchange += other;
+                other = -other;
+            }
+            const float scaled = -inv_d * rstd;
+            const float2 m1p = splat(m1 * scaled), m2p = splat(m2 * scaled);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (in[i]) {
+                    float f[N];
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const float2 v = __ffma2_rn(g[i][h], r2, __ffma2_rn(n[i][h], m2p, m1p));
+                        f[2 * h] = v.x;
+                        f[2 * h + 1] = v.y;
+                    }
+                    if (p.add) {
+                        float o[N];
+                        P::decode(P::load(add + i * threads * N), o);
+#pragma unroll
+                        for (int q = 0; q < N; ++q) f[q] += o[q];
+                    }
+                    P::store(dst + i * threads * N, P::encode(f));
+                }
+            dst += dst_step;
+            add += dst_step;
+        }
+        __syncwarp();                                       // before a fetch overwrites a slot another lane may still read
+    }
+    if (!p.dw && !p.db) return;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                        // the ring is free: the groups add up in order through it
+    float2* columns = reinterpret_cast<float2*>(ring_smem);      // [2 * NV * H][threads]
+    for (int q = 0; q + 1 < groups; ++q) {
+        if (group == q) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    columns[(i * H + h) * threads + gt] = aw[i][h];
+                    columns[((NV + i) * H + h) * threads + gt] = ab[i][h];
+                }
+        }
+        __syncthreads();
+        if (group == q + 1) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    aw[i][h] = __fadd2_rn(aw[i][h], columns[(i * H + h) * threads + gt]);
+                    ab[i][h] = __fadd2_rn(ab[i][h], columns[((NV + i) * H + h) * threads + gt]);
+                }
+        }
+        __syncthreads();
+    }
+    if (group == groups - 1) {
+        float* out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.D;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (in[i]) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const int c = (gt + i * threads) * N + 2 * h;
+                    *reinterpret_cast<float2*>(out + c) = aw[i][h];
+                    *reinterpret_cast<float2*>(out + p.D + c) = ab[i][h];
+                }
+            }
+    }
+}
+
+// `splits` partial rows to the gradients: 32 columns by 32 lanes of partials per block, so that a lane's few loads are
+// all in flight at once
+constexpr int JOIN_LANES = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormGradParams p) {
-    __shared__ float sw[8][33], sb[8][33];
+__global__ void __launch_bounds__(32 * JOIN_LANES) norm_grad_join_kernel(const NormGradParams p) {
+    __shared__ float sw[JOIN_LANES][33], sb[JOIN_LANES][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
     float aw = 0.f, ab = 0.f;
     if (c < p.D) {
-#pragma unroll 4
-        for (int i = ty; i < p.splits; i += 8) {
-            aw += p.partial[static_cast<int64_t>(i) * 2 * p.D + c];
-            ab += p.partial[(static_cast<int64_t>(i) * 2 + 1) * p.D + c];
+#pragma unroll
+        for (int k = 0; k < (GRID_SMS + JOIN_LANES - 1) / JOIN_LANES; ++k) {
+            const int i = ty + k * JOIN_LANES;
+            if (i < p.splits) {
+                aw += p.partial[static_cast<int64_t>(i) * 2 * p.D + c];
+                ab += p.partial[(static_cast<int64_t>(i) * 2 + 1) * p.D + c];
+            }
         }
     }
     sw[ty][tx] = aw;
     sb[ty][tx] = ab;
     __syncthreads();
-    if (ty != 0 || c >= p.D) return;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) { aw += sw[i][tx]; ab += sb[i][tx]; }
-    if (p.dw) { if (p.param_f32) static_cast<float*>(p.dw)[c] = aw; else static_cast<T*>(p.dw)[c] = from_f32<T>(aw); }
-    if (p.db) { if (p.param_f32) static_cast<float*>(p.db)[c] = ab; else static_cast<T*>(p.db)[c] = from_f32<T>(ab); }
+    // warp ty finishes column ty: lane tx holds the partial sum of lane row tx
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + ty;
+    aw = warp_sum(sw[tx][ty]);
+    ab = warp_sum(sb[tx][ty]);
+    if (tx != 0 || col >= p.D) return;
+    if (p.dw) { if (p.param_f32) static_cast<float*>(p.dw)[col] = aw; else static_cast<T*>(p.dw)[col] = from_f32<T>(aw); }
+    if (p.db) { if (p.param_f32) static_cast<float*>(p.db)[col] = ab; else static_cast<T*>(p.db)[col] = from_f32<T>(ab); }
 }
 
 constexpr int MAX_SPLITS = GRID_SMS;       // one block per SM: rows of partial column sums
@@ -467,28 +838,68 @@ int splits_for(int64_t rows) {
 
 unsigned row_blocks(int64_t rows) { return static_cast<unsigned>(rows < 148 * 64 ? rows : 148 * 64); }
 
-template <typename T, bool WIDE, int NV, int U, bool PACK>
+constexpr int64_t RING_ROWS = 1024;   // below, a block sees too few rows for a ring to run ahead
+
+// the width a ring kernel is built for: W full warps when the row is exactly that, else 0
+inline int ring_width(int64_t D) {
+    for (int w = 1; w <= MAX_WARPS; w *= 2)
+        if (D == static_cast<int64_t>(w) * 32 * RING_COLUMNS) return w;
+    return 0;
+}
+inline int ring_warps(int64_t D) { return static_cast<int>((D + 32 * RING_COLUMNS - 1) / (32 * RING_COLUMNS)); }
+
+template <typename T, int W, bool PACK>
+cudaError_t norm_ring_width(const NormParams& p, cudaStream_t s) {
+    constexpr int STAGES = sizeof(T) == 4 ? 4 : 6;           // 128 KB, 96 KB
+    constexpr int SMEM = STAGES * RING_THREADS * RING_COLUMNS * static_cast<int>(sizeof(T));
+    auto* kernel = norm_ring_kernel<T, W, PACK, STAGES>;
+    const int warps = ring_warps(p.D), groups = MAX_WARPS / warps;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t need = (p.rows + groups - 1) / groups;
+    kernel<<<static_cast<unsigned>(need < GRID_SMS ? need : GRID_SMS), groups * warps * 32, SMEM, s>>>(p, warps);
+    return cudaGetLastError();
+}
+template <typename T, bool PACK>
+cudaError_t norm_ring_launch(const NormParams& p, cudaStream_t s) {
+    switch (ring_width(p.D)) {
+        case 1: return norm_ring_width<T, 1, PACK>(p, s);
+        case 2: return norm_ring_width<T, 2, PACK>(p, s);
+        case 4: return norm_ring_width<T, 4, PACK>(p, s);
+        case 8: return norm_ring_width<T, 8, PACK>(p, s);
+        case 16: return norm_ring_width<T, 16, PACK>(p, s);
+        default: return norm_ring_width<T, 0, PACK>(p, s);
+    }
+}
+
+template <typename T, bool WIDE, int NV, bool PACK>
 cudaError_t norm_launch(const NormParams& p, const RowShape& h, cudaStream_t s) {
-    const int64_t need = (p.rows + static_cast<int64_t>(h.groups) * h.u_rows - 1) / (static_cast<int64_t>(h.groups) * h.u_rows);
-    const unsigned grid = static_cast<unsigned>(need < 148 * 4 ? need : 148 * 4), threads = h.warps * h.groups * 32;
-    if (h.warps > 1) norm_kernel<T, WIDE, NV, U, true, PACK><<<grid, threads, 0, s>>>(p, h.warps, h.u_rows);
-    else norm_kernel<T, WIDE, NV, U, false, PACK><<<grid, threads, 0, s>>>(p, h.warps, h.u_rows);
+    const int64_t need = (p.rows + h.groups - 1) / h.groups;
+    const unsigned grid = static_cast<unsigned>(need < GRID_SMS * 16 ? need : GRID_SMS * 16), threads = h.warps * h.groups * 32;
+    if (h.warps > 1) norm_kernel<T, WIDE, NV, true, PACK><<<grid, threads, 0, s>>>(p, h.warps);
+    else norm_kernel<T, WIDE, NV, false, PACK><<<grid, threads, 0, s>>>(p, h.warps);
     return cudaGetLastError();
 }
 
 template <typename T, bool PACK>
 cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
-    const bool wide = p.D % N == 0 && p.x_stride % N == 0 && aligned16(p.x) && aligned16(p.y) &&
-                      (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0;
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 8, 4) : row_shape(p.rows, p.D, 4, 16, 8, 2);
+    const bool wide = p.D % N == 0 && p.x_stride % N == 0 && aligned16(p.x) && aligned16(p.y) && (!p.w || aligned16(p.w)) &&
+                      (!p.b || aligned16(p.b)) && (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0;
+    if (wide && p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) return norm_ring_launch<T, PACK>(p, s);
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8, 1) : row_shape(p.rows, p.D, 4, 16, 8, 1);
     if (h.warps == 0) {
         norm_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         return cudaGetLastError();
     }
-    if (!wide) return h.nv == 4 ? norm_launch<T, false, 4, 2, PACK>(p, h, s) : norm_launch<T, false, 16, 2, PACK>(p, h, s);
-    if (h.nv == 1) return norm_launch<T, true, 1, 4, PACK>(p, h, s);
-    return norm_launch<T, true, 16 / N, 4, PACK>(p, h, s);
+    if (!wide) return h.nv == 4 ? norm_launch<T, false, 4, PACK>(p, h, s)
+                    : h.nv == 8 ? norm_launch<T, false, 8, PACK>(p, h, s) : norm_launch<T, false, 16, PACK>(p, h, s);
+    switch (h.nv) {
+        case 1: return norm_launch<T, true, 1, PACK>(p, h, s);
+        case 2: return norm_launch<T, true, 2, PACK>(p, h, s);
+        case 4: return norm_launch<T, true, 4, PACK>(p, h, s);
+        default: return norm_launch<T, true, 8, PACK>(p, h, s);
+    }
 }
 
 template <typename T>
@@ -506,14 +917,44 @@ cudaError_t norm_grad_launch(const NormGradParams& p, const RowShape& h, cudaStr
     return cudaGetLastError();
 }
 
+template <typename T, int W, bool KEPT>
+cudaError_t norm_grad_ring_width(NormGradParams& p, cudaStream_t s) {
+    constexpr int X = KEPT ? 1 : static_cast<int>(sizeof(T));           // bytes of a kept value
+    constexpr int STAGES = sizeof(T) == 4 ? 3 : 6;                       // at most 193 KB
+    constexpr int SMEM = STAGES * (RING_THREADS * RING_COLUMNS * (static_cast<int>(sizeof(T)) + X) + RING_THREADS / 2);
+    auto* kernel = norm_grad_ring_kernel<T, W, KEPT, STAGES>;
+    const int warps = ring_warps(p.D), groups = MAX_WARPS / warps;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t need = (p.rows + groups - 1) / groups;
+    p.splits = static_cast<int>(need < MAX_SPLITS ? need : MAX_SPLITS);
+    kernel<<<p.splits, groups * warps * 32, SMEM, s>>>(p, warps);
+    return cudaGetLastError();
+}
+template <typename T, bool KEPT>
+cudaError_t norm_grad_ring_launch(NormGradParams& p, cudaStream_t s) {
+    switch (ring_width(p.D)) {
+        case 1: return norm_grad_ring_width<T, 1, KEPT>(p, s);
+        case 2: return norm_grad_ring_width<T, 2, KEPT>(p, s);
+        case 4: return norm_grad_ring_width<T, 4, KEPT>(p, s);
+        case 8: return norm_grad_ring_width<T, 8, KEPT>(p, s);
+        case 16: return norm_grad_ring_width<T, 16, KEPT>(p, s);
+        default: return norm_grad_ring_width<T, 0, KEPT>(p, s);
+    }
+}
+
 template <typename T, bool KEPT>
 cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
-    bool wide = p.D % N == 0 && p.dy_stride % N == 0 && aligned16(p.dy) && (!p.dx || aligned16(p.dx)) && (!p.add || aligned16(p.add));
+    bool wide = p.D % N == 0 && p.dy_stride % N == 0 && aligned16(p.dy) && (!p.dx || aligned16(p.dx)) && (!p.add || aligned16(p.add)) &&
+                (!p.w || aligned16(p.w));
     wide = wide && (KEPT ? (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0 : p.x_stride % N == 0 && aligned16(p.x));
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16, 2) : row_shape(p.rows, p.D, 4, 16, 16, 1);
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16, 1) : row_shape(p.rows, p.D, 4, 16, 16, 1);
     const bool sums = p.dw || p.db;
-    if (h.warps == 0 || p.rows == 0) {
+    if (wide && p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) {
+        const cudaError_t e = norm_grad_ring_launch<T, KEPT>(p, s);
+        if (e != cudaSuccess) return e;
+    } else if (h.warps == 0 || p.rows == 0) {
         p.splits = splits_for(p.rows);
         if (p.dx) norm_grad_rows_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         if (sums) norm_grad_cols_loop_kernel<T><<<dim3(static_cast<unsigned>((p.D + 31) / 32), static_cast<unsigned>(p.splits)), 256, 0, s>>>(p);
@@ -521,12 +962,14 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
         const int64_t need = (p.rows + static_cast<int64_t>(h.groups) * h.u_rows - 1) / (static_cast<int64_t>(h.groups) * h.u_rows);
         p.splits = static_cast<int>(need < MAX_SPLITS ? need : MAX_SPLITS);
         cudaError_t e;
-        if (!wide) e = h.nv == 4 ? norm_grad_launch<T, false, 4, 1, KEPT>(p, h, s) : norm_grad_launch<T, false, 16, 1, KEPT>(p, h, s);
+        if (!wide) e = h.nv == 4 ? norm_grad_launch<T, false, 4, 1, KEPT>(p, h, s)
+                     : h.nv == 8 ? norm_grad_launch<T, false, 8, 1, KEPT>(p, h, s) : norm_grad_launch<T, false, 16, 1, KEPT>(p, h, s);
         else if (h.nv == 1) e = norm_grad_launch<T, true, 1, 2, KEPT>(p, h, s);
-        else e = norm_grad_launch<T, true, 16 / N, 2, KEPT>(p, h, s);
+        else if (h.nv == 16 / N) e = norm_grad_launch<T, true, 16 / N, 1, KEPT>(p, h, s);
+        else e = norm_grad_launch<T, true, 2, 1, KEPT>(p, h, s);
         if (e != cudaSuccess) return e;
     }
-    if (sums) norm_grad_join_kernel<T><<<static_cast<unsigned>((p.D + 31) / 32), 256, 0, s>>>(p);
+    if (sums) norm_grad_join_kernel<T><<<static_cast<unsigned>((p.D + 31) / 32), 32 * JOIN_LANES, 0, s>>>(p);
     return cudaGetLastError();
 }
 

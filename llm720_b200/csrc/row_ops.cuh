@@ -52,6 +52,8 @@ template <> __device__ __forceinline__ float max_finite<__nv_bfloat16>() { retur
 template <> __device__ __forceinline__ float max_finite<__half>() { return 65504.0f; }
 template <typename T> __device__ __forceinline__ float unpacked(float payload_value, float scale) {
     const float v = payload_value * scale;
+    // 448 * scale fits below these scales: the test is the same for a whole row
+    if (scale < (sizeof(T) == 2 && max_finite<T>() < 1e5f ? 256.f : 1.329227996e36f)) return v;
     return fabsf(v) > max_finite<T>() ? copysignf(max_finite<T>(), v) : v;     // NaN stays NaN
 }
 
@@ -275,11 +277,14 @@ struct RowShape { int warps, groups, nv, u_rows; };
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Many rows: nv_max pieces per thread, so that a row needs few warps and few exchanges between them.  Fewer than 1024
-// rows (under seven per SM): nv_min, a row is then spread wider and finished sooner.
+// Many rows: up to nv_max pieces per thread (doubling from nv_min until one warp takes the row), so that a row needs
+// few warps and few exchanges between them.  Fewer than 1024 rows (under seven per SM): nv_min, a row is then spread
+// wider and finished sooner.
 inline RowShape row_shape(int64_t rows, int64_t pieces, int nv_min, int nv_max, int block_warps, int u_max) {
     RowShape s{};
-    s.nv = ((rows < 1024 && pieces <= 32 * MAX_ROW_WARPS * nv_min) || pieces <= 32 * nv_min) ? nv_min : nv_max;
+    s.nv = nv_min;
+    if (rows >= 1024 || pieces > 32 * MAX_ROW_WARPS * nv_min)
+        while (s.nv < nv_max && pieces > 32 * s.nv) s.nv *= 2;
     const int64_t warps = (pieces + 32 * s.nv - 1) / (32 * s.nv);
     if (warps > MAX_ROW_WARPS) return s;
     s.warps = static_cast<int>(warps);

@@ -122,16 +122,21 @@ cudaError_t pack_t(const void* xv, int64_t x_stride, int64_t rows, int64_t D, ui
     constexpr int N = 16 / sizeof(T);
     const T* x = static_cast<const T*>(xv);
     const bool wide = D % N == 0 && x_stride % N == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(payload) & (N - 1)) == 0;
-    const RowShape h = wide ? row_shape(rows, D / N, 2, 8, 8, 1) : row_shape(rows, D, 4, 16, 8, 1);
+    const RowShape h = wide ? row_shape(rows, D / N, 1, 8, 8, 1) : row_shape(rows, D, 4, 16, 8, 1);
     if (h.warps == 0) {
         const unsigned grid = static_cast<unsigned>(rows < GRID_SMS * 64 ? rows : GRID_SMS * 64);
         pack_rows_loop_kernel<T><<<grid, 256, 0, s>>>(x, x_stride, rows, D, payload, scale);
         return cudaGetLastError();
     }
     if (!wide) return h.nv == 4 ? pack_launch<T, false, 4>(x, x_stride, rows, D, payload, scale, h, s)
+                    : h.nv == 8 ? pack_launch<T, false, 8>(x, x_stride, rows, D, payload, scale, h, s)
                                 : pack_launch<T, false, 16>(x, x_stride, rows, D, payload, scale, h, s);
-    return h.nv == 2 ? pack_launch<T, true, 2>(x, x_stride, rows, D, payload, scale, h, s)
-                     : pack_launch<T, true, 8>(x, x_stride, rows, D, payload, scale, h, s);
+    switch (h.nv) {
+        case 1: return pack_launch<T, true, 1>(x, x_stride, rows, D, payload, scale, h, s);
+        case 2: return pack_launch<T, true, 2>(x, x_stride, rows, D, payload, scale, h, s);
+        case 4: return pack_launch<T, true, 4>(x, x_stride, rows, D, payload, scale, h, s);
+        default: return pack_launch<T, true, 8>(x, x_stride, rows, D, payload, scale, h, s);
+    }
 }
 
 template <typename T>

@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float f[N], d[N];
-                if constexpr (KEPT) P::decode_packed(x[u][i], sc[u], f); else P::decode(x[u][i], f);
+                if constexpr (KEPT) unpack_piece<T, WIDE>(x[u][i], sc[u], f); else P::decode(x[u][i], f);
                 P::decode(dy[u][i], d);                     // zero where there is no column or no row
 #pragma unroll
                 for (int q = 0; q < N; ++q) {
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
                 const int64_t c = gt + static_cast<int64_t>(i) * threads;
                 if (c >= pieces) break;
                 float f[N], d[N], a[N];
-                if constexpr (KEPT) P::decode_packed(x[u][i], sc[u], f); else P::decode(x[u][i], f);
+                if constexpr (KEPT) unpack_piece<T, WIDE>(x[u][i], sc[u], f); else P::decode(x[u][i], f);
                 P::decode(dy[u][i], d);
                 if (p.add) P::decode(P::load(static_cast<const T*>(p.add) + r * p.D + c * N), a);
 #pragma unroll
@@ -388,6 +388,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
         }
     }
     if (!p.dw && !p.db) return;
+    grid_release();
     // the block's groups add up in order, then the block writes its partial row
     const int wide = threads * E;
     for (int g = 0; g + 1 < groups; ++g) {
@@ -691,19 +692,29 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const N
             rstd = __uint_as_float(v.y);
             sc = __uint_as_float(v.z);
         }
-        const float2 r2 = splat(rstd), c2 = splat(-mean * rstd);
+        // kept in 8 bits: the scale, a power of two, goes into the factor, unless the row's values may need the clamp
+        const bool clamp = KEPT && may_clamp<T>(sc);
+        const float2 r2 = splat(rstd), rx = splat(KEPT && !clamp ? rstd * sc : rstd), c2 = splat(-mean * rstd);
         float2 n[NV][H], g[NV][H], s1 = splat(0.f), s2 = splat(0.f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const X xr = in[i] ? shared_at<X>(slot + x_at + i * RING_THREADS * XB) : X{};
             const uint4 dr = in[i] ? shared_at<uint4>(slot + dy_at + i * RING_THREADS * 16) : P::zero();
             float f[N], d[N];
-            if constexpr (KEPT) P::decode_packed(xr, sc, f); else P::decode(xr, f);
+            if constexpr (KEPT) {
+                P::decode_packed(xr, f);
+                if (clamp) {
+#pragma unroll
+                    for (int q = 0; q < N; ++q) f[q] = unpacked<T>(f[q], sc);
+                }
+            } else {
+                P::decode(xr, f);
+            }
             P::decode(dr, d);
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 const float2 dv = make_float2(d[2 * h], d[2 * h + 1]);
-                n[i][h] = __ffma2_rn(make_float2(f[2 * h], f[2 * h + 1]), r2, c2);
+                n[i][h] = __ffma2_rn(make_float2(f[2 * h], f[2 * h + 1]), rx, c2);
                 g[i][h] = __fmul2_rn(dv, w[i][h]);
                 s1 = __fadd2_rn(s1, g[i][h]);
                 s2 = __ffma2_rn(g[i][h], n[i][h], s2);
@@ -758,6 +769,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const N
         __syncwarp();                                       // before a fetch overwrites a slot another lane may still read
     }
     if (!p.dw && !p.db) return;
+    grid_release();
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                        // the ring is free: the groups add up in order through it
     float2* columns = reinterpret_cast<float2*>(ring_smem);      // [2 * NV * H][threads]
@@ -807,6 +819,7 @@ __global__ void __launch_bounds__(32 * JOIN_LANES) norm_grad_join_kernel(const N
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
     float aw = 0.f, ab = 0.f;
+    grid_wait();
     if (c < p.D) {
 #pragma unroll
         for (int k = 0; k < (GRID_SMS + JOIN_LANES - 1) / JOIN_LANES; ++k) {
@@ -887,7 +900,7 @@ cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
     const bool wide = p.D % N == 0 && p.x_stride % N == 0 && aligned16(p.x) && aligned16(p.y) && (!p.w || aligned16(p.w)) &&
                       (!p.b || aligned16(p.b)) && (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0;
     if (wide && p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) return norm_ring_launch<T, PACK>(p, s);
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8, 1) : row_shape(p.rows, p.D, 4, 16, 8, 1);
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8, 1) : narrow_shape(p.rows, p.D, 8);
     if (h.warps == 0) {
         norm_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         return cudaGetLastError();
@@ -949,7 +962,7 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     bool wide = p.D % N == 0 && p.dy_stride % N == 0 && aligned16(p.dy) && (!p.dx || aligned16(p.dx)) && (!p.add || aligned16(p.add)) &&
                 (!p.w || aligned16(p.w));
     wide = wide && (KEPT ? (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0 : p.x_stride % N == 0 && aligned16(p.x));
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16, 1) : row_shape(p.rows, p.D, 4, 16, 16, 1);
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16, 1) : narrow_shape(p.rows, p.D, 16);
     const bool sums = p.dw || p.db;
     if (wide && p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) {
         const cudaError_t e = norm_grad_ring_launch<T, KEPT>(p, s);
@@ -969,7 +982,7 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
         else e = norm_grad_launch<T, true, 2, 1, KEPT>(p, h, s);
         if (e != cudaSuccess) return e;
     }
-    if (sums) norm_grad_join_kernel<T><<<static_cast<unsigned>((p.D + 31) / 32), 32 * JOIN_LANES, 0, s>>>(p);
+    if (sums) return launch_behind(norm_grad_join_kernel<T>, dim3(static_cast<unsigned>((p.D + 31) / 32)), dim3(32 * JOIN_LANES), s, p);
     return cudaGetLastError();
 }
 

@@ -52,9 +52,11 @@ template <> __device__ __forceinline__ float max_finite<__nv_bfloat16>() { retur
 template <> __device__ __forceinline__ float max_finite<__half>() { return 65504.0f; }
 template <typename T> __device__ __forceinline__ float unpacked(float payload_value, float scale) {
     const float v = payload_value * scale;
-    // 448 * scale fits below these scales: the test is the same for a whole row
-    if (scale < (sizeof(T) == 2 && max_finite<T>() < 1e5f ? 256.f : 1.329227996e36f)) return v;
     return fabsf(v) > max_finite<T>() ? copysignf(max_finite<T>(), v) : v;     // NaN stays NaN
+}
+// a row with such a scale may hold values that need the clamp: 448 * scale does not fit the type
+template <typename T> __device__ __forceinline__ bool may_clamp(float scale) {
+    return scale >= (max_finite<T>() < 1e5f ? 256.f : 1.329227996e36f);         // 2^8, 2^120
 }
 
 __device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(FULL_MASK, v); }
@@ -112,7 +114,7 @@ template <typename T> struct Piece<T, false> {
     __device__ static __forceinline__ void decode(const Raw& r, float (&f)[1]) { f[0] = to_f32<T>(r); }
     __device__ static __forceinline__ Raw encode(const float (&f)[1]) { return from_f32<T>(f[0]); }
     __device__ static __forceinline__ Packed load_packed(const uint8_t* p) { return __ldg(p); }
-    __device__ static __forceinline__ void decode_packed(const Packed& r, float s, float (&f)[1]) { f[0] = unpacked<T>(e4m3_value(r), s); }
+    __device__ static __forceinline__ void decode_packed(const Packed& r, float (&f)[1]) { f[0] = e4m3_value(r); }
     __device__ static __forceinline__ Packed encode_packed(const float (&f)[1]) { return static_cast<uint8_t>(e4m3_pair(f[0], 0.f)); }
 };
 template <> struct Piece<float, true> {
@@ -129,9 +131,9 @@ template <> struct Piece<float, true> {
         return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
     }
     __device__ static __forceinline__ Packed load_packed(const uint8_t* p) { return __ldg(reinterpret_cast<const uint32_t*>(p)); }
-    __device__ static __forceinline__ void decode_packed(const Packed& r, float s, float (&f)[4]) {
+    __device__ static __forceinline__ void decode_packed(const Packed& r, float (&f)[4]) {
         const float2 a = e4m3_pair_values(static_cast<uint16_t>(r)), b = e4m3_pair_values(static_cast<uint16_t>(r >> 16));
-        f[0] = unpacked<float>(a.x, s); f[1] = unpacked<float>(a.y, s); f[2] = unpacked<float>(b.x, s); f[3] = unpacked<float>(b.y, s);
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
     }
     __device__ static __forceinline__ Packed encode_packed(const float (&f)[4]) {
         return e4m3_pair(f[0], f[1]) | (static_cast<uint32_t>(e4m3_pair(f[2], f[3])) << 16);
@@ -157,13 +159,13 @@ template <typename T> struct Piece<T, true> {
         return r;
     }
     __device__ static __forceinline__ Packed load_packed(const uint8_t* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
-    __device__ static __forceinline__ void decode_packed(const Packed& r, float s, float (&f)[8]) {
+    __device__ static __forceinline__ void decode_packed(const Packed& r, float (&f)[8]) {
         const uint32_t h[2] = {r.x, r.y};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float2 a = e4m3_pair_values(static_cast<uint16_t>(h[q >> 1] >> (16 * (q & 1))));
-            f[2 * q] = unpacked<T>(a.x, s);
-            f[2 * q + 1] = unpacked<T>(a.y, s);
+            f[2 * q] = a.x;
+            f[2 * q + 1] = a.y;
         }
     }
     __device__ static __forceinline__ Packed encode_packed(const float (&f)[8]) {
@@ -171,6 +173,19 @@ template <typename T> struct Piece<T, true> {
                           e4m3_pair(f[4], f[5]) | (static_cast<uint32_t>(e4m3_pair(f[6], f[7])) << 16));
     }
 };
+
+// a piece's values from its packed form
+template <typename T, bool WIDE>
+__device__ __forceinline__ void unpack_piece(const typename Piece<T, WIDE>::Packed& r, float scale, float (&f)[Piece<T, WIDE>::N]) {
+    Piece<T, WIDE>::decode_packed(r, f);
+    if (may_clamp<T>(scale)) {                              // the same for the whole row
+#pragma unroll
+        for (int q = 0; q < Piece<T, WIDE>::N; ++q) f[q] = unpacked<T>(f[q], scale);
+    } else {
+#pragma unroll
+        for (int q = 0; q < Piece<T, WIDE>::N; ++q) f[q] *= scale;
+    }
+}
 
 // Largest magnitude of raw pieces as an unsigned number in the storage type's own bit pattern (two 16-bit lanes per
 // word: `join` folds them), which orders like the magnitude itself; at `not_finite` or above it an infinity or NaN was
@@ -268,6 +283,28 @@ __device__ __forceinline__ void group_sync(int group, int threads) {
 
 
 // ---------------------------------------------------------------------------
+// Programmatic dependent launch: a kernel launched with `launch_behind` may be set up while the one before it in the
+// stream still runs.  `grid_wait` in it returns when that one has completed and its writes are visible; `grid_release`
+// in the earlier kernel says that a block no longer minds.  Saves the 2 us between a kernel and a short one behind it.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+inline cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+// ---------------------------------------------------------------------------
 // How a row is spread over threads: `warps` warps per row, `groups` rows' worth of warps per block, nv pieces per
 // thread, u_rows rows at a time per group.  warps == 0: the row is longer than MAX_ROW_WARPS warps take.
 // ---------------------------------------------------------------------------
@@ -292,6 +329,11 @@ inline RowShape row_shape(int64_t rows, int64_t pieces, int nv_min, int nv_max, 
     const int64_t ru = (rows + GRID_SMS * s.groups - 1) / (GRID_SMS * s.groups);      // all u_max only when every SM gets some
     s.u_rows = static_cast<int>(ru < 1 ? 1 : (ru > u_max ? u_max : ru));
     return s;
+}
+
+// rows that are not whole 16-byte pieces: one value at a time, 8 per thread (16 spill) unless the row is wider
+inline RowShape narrow_shape(int64_t rows, int64_t D, int block_warps) {
+    return row_shape(rows, D, 4, D <= 32 * MAX_ROW_WARPS * 8 ? 8 : 16, block_warps, 1);
 }
 
 }  // namespace peer

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256) unpack_rows_kernel(const uint8_t* __restr
         for (int i = 0; i < SEGMENT; ++i)
             if (c0 + i * 32 < pieces) {
                 float f[N];
-                P::decode_packed(v[i], s, f);
+                unpack_piece<T, true>(v[i], s, f);
                 P::store(out + r * D + (c0 + i * 32) * N, P::encode(f));
             }
     }
@@ -122,7 +122,7 @@ cudaError_t pack_t(const void* xv, int64_t x_stride, int64_t rows, int64_t D, ui
     constexpr int N = 16 / sizeof(T);
     const T* x = static_cast<const T*>(xv);
     const bool wide = D % N == 0 && x_stride % N == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(payload) & (N - 1)) == 0;
-    const RowShape h = wide ? row_shape(rows, D / N, 1, 8, 8, 1) : row_shape(rows, D, 4, 16, 8, 1);
+    const RowShape h = wide ? row_shape(rows, D / N, 1, 8, 8, 1) : narrow_shape(rows, D, 8);
     if (h.warps == 0) {
         const unsigned grid = static_cast<unsigned>(rows < GRID_SMS * 64 ? rows : GRID_SMS * 64);
         pack_rows_loop_kernel<T><<<grid, 256, 0, s>>>(x, x_stride, rows, D, payload, scale);

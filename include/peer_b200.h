@@ -385,7 +385,7 @@ int peer_embedding(const void* ids, int32_t id_bytes, int64_t n_ids, const void*
 int64_t peer_embedding_workspace(int64_t n_ids, int64_t dim);
 
 /* grad_weight[v] = scale * sum of grad[t] over ids[t] = v: every row of grad_weight [vocab, dim] is written, the sums are
- * in fp32 in the order of t and rounded once.  Ids outside the table, and padding_idx (-1: none), take no part.
+ * in fp32, in an order that depends on the ids alone, and rounded once.  Ids outside the table, and padding_idx (-1: none), take no part.
  * workspace: peer_embedding_workspace bytes, 16-byte aligned. */
 int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_t n_ids, const void* grad, int64_t grad_stride,
                             int32_t dtype, int64_t vocab, int64_t dim, float scale, int64_t padding_idx, void* grad_weight,

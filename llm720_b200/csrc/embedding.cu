@@ -11,8 +11,9 @@
 //
 // The sorted positions are cut into tiles of equal length, whatever the ids'
 // frequencies are (text: one id can hold a tenth of all tokens).  An id whose
-// positions lie in one tile is finished there; one that crosses tiles leaves a
-// partial row per tile, and the join kernel adds those in tile order.
+// positions lie in one tile is finished there, in the order of its positions;
+// one that crosses tiles leaves a partial row per tile, and the join kernel adds
+// those in a fixed order (four interleaved runs, then the runs).
 #include <cstdio>
 
 #include "kernels.h"
@@ -93,83 +94,188 @@ struct SumParams {
     float scale;
     void* out; int64_t D;
     float* partial;                                // [tiles][2][D]
-    int per_tile; int64_t tiles;
+    int* open_tiles; int* open_count;              // tiles in which an id begins that goes on behind them
+    int64_t tiles;
+    int row_threads, slabs;                        // threads of a tile, column slabs of row_threads pieces
+    int zero_blocks;                               // leading blocks write the rows no position names
 };
 
-// block: one tile of sorted positions, SUM_THREADS * VEC columns
-template <typename T, int VEC>
-__global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p) {
-    const int64_t c = (static_cast<int64_t>(blockIdx.y) * SUM_THREADS + threadIdx.x) * VEC;
-    if (c >= p.D) return;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per_tile;
-    const int64_t t1 = t0 + p.per_tile < p.n ? t0 + p.per_tile : p.n;
-    uint32_t cur = p.keys[t0];
-    if (cur == p.vocab) return;
-    bool open_left = t0 > 0 && p.keys[t0 - 1] == cur;      // the id's positions begin in an earlier tile
-    float acc[VEC];
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-    for (int64_t j = t0; j <= t1; ++j) {
-        const uint32_t key = j < p.n ? p.keys[j] : p.vocab;
-        if (key != cur || j == t1) {
-            const bool open_right = key == cur;
-            if (open_left || open_right) {
-                float* dst = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (open_left ? 0 : 1)) * p.D + c;
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) dst[q] = acc[q];
-            } else {
-                float f[VEC];
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) f[q] = acc[q] * p.scale;
-                Load<T, VEC>::put(static_cast<T*>(p.out) + static_cast<int64_t>(cur) * p.D + c, f);
-            }
-            if (j == t1 || key == p.vocab) return;
-            cur = key;
-            open_left = false;
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-        }
-        float f[VEC];
-        Load<T, VEC>::get(static_cast<const T*>(p.src) + static_cast<int64_t>(p.order[j]) * p.src_stride + c, f);
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) acc[q] += f[q];
-    }
-}
-
-// first index in [0, n) whose key is not below `key`
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* __restrict__ keys, int64_t n, uint32_t key) {
-    int64_t lo = 0, hi = n;
+// 32-ary search by the warp over a sorted array: number of leading entries (of n, `stride` apart) for which
+// below(i) holds.  below() must be true, then false.
+template <typename F>
+__device__ __forceinline__ int64_t warp_count(int64_t n, const F& below) {
+    const int lane = threadIdx.x & 31;
+    int64_t lo = 0, hi = n;                                // below(i) for i < lo, not for i >= hi
     while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < key) lo = mid + 1; else hi = mid;
+        const int64_t step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const unsigned yes = __ballot_sync(FULL_MASK, i < hi && below(i));
+        const int k = __popc(yes);                         // the first k samples hold
+        const int64_t next_lo = k ? lo + (k - 1) * step + 1 : lo, next_hi = lo + k * step;
+        hi = next_hi < hi ? next_hi : hi;
+        lo = next_lo;
     }
     return lo;
 }
 
-// the id whose positions begin in tile blockIdx.x and reach past its end: the sum of its partial rows
+constexpr int ZERO_ROWS = 64;
+
+// rows [first, first + ZERO_ROWS): which of them the sorted keys name, then zeros for the others
 template <typename T>
-__global__ void __launch_bounds__(SUM_THREADS) row_sum_join_kernel(const SumParams p) {
-    const int64_t c = static_cast<int64_t>(blockIdx.y) * SUM_THREADS + threadIdx.x;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per_tile, t1 = t0 + p.per_tile;
-    if (t1 >= p.n || c >= p.D) return;
-    const uint32_t cur = p.keys[t1 - 1];
-    if (cur == p.vocab || p.keys[t1] != cur) return;
-    if (t0 > 0 && p.keys[t0] == cur && p.keys[t0 - 1] == cur) return;      // began in an earlier tile
-    const int64_t last = (lower_bound(p.keys, p.n, cur + 1) - 1) / p.per_tile;
-    float acc = p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.D + c];
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) + 1; u <= last; ++u) acc += p.partial[u * 2 * p.D + c];
-    static_cast<T*>(p.out)[static_cast<int64_t>(cur) * p.D + c] = from_f32<T>(acc * p.scale);
+__device__ __forceinline__ void zero_rows(const SumParams& p, int64_t first) {
+    __shared__ uint32_t named[ZERO_ROWS / 32];
+    if (threadIdx.x < ZERO_ROWS / 32) named[threadIdx.x] = 0u;
+    __shared__ int64_t from;
+    const int64_t last = first + ZERO_ROWS < p.vocab ? first + ZERO_ROWS : p.vocab;
+    if (threadIdx.x < 32) {
+        const int64_t at = warp_count(p.n, [&](int64_t i) { return p.keys[i] < static_cast<uint32_t>(first); });
+        if (threadIdx.x == 0) from = at;
+    }
+    __syncthreads();
+    // one thread per position of these rows; an id with many positions is met at its first few strides only once per
+    // stride, so rows are skipped to by search when a stride brought no new one
+    for (int64_t j0 = from; j0 < p.n;) {
+        const int64_t j = j0 + threadIdx.x;
+        const uint32_t key = j < p.n ? p.keys[j] : p.vocab;
+        if (key < last) atomicOr(&named[(key - first) >> 5], 1u << ((key - first) & 31));
+        const uint32_t end_key = j0 + blockDim.x - 1 < p.n ? p.keys[j0 + blockDim.x - 1] : p.vocab;
+        if (end_key >= last) break;
+        // the stride ended inside end_key's positions: go on behind them
+        j0 += blockDim.x;
+        if (p.keys[j0 < p.n ? j0 : p.n - 1] == end_key)
+            j0 += warp_count(p.n - j0, [&](int64_t i) { return p.keys[j0 + i] <= end_key; });
+    }
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = p.D % V == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+    for (int64_t v = first + warp; v < last; v += blockDim.x >> 5) {
+        if (named[(v - first) >> 5] >> ((v - first) & 31) & 1u) continue;
+        T* row = static_cast<T*>(p.out) + v * p.D;
+        if (vec) for (int64_t c = lane; c < p.D / V; c += 32) reinterpret_cast<uint4*>(row)[c] = make_uint4(0u, 0u, 0u, 0u);
+        else for (int64_t c = lane; c < p.D; c += 32) row[c] = from_f32<T>(0.f);
+    }
 }
 
-// rows that no position names: zeros (one warp per row)
-template <typename T>
-__global__ void __launch_bounds__(256) row_zero_kernel(const SumParams p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t stride = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-    for (int64_t v = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; v < p.vocab; v += stride) {
-        const int64_t at = lower_bound(p.keys, p.n, static_cast<uint32_t>(v));
-        if (at < p.n && p.keys[at] == static_cast<uint32_t>(v)) continue;
-        for (int64_t c = lane; c < p.D; c += 32) static_cast<T*>(p.out)[v * p.D + c] = from_f32<T>(0.f);
+// Blocks behind the zero blocks: tiles of PER sorted positions, row_threads pieces of columns each (several tiles per
+// block when rows are short).  Eight rows' pieces are in flight per thread; the additions keep the order of positions.
+template <typename T, bool WIDE, int PER>
+__global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p) {
+    using P = Piece<T, WIDE>;
+    constexpr int N = P::N, U = 8;
+    __shared__ uint32_t s_key[SUM_THREADS / 8 * PER], s_pos[SUM_THREADS / 8 * PER];
+    grid_wait();                                           // the sort's results
+    if (static_cast<int>(blockIdx.x) < p.zero_blocks) {
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * ZERO_ROWS; r < p.vocab; r += static_cast<int64_t>(p.zero_blocks) * ZERO_ROWS) {
+            zero_rows<T>(p, r);
+            __syncthreads();
+        }
+        return;
+    }
+    const int subs = SUM_THREADS / p.row_threads, sub = threadIdx.x / p.row_threads;
+    const int64_t job = blockIdx.x - p.zero_blocks, slab = job % p.slabs, tile0 = job / p.slabs * subs;
+    for (int i = threadIdx.x; i < subs * PER; i += SUM_THREADS) {
+        const int64_t j = tile0 * PER + i;
+        s_key[i] = j < p.n ? p.keys[j] : p.vocab;
+        s_pos[i] = j < p.n ? p.order[j] : 0u;
+    }
+    __syncthreads();
+    const int64_t tile = tile0 + sub, t0 = tile * PER;
+    const int64_t c = (slab * p.row_threads + (threadIdx.x - sub * p.row_threads)) * N;
+    if (t0 >= p.n || c >= p.D) return;
+    const uint32_t* key = s_key + sub * PER;
+    const uint32_t* pos = s_pos + sub * PER;
+    uint32_t cur = key[0];
+    if (cur == p.vocab) return;
+    bool open_left = t0 > 0 && p.keys[t0 - 1] == cur;      // the id's positions begin in an earlier tile
+    const bool goes_on = t0 + PER < p.n && key[PER - 1] != p.vocab && p.keys[t0 + PER] == key[PER - 1];
+    const T* src = static_cast<const T*>(p.src) + c;
+    float acc[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) acc[q] = 0.f;
+    auto flush = [&](bool open_right) {
+        if (open_left || open_right) {
+            float* dst = p.partial + (tile * 2 + (open_left ? 0 : 1)) * p.D + c;
+#pragma unroll
+            for (int q = 0; q < N; ++q) dst[q] = acc[q];
+            if (!open_left && c == 0) p.open_tiles[atomicAdd(p.open_count, 1)] = static_cast<int>(tile);
+        } else {
+            float f[N];
+#pragma unroll
+            for (int q = 0; q < N; ++q) f[q] = acc[q] * p.scale;
+            P::store(static_cast<T*>(p.out) + static_cast<int64_t>(cur) * p.D + c, P::encode(f));
+        }
+    };
+    bool done = false;
+    for (int j0 = 0; j0 < PER && !done; j0 += U) {
+        typename P::Raw raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            raw[u] = key[j0 + u] != p.vocab ? P::load(src + static_cast<int64_t>(pos[j0 + u]) * p.src_stride) : P::zero();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t k = key[j0 + u];
+            if (k != cur && !done) {
+                flush(false);
+                if (k == p.vocab) { done = true; }
+                cur = k;
+                open_left = false;
+#pragma unroll
+                for (int q = 0; q < N; ++q) acc[q] = 0.f;
+            }
+            float f[N];
+            P::decode(raw[u], f);
+#pragma unroll
+            for (int q = 0; q < N; ++q) acc[q] += f[q];
+        }
+    }
+    if (!done) flush(goes_on);
+}
+
+// Sums of the partial rows of ids that cross tiles: jobs are (entry of open_tiles, slab of 256 columns); 64 threads of
+// four columns (one, if rows are no multiples of four) by four lanes of partial rows.
+template <typename T, int V, int PER>
+__global__ void __launch_bounds__(SUM_THREADS) row_sum_join_kernel(const SumParams p) {
+    __shared__ float lanes[4][64 * V];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int64_t slabs = (p.D + 64 * V - 1) / (64 * V);
+    grid_wait();
+    const int64_t jobs = static_cast<int64_t>(*p.open_count) * slabs;
+    for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const int64_t tile = p.open_tiles[job / slabs], c = (job % slabs) * 64 * V + tx * V;
+        const uint32_t cur = p.keys[tile * PER + PER - 1];
+        // tiles behind this one whose last position is still cur's, and the one in which cur ends
+        const int64_t more = warp_count(p.tiles - tile - 1, [&](int64_t i) {
+            const int64_t e = (tile + 2 + i) * PER;
+            return e < p.n && p.keys[e - 1] == cur && p.keys[e] == cur;
+        }) + 1;
+        float acc[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] = 0.f;
+        if (c < p.D) {
+            const float* own = p.partial + (tile * 2 + 1) * p.D + c;
+            const float* rest = p.partial + (tile + 1) * 2 * p.D + c;
+#pragma unroll 4
+            for (int64_t u = ty; u <= more; u += 4) {
+                const float* row = u == 0 ? own : rest + (u - 1) * 2 * p.D;
+                if constexpr (V == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(row);
+                    acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
+                } else {
+                    acc[0] += row[0];
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < V; ++q) lanes[ty][tx * V + q] = acc[q];
+        __syncthreads();
+        if (ty == 0 && c < p.D) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                const float s = lanes[0][tx * V + q] + lanes[1][tx * V + q] + lanes[2][tx * V + q] + lanes[3][tx * V + q];
+                static_cast<T*>(p.out)[static_cast<int64_t>(cur) * p.D + c + q] = from_f32<T>(s * p.scale);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -188,21 +294,32 @@ cudaError_t embed_t(const void* ids, int id_bytes, int64_t n, const void* w, int
     return cudaGetLastError();
 }
 
+template <typename T, bool WIDE, int PER>
+cudaError_t sums_launch(SumParams p, cudaStream_t s) {
+    constexpr int N = Piece<T, WIDE>::N;
+    const int64_t pieces = p.D / N;
+    p.row_threads = 8;
+    while (p.row_threads < SUM_THREADS && p.row_threads < pieces) p.row_threads *= 2;
+    p.slabs = static_cast<int>((pieces + p.row_threads - 1) / p.row_threads);
+    const int subs = SUM_THREADS / p.row_threads;
+    const int64_t zb = (static_cast<int64_t>(p.vocab) + ZERO_ROWS - 1) / ZERO_ROWS;
+    p.zero_blocks = static_cast<int>(zb < GRID_SMS * 32 ? zb : GRID_SMS * 32);
+    const int64_t blocks = p.zero_blocks + (p.tiles + subs - 1) / subs * p.slabs;
+    cudaError_t e = launch_behind(row_sum_kernel<T, WIDE, PER>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), s, p);
+    if (e != cudaSuccess || p.tiles <= 1) return e;
+    const int64_t jobs = p.tiles * ((p.D + 255) / 256);
+    const dim3 grid(static_cast<unsigned>(jobs < GRID_SMS * 8 ? jobs : GRID_SMS * 8));
+    return p.D % 4 == 0 ? launch_behind(row_sum_join_kernel<T, 4, PER>, grid, dim3(SUM_THREADS), s, p)
+                        : launch_behind(row_sum_join_kernel<T, 1, PER>, grid, dim3(SUM_THREADS), s, p);
+}
+
 template <typename T>
 cudaError_t sums_t(const SumParams& p, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = p.D % V == 0 && p.src_stride % V == 0 &&
-                     ((reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0;
-    const int64_t zb = (static_cast<int64_t>(p.vocab) + 7) / 8;
-    row_zero_kernel<T><<<static_cast<unsigned>(zb < 148 * 16 ? zb : 148 * 16), 256, 0, s>>>(p);
-    if (p.n > 0) {
-        auto slabs = [&](int v) { return static_cast<unsigned>((p.D + SUM_THREADS * v - 1) / (SUM_THREADS * v)); };
-        const unsigned tiles = static_cast<unsigned>(p.tiles);
-        if (vec) row_sum_kernel<T, V><<<dim3(tiles, slabs(V)), SUM_THREADS, 0, s>>>(p);
-        else row_sum_kernel<T, 1><<<dim3(tiles, slabs(1)), SUM_THREADS, 0, s>>>(p);
-        if (p.tiles > 1) row_sum_join_kernel<T><<<dim3(tiles, slabs(1)), SUM_THREADS, 0, s>>>(p);
-    }
-    return cudaGetLastError();
+    constexpr int N = 16 / sizeof(T);
+    if (p.n == 0) return cudaMemsetAsync(p.out, 0, sizeof(T) * static_cast<size_t>(p.vocab) * static_cast<size_t>(p.D), s);
+    const bool wide = p.D % N == 0 && p.src_stride % N == 0 && aligned16(p.src) && aligned16(p.out);
+    if (per_tile_for(p.n) == 16) return wide ? sums_launch<T, true, 16>(p, s) : sums_launch<T, false, 16>(p, s);
+    return wide ? sums_launch<T, true, 64>(p, s) : sums_launch<T, false, 64>(p, s);
 }
 
 int report(const char* name, cudaError_t e) {
@@ -241,7 +358,7 @@ extern "C" int64_t peer_embedding_workspace(int64_t n_ids, int64_t dim) {
     if (n_ids <= 0 || dim < 1) return 0;
     const int per = per_tile_for(n_ids);
     const int64_t tiles = (n_ids + per - 1) / per;
-    return row_sort_bytes(n_ids) + tiles * 2 * dim * static_cast<int64_t>(sizeof(float));
+    return row_sort_bytes(n_ids) + ((tiles + 4) * 4 + 255) / 256 * 256 + tiles * 2 * dim * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_t n_ids, const void* grad, int64_t grad_stride,
@@ -262,13 +379,16 @@ extern "C" int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_
     p.n = n_ids; p.vocab = static_cast<uint32_t>(vocab); p.src = grad; p.src_stride = grad_stride; p.scale = scale;
     p.out = grad_weight; p.D = dim;
     if (n_ids > 0) {
+        const int per = per_tile_for(n_ids);
+        p.tiles = (n_ids + per - 1) / per;
         row_sort_layout(a, workspace);
+        char* rest = static_cast<char*>(workspace) + row_sort_bytes(n_ids);
+        p.open_count = a.counter = reinterpret_cast<int*>(rest);
+        p.open_tiles = p.open_count + 4;
+        p.partial = reinterpret_cast<float*>(rest + ((p.tiles + 4) * 4 + 255) / 256 * 256);
         const cudaError_t e = launch_row_sort(a, s);
         if (e != cudaSuccess) return report("peer_embedding_backward", e);
         p.keys = a.sorted_keys; p.order = a.order;
-        p.per_tile = per_tile_for(n_ids);
-        p.tiles = (n_ids + p.per_tile - 1) / p.per_tile;
-        p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + row_sort_bytes(n_ids));
     }
     if (dtype == PEER_DTYPE_F32) return report("peer_embedding_backward", sums_t<float>(p, s));
     if (dtype == PEER_DTYPE_BF16) return report("peer_embedding_backward", sums_t<__nv_bfloat16>(p, s));

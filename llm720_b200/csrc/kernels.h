@@ -214,6 +214,7 @@ struct RowSortArgs {
     int64_t n, vocab, skip;               // ids outside [0, vocab) and the id `skip` are left out
     uint32_t* keys[2]; uint32_t* pos[2]; uint32_t* counts; uint32_t* totals;
     uint32_t* sorted_keys; uint32_t* order;
+    int* counter;                         // optional: set to zero for the kernels behind the sort
 };
 int64_t row_sort_bytes(int64_t n);
 void row_sort_layout(RowSortArgs& a, void* workspace);

@@ -4,7 +4,11 @@
 // order.  Ids outside [0, vocab), and the one id given as `skip`, get the key
 // `vocab` and end up behind all others.
 //
-// Per digit: (1) every tile of keys counts its digits, (2) every digit scans its
+// Up to 65,536 ids (a training batch): one launch.  A cluster of eight blocks holds all pairs in registers and
+// shared memory; per digit the blocks tell one another their counts and send every pair to its place in distributed
+// shared memory.  16,384 ids below 32,000: SORT_US.
+//
+// More ids: three launches per digit.  (1) every tile of keys counts its digits, (2) every digit scans its
 // counts over the tiles, (3) every tile scatters its keys; the rank of a key
 // among its tile's equal digits comes from a vote over the warp
 // (match.any) on top of a running count per warp and digit.
@@ -28,6 +32,7 @@ template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const RowSortArgs a, const uint32_t* __restrict__ keys, int shift,
                                                                   int digits, int items, int tiles) {
     __shared__ uint32_t hist[MAX_DIGITS];
+    if (FIRST && blockIdx.x == 0 && threadIdx.x == 0 && a.counter) *a.counter = 0;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0u;
     __syncthreads();
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * SORT_THREADS * items;
@@ -139,6 +144,150 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const RowSor
     }
 }
 
+// ---- one cluster ------------------------------------------------------------------------------------------------
+constexpr int CL_BLOCKS = 8, CL_THREADS = 1024, CL_WARPS = CL_THREADS / 32;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address of this block's shared memory location in another block of the cluster
+__device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t a, uint32_t b) {
+    asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+
+struct ClusterShared {
+    uint32_t seen[CL_WARPS][MAX_DIGITS];      // per warp and digit: count, then first slot
+    uint32_t totals[CL_BLOCKS][MAX_DIGITS];   // every block's count per digit
+    uint32_t warp_total[CL_WARPS];
+};
+
+// pairs i of block b, warp w, round k, lane l:  i = ((b * CL_WARPS + w) * IT + k) * 32 + l
+template <int IT>
+__global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const RowSortArgs a, int passes,
+                                                                                                       int per, uint32_t* keys_out,
+                                                                                                       uint32_t* order_out) {
+    extern __shared__ __align__(16) unsigned char cluster_smem[];
+    ClusterShared& sh = *reinterpret_cast<ClusterShared*>(cluster_smem);
+    uint2* pairs = reinterpret_cast<uint2*>(cluster_smem + sizeof(ClusterShared));      // [CL_THREADS * IT]
+    constexpr uint32_t EACH = CL_THREADS * IT;
+    const uint32_t rank = cluster_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t local0 = warp * IT * 32 + lane, i0 = rank * EACH + local0;
+    const uint32_t n = static_cast<uint32_t>(a.n), digits = 1u << per;
+    if (rank == 0 && tid == 0 && a.counter) *a.counter = 0;
+    uint32_t key[IT], pos[IT], slot[IT];
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        pos[k] = i0 + k * 32;
+        key[k] = pos[k] < n ? source_key(a, pos[k]) : 0xffffffffu;      // behind everything, in every digit
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * per;
+        for (int d = tid; d < CL_WARPS * MAX_DIGITS; d += CL_THREADS) (&sh.seen[0][0])[d] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const uint32_t digit = (key[k] >> shift) & (digits - 1);
+            const unsigned same = __match_any_sync(FULL_MASK, digit);
+            const int leader = __ffs(same) - 1;
+            uint32_t before = 0u;
+            if (lane == leader) {
+                before = sh.seen[warp][digit];
+                sh.seen[warp][digit] = before + __popc(same);
+            }
+            before = __shfl_sync(FULL_MASK, before, leader);
+            slot[k] = before + __popc(same & ((1u << lane) - 1u));
+            __syncwarp();
+        }
+        __syncthreads();
+        // thread (digit, quarter): the quarter's warps of one digit, turned into running sums within the quarter
+        {
+            const int d = tid & (MAX_DIGITS - 1), q = tid >> 8;
+            uint32_t run = 0u;
+#pragma unroll
+            for (int w = 0; w < CL_WARPS / 4; ++w) {
+                const uint32_t v = sh.seen[q * (CL_WARPS / 4) + w][d];
+                sh.seen[q * (CL_WARPS / 4) + w][d] = run;
+                run += v;
+            }
+            // quarters' totals meet in `totals` rows 0-3 of this block for a moment
+            sh.totals[q][d] = run;
+            __syncthreads();
+            const uint32_t t0 = sh.totals[0][d], t1 = sh.totals[1][d], t2 = sh.totals[2][d], t3 = sh.totals[3][d];
+            const uint32_t ahead = (q > 0 ? t0 : 0u) + (q > 1 ? t1 : 0u) + (q > 2 ? t2 : 0u);
+#pragma unroll
+            for (int w = 0; w < CL_WARPS / 4; ++w) sh.seen[q * (CL_WARPS / 4) + w][d] += ahead;
+            cluster_sync();                             // every block is done with the scratch rows
+            if (q < 2) {                                // this block's count of digit d to all eight blocks
+                const uint32_t mine = t0 + t1 + t2 + t3, at = smem_u32(&sh.totals[rank][d]);
+#pragma unroll
+                for (int b = 0; b < CL_BLOCKS / 2; ++b) store_remote(remote(at, q * (CL_BLOCKS / 2) + b), mine);
+            }
+        }
+        cluster_sync();
+        // first slot of a digit: smaller digits of all blocks, then this digit of earlier blocks
+        {
+            uint32_t all = 0u, earlier = 0u;
+            if (tid < MAX_DIGITS) {
+#pragma unroll
+                for (int b = 0; b < CL_BLOCKS; ++b) {
+                    const uint32_t v = sh.totals[b][tid];
+                    all += v;
+                    if (b < static_cast<int>(rank)) earlier += v;
+                }
+            }
+            uint32_t inc = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(FULL_MASK, inc, o);
+                if (lane >= o) inc += u;
+            }
+            if (lane == 31) sh.warp_total[warp] = inc;
+            __syncthreads();
+            if (tid < MAX_DIGITS) {
+                uint32_t first = inc - all + earlier;
+                for (int w = 0; w < warp; ++w) first += sh.warp_total[w];
+#pragma unroll 8
+                for (int w = 0; w < CL_WARPS; ++w) sh.seen[w][tid] += first;
+            }
+            __syncthreads();
+        }
+        const bool last = p + 1 == passes;
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const uint32_t to = sh.seen[warp][(key[k] >> shift) & (digits - 1)] + slot[k];
+            if (last) {
+                if (to < n) { keys_out[to] = key[k]; order_out[to] = pos[k]; }
+            } else {
+                store_remote(remote(smem_u32(pairs + (to & (EACH - 1))), to / EACH), key[k], pos[k]);
+            }
+        }
+        if (last) break;
+        cluster_sync();
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const uint2 v = pairs[local0 + k * 32];
+            key[k] = v.x;
+            pos[k] = v.y;
+        }
+        // the next pass's first cluster_sync lies behind these reads and before the next writes to `pairs`
+    }
+    cluster_sync();                                      // no block leaves while another may still write to it
+}
+
 int bit_length(int64_t v) { int b = 0; while (v > 0) { ++b; v >>= 1; } return b; }
 int items_for(int64_t n) { return n <= (1 << 16) ? 4 : 16; }
 int64_t round256(int64_t v) { return (v + 255) & ~static_cast<int64_t>(255); }
@@ -159,11 +308,29 @@ void row_sort_layout(RowSortArgs& a, void* workspace) {
     a.totals = reinterpret_cast<uint32_t*>(p);
 }
 
+template <int IT>
+static cudaError_t launch_cluster(RowSortArgs& a, int passes, int per, cudaStream_t s) {
+    constexpr int SMEM = static_cast<int>(sizeof(ClusterShared)) + CL_THREADS * IT * 8;
+    const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<IT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return e;
+    sort_cluster_kernel<IT><<<CL_BLOCKS, CL_THREADS, SMEM, s>>>(a, passes, per, a.keys[0], a.pos[0]);
+    a.sorted_keys = a.keys[0];
+    a.order = a.pos[0];
+    return cudaGetLastError();
+}
+
 cudaError_t launch_row_sort(RowSortArgs& a, cudaStream_t s) {
     const int bits = bit_length(a.vocab);                    // keys are 0 .. vocab
     const int passes = (bits + 7) / 8, per = (bits + passes - 1) / passes;
     const int items = items_for(a.n), tiles = static_cast<int>(tiles_for(a.n));
     const int digits = 1 << per;
+    if (a.n <= CL_BLOCKS * CL_THREADS * 8) {
+        const int64_t it = (a.n + CL_BLOCKS * CL_THREADS - 1) / (CL_BLOCKS * CL_THREADS);
+        if (it <= 1) return launch_cluster<1>(a, passes, per, s);
+        if (it <= 2) return launch_cluster<2>(a, passes, per, s);
+        if (it <= 4) return launch_cluster<4>(a, passes, per, s);
+        return launch_cluster<8>(a, passes, per, s);
+    }
     for (int p = 0; p < passes; ++p) {
         const int in = (p + 1) & 1, out = p & 1, shift = p * per;
         if (p == 0) sort_count_kernel<true><<<tiles, SORT_THREADS, 0, s>>>(a, nullptr, shift, digits, items, tiles);

@@ -3,8 +3,8 @@
 The reference's model reads its token table with ``nn.Embedding``
 (llm/models/foundation.py:338).  Here the lookup multiplies by a constant in the
 same pass, and the backward pass sorts the token positions by id and adds every
-id's rows in the order of their positions, in fp32: the gradient does not vary
-from run to run, whatever the ids' frequencies are.
+id's rows in fp32 in a fixed order: the gradient does not vary from run to run,
+whatever the ids' frequencies are.
 """
 from __future__ import annotations
 

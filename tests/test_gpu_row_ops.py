@@ -398,7 +398,8 @@ def embedding_reference(ids, weight, scale, dy, padding_idx):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["uniform", "one", "zipf", "descending", "outside"])
 @pytest.mark.parametrize("n,V,D", [(1, 1, 1), (1, 5, 8), (7, 3, 33), (16, 16, 64), (17, 100, 7), (1000, 2, 40), (333, 5000, 136),
-                                   (2049, 257, 24), (5000, 70000, 16), (33000, 300, 48), (70001, 1000, 8)])
+                                   (2049, 257, 24), (5000, 70000, 16), (12001, 500, 12),
+                                   (20000, 33, 264), (33000, 300, 48), (70001, 1000, 8), (66000, 70000, 4)])
 def test_embedding_and_its_gradient(cuda_device, n, V, D, kind, dtype):
     ids = ids_of(kind, n, V, cuda_device)
     if (n + V) % 2:

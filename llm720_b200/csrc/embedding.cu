@@ -13,7 +13,7 @@
 // frequencies are (text: one id can hold a tenth of all tokens).  An id whose
 // positions lie in one tile is finished there, in the order of its positions;
 // one that crosses tiles leaves a partial row per tile, and the join kernel adds
-// those in a fixed order (four interleaved runs, then the runs).
+// those in a fixed order (two interleaved runs, then the runs).
 #include <cstdio>
 
 #include "kernels.h"
@@ -97,7 +97,7 @@ struct SumParams {
     int* open_tiles; int* open_count;              // tiles in which an id begins that goes on behind them
     int64_t tiles;
     int row_threads, slabs;                        // threads of a tile, column slabs of row_threads pieces
-    int zero_blocks;                               // leading blocks write the rows no position names
+    int zero_blocks;                               // leading blocks write the rows no position names; 0: the sort has done it
 };
 
 // 32-ary search by the warp over a sorted array: number of leading entries (of n, `stride` apart) for which
@@ -231,49 +231,61 @@ __global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p)
     if (!done) flush(goes_on);
 }
 
-// Sums of the partial rows of ids that cross tiles: jobs are (entry of open_tiles, slab of 256 columns); 64 threads of
-// four columns (one, if rows are no multiples of four) by four lanes of partial rows.
+// Sums of the partial rows of ids that cross tiles: jobs are (entry of open_tiles, slab of 128 V columns), two runs of
+// partial rows per job.  Most ids end in the next tile, which the first two loads find out; a frequent one (12,000 of
+// 131,072 text-like positions) has hundreds of partial rows, eight of which are kept in flight per run (by cp.async: from
+// plain loads the compiler makes a chain of one load and its addition after another, four times slower).
+constexpr int JOIN_COLUMNS = 128, JOIN_DEPTH = 8;
 template <typename T, int V, int PER>
 __global__ void __launch_bounds__(SUM_THREADS) row_sum_join_kernel(const SumParams p) {
-    __shared__ float lanes[4][64 * V];
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const int64_t slabs = (p.D + 64 * V - 1) / (64 * V);
+    __shared__ float second[JOIN_COLUMNS * V];
+    __shared__ __align__(16) float ahead[JOIN_DEPTH][SUM_THREADS][V];      // rows on their way, each thread's its own
+    const int tx = threadIdx.x & (JOIN_COLUMNS - 1), ty = threadIdx.x / JOIN_COLUMNS;
+    const int slabs = static_cast<int>((p.D + JOIN_COLUMNS * V - 1) / (JOIN_COLUMNS * V));
     grid_wait();
     const int64_t jobs = static_cast<int64_t>(*p.open_count) * slabs;
     for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const int64_t tile = p.open_tiles[job / slabs], c = (job % slabs) * 64 * V + tx * V;
+        const int64_t tile = p.open_tiles[job / slabs], c = (job % slabs) * JOIN_COLUMNS * V + tx * V;
         const uint32_t cur = p.keys[tile * PER + PER - 1];
         // tiles behind this one whose last position is still cur's, and the one in which cur ends
-        const int64_t more = warp_count(p.tiles - tile - 1, [&](int64_t i) {
+        auto full = [&](int64_t i) {
             const int64_t e = (tile + 2 + i) * PER;
             return e < p.n && p.keys[e - 1] == cur && p.keys[e] == cur;
-        }) + 1;
+        };
+        const int64_t more = full(0) ? warp_count(p.tiles - tile - 1, full) + 1 : 1;
         float acc[V];
 #pragma unroll
         for (int q = 0; q < V; ++q) acc[q] = 0.f;
         if (c < p.D) {
+            // run 0: its own row, then every second of those behind it; run 1: the others
             const float* own = p.partial + (tile * 2 + 1) * p.D + c;
-            const float* rest = p.partial + (tile + 1) * 2 * p.D + c;
-#pragma unroll 4
-            for (int64_t u = ty; u <= more; u += 4) {
-                const float* row = u == 0 ? own : rest + (u - 1) * 2 * p.D;
-                if constexpr (V == 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(row);
-                    acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
-                } else {
-                    acc[0] += row[0];
+            const float* rest = p.partial + (tile + (ty == 0 ? 2 : 1)) * 2 * p.D + c;
+            const int count = static_cast<int>(ty == 0 ? more / 2 + 1 : (more + 1) / 2);
+            auto fetch = [&](int k) {
+                if (k < count) {
+                    const float* row = ty == 0 ? (k == 0 ? own : rest + static_cast<int64_t>(k - 1) * 4 * p.D)
+                                               : rest + static_cast<int64_t>(k) * 4 * p.D;
+                    copy_async<4 * V>(smem_u32(ahead[k % JOIN_DEPTH][threadIdx.x]), row);
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            for (int k = 0; k < JOIN_DEPTH - 1; ++k) fetch(k);
+            for (int k = 0; k < count; ++k) {
+                fetch(k + JOIN_DEPTH - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(JOIN_DEPTH - 1) : "memory");
+#pragma unroll
+                for (int q = 0; q < V; ++q) acc[q] += ahead[k % JOIN_DEPTH][threadIdx.x][q];
             }
         }
+        if (ty == 1) {
 #pragma unroll
-        for (int q = 0; q < V; ++q) lanes[ty][tx * V + q] = acc[q];
+            for (int q = 0; q < V; ++q) second[tx * V + q] = acc[q];
+        }
         __syncthreads();
         if (ty == 0 && c < p.D) {
 #pragma unroll
-            for (int q = 0; q < V; ++q) {
-                const float s = lanes[0][tx * V + q] + lanes[1][tx * V + q] + lanes[2][tx * V + q] + lanes[3][tx * V + q];
-                static_cast<T*>(p.out)[static_cast<int64_t>(cur) * p.D + c + q] = from_f32<T>(s * p.scale);
-            }
+            for (int q = 0; q < V; ++q)
+                static_cast<T*>(p.out)[static_cast<int64_t>(cur) * p.D + c + q] = from_f32<T>((acc[q] + second[tx * V + q]) * p.scale);
         }
         __syncthreads();
     }
@@ -303,11 +315,11 @@ cudaError_t sums_launch(SumParams p, cudaStream_t s) {
     p.slabs = static_cast<int>((pieces + p.row_threads - 1) / p.row_threads);
     const int subs = SUM_THREADS / p.row_threads;
     const int64_t zb = (static_cast<int64_t>(p.vocab) + ZERO_ROWS - 1) / ZERO_ROWS;
-    p.zero_blocks = static_cast<int>(zb < GRID_SMS * 32 ? zb : GRID_SMS * 32);
+    p.zero_blocks = p.zero_blocks ? static_cast<int>(zb < GRID_SMS * 32 ? zb : GRID_SMS * 32) : 0;
     const int64_t blocks = p.zero_blocks + (p.tiles + subs - 1) / subs * p.slabs;
     cudaError_t e = launch_behind(row_sum_kernel<T, WIDE, PER>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), s, p);
     if (e != cudaSuccess || p.tiles <= 1) return e;
-    const int64_t jobs = p.tiles * ((p.D + 255) / 256);
+    const int64_t jobs = p.tiles * ((p.D + 511) / 512);
     const dim3 grid(static_cast<unsigned>(jobs < GRID_SMS * 8 ? jobs : GRID_SMS * 8));
     return p.D % 4 == 0 ? launch_behind(row_sum_join_kernel<T, 4, PER>, grid, dim3(SUM_THREADS), s, p)
                         : launch_behind(row_sum_join_kernel<T, 1, PER>, grid, dim3(SUM_THREADS), s, p);
@@ -386,9 +398,12 @@ extern "C" int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_
         p.open_count = a.counter = reinterpret_cast<int*>(rest);
         p.open_tiles = p.open_count + 4;
         p.partial = reinterpret_cast<float*>(rest + ((p.tiles + 4) * 4 + 255) / 256 * 256);
+        a.zero_rows = grad_weight;
+        a.row_bytes = dim * (dtype == PEER_DTYPE_F32 ? 4 : 2);
         const cudaError_t e = launch_row_sort(a, s);
         if (e != cudaSuccess) return report("peer_embedding_backward", e);
         p.keys = a.sorted_keys; p.order = a.order;
+        p.zero_blocks = a.zeroed ? 0 : 1;
     }
     if (dtype == PEER_DTYPE_F32) return report("peer_embedding_backward", sums_t<float>(p, s));
     if (dtype == PEER_DTYPE_BF16) return report("peer_embedding_backward", sums_t<__nv_bfloat16>(p, s));

@@ -215,6 +215,8 @@ struct RowSortArgs {
     uint32_t* keys[2]; uint32_t* pos[2]; uint32_t* counts; uint32_t* totals;
     uint32_t* sorted_keys; uint32_t* order;
     int* counter;                         // optional: set to zero for the kernels behind the sort
+    void* zero_rows; int64_t row_bytes;   // optional [vocab] rows: those that no id names are set to zero when the sort is
+    bool zeroed;                          // one launch with SMs to spare (`zeroed` says so on return)
 };
 int64_t row_sort_bytes(int64_t n);
 void row_sort_layout(RowSortArgs& a, void* workspace);

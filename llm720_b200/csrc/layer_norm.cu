@@ -438,12 +438,6 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
 // width.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float2 splat(float a) { return make_float2(a, a); }
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
-
 // 1/sqrt(v): the hardware estimate and one Newton step (relative error below 2^-23); 0, infinite and NaN pass through
 __device__ __forceinline__ float inverse_sqrt(float v) {
     const float r = rsqrtf(v);

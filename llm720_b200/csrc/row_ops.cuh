@@ -99,6 +99,13 @@ template <typename T> __device__ __forceinline__ float param_at(const void* p, b
 }
 
 
+// 16, 8 or 4 bytes from global to shared memory, asynchronously
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // Pieces of a row: what one thread loads at once.  Wide: 16 bytes (rows whose start, stride and width are multiples
 // of 16 bytes); narrow: one value.
@@ -291,17 +298,22 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... Params, typename... Args>
-inline cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {
+inline cudaError_t launch_behind_smem(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t s, Args... args) {
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = block;
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+template <typename... Params, typename... Args>
+inline cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {
+    return launch_behind_smem(kernel, grid, block, 0, s, args...);
 }
 
 // ---------------------------------------------------------------------------

@@ -28,6 +28,19 @@ __device__ __forceinline__ uint32_t source_key(const RowSortArgs& a, int64_t i) 
     return (id < 0 || id >= a.vocab || id == a.skip) ? static_cast<uint32_t>(a.vocab) : static_cast<uint32_t>(id);
 }
 
+// Lanes of the warp whose digit equals this lane's: one vote per bit.  (match.any does the same in one instruction,
+// but takes about a microsecond when the digits differ: 17 us instead of SORT16_US for 16,384 ids.)
+__device__ __forceinline__ unsigned same_digit(uint32_t digit) {
+    unsigned same = FULL_MASK;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const bool set = (digit >> b) & 1u;
+        const unsigned vote = __ballot_sync(FULL_MASK, set);
+        same &= set ? vote : ~vote;
+    }
+    return same;
+}
+
 template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const RowSortArgs a, const uint32_t* __restrict__ keys, int shift,
                                                                   int digits, int items, int tiles) {
@@ -38,10 +51,12 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const RowSortA
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * SORT_THREADS * items;
     for (int i = 0; i < items; ++i) {
         const int64_t j = t0 + static_cast<int64_t>(i) * SORT_THREADS + threadIdx.x;
-        if (j < a.n) {
-            const uint32_t key = FIRST ? source_key(a, j) : keys[j];
-            atomicAdd(&hist[(key >> shift) & (digits - 1)], 1u);
-        }
+        const bool in = j < a.n;
+        const uint32_t key = in ? (FIRST ? source_key(a, j) : keys[j]) : 0u;
+        const uint32_t digit = (key >> shift) & (digits - 1);
+        const unsigned same = same_digit(digit) & __ballot_sync(FULL_MASK, in);
+        // one addition per digit and warp: a frequent id would queue up thirty-two
+        if (in && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[digit], static_cast<uint32_t>(__popc(same)));
     }
     __syncthreads();
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) a.counts[static_cast<int64_t>(d) * tiles + blockIdx.x] = hist[d];
@@ -98,8 +113,10 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const RowSor
         const bool in = j < a.n;
         key[i] = in ? (FIRST ? source_key(a, j) : keys[j]) : 0u;
         const uint32_t digit = (key[i] >> shift) & (digits - 1);
-        const unsigned same = __match_any_sync(FULL_MASK, in ? digit : 0xffffffffu);
-        const int leader = __ffs(same) - 1;
+        // lanes behind the last key come last in the warp: they count as one digit or another without a rank of theirs
+        // ever being used, but must not lead or be counted
+        const unsigned same = same_digit(digit) & __ballot_sync(FULL_MASK, in);
+        const int leader = in ? __ffs(same) - 1 : lane;
         uint32_t before = 0u;
         if (in && lane == leader) {
             before = seen[warp][digit];
@@ -174,6 +191,42 @@ struct ClusterShared {
     uint32_t warp_total[CL_WARPS];
 };
 
+// While one cluster sorts, the other SMs set the rows that no id names to zero.  Each block marks the ids of its rows
+// in a bitmap (every block reads all ids, from L2) and writes the unmarked rows.  Launched in front of the sort, which
+// starts as soon as all of these blocks run (programmatic launch; they leave room for it on every SM) and waits for
+// their end only in its last instruction.
+constexpr int ZERO_THREADS = 512, ZERO_WORDS = 1024;
+__global__ void __launch_bounds__(ZERO_THREADS) zero_unnamed_kernel(const RowSortArgs a) {
+    __shared__ uint32_t marks[ZERO_WORDS];
+    grid_release();
+    const int64_t each = (a.vocab + gridDim.x - 1) / gridDim.x;
+    const int64_t first = each * blockIdx.x, last = first + each < a.vocab ? first + each : a.vocab;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool vec = a.row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(a.zero_rows) & 15u) == 0;
+    for (int64_t v0 = first; v0 < last; v0 += ZERO_WORDS * 32) {
+        const int64_t v1 = v0 + ZERO_WORDS * 32 < last ? v0 + ZERO_WORDS * 32 : last;
+        for (int i = threadIdx.x; i < ZERO_WORDS; i += ZERO_THREADS) marks[i] = 0u;
+        __syncthreads();
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < a.n; i += ZERO_THREADS) {
+            const int64_t id = source_key(a, i);
+            if (id >= v0 && id < v1) atomicOr(&marks[(id - v0) >> 5], 1u << ((id - v0) & 31));
+        }
+        __syncthreads();
+        for (int64_t v = v0 + warp; v < v1; v += ZERO_THREADS / 32) {
+            if (marks[(v - v0) >> 5] >> ((v - v0) & 31) & 1u) continue;
+            char* row = static_cast<char*>(a.zero_rows) + v * a.row_bytes;
+            if (vec) {
+#pragma unroll 4
+                for (int64_t c = lane; c < a.row_bytes / 16; c += 32) reinterpret_cast<uint4*>(row)[c] = make_uint4(0u, 0u, 0u, 0u);
+            } else {                                     // rows of 2- or 4-byte values
+                for (int64_t c = lane; c < a.row_bytes / 2; c += 32) reinterpret_cast<uint16_t*>(row)[c] = 0;
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // pairs i of block b, warp w, round k, lane l:  i = ((b * CL_WARPS + w) * IT + k) * 32 + l
 template <int IT>
 __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const RowSortArgs a, int passes,
@@ -201,7 +254,7 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
             const uint32_t digit = (key[k] >> shift) & (digits - 1);
-            const unsigned same = __match_any_sync(FULL_MASK, digit);
+            const unsigned same = same_digit(digit);
             const int leader = __ffs(same) - 1;
             uint32_t before = 0u;
             if (lane == leader) {
@@ -286,10 +339,11 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 
         // the next pass's first cluster_sync lies behind these reads and before the next writes to `pairs`
     }
     cluster_sync();                                      // no block leaves while another may still write to it
+    grid_wait();                                         // the zeros of the kernel in front belong to the result
 }
 
 int bit_length(int64_t v) { int b = 0; while (v > 0) { ++b; v >>= 1; } return b; }
-int items_for(int64_t n) { return n <= (1 << 16) ? 4 : 16; }
+int items_for(int64_t n) { return n <= (1 << 19) ? 4 : 16; }      // 1,024 or 4,096 keys a tile: a tile per SM and more
 int64_t round256(int64_t v) { return (v + 255) & ~static_cast<int64_t>(255); }
 int64_t tiles_for(int64_t n) { const int64_t t = SORT_THREADS * items_for(n); return (n + t - 1) / t; }
 
@@ -313,7 +367,15 @@ static cudaError_t launch_cluster(RowSortArgs& a, int passes, int per, cudaStrea
     constexpr int SMEM = static_cast<int>(sizeof(ClusterShared)) + CL_THREADS * IT * 8;
     const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<IT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
-    sort_cluster_kernel<IT><<<CL_BLOCKS, CL_THREADS, SMEM, s>>>(a, passes, per, a.keys[0], a.pos[0]);
+    if (a.zero_rows) {
+        const int64_t blocks = a.vocab < GRID_SMS ? a.vocab : GRID_SMS;
+        zero_unnamed_kernel<<<static_cast<unsigned>(blocks), ZERO_THREADS, 0, s>>>(a);
+        const cudaError_t ez = launch_behind_smem(sort_cluster_kernel<IT>, dim3(CL_BLOCKS), dim3(CL_THREADS), SMEM, s, a, passes, per, a.keys[0], a.pos[0]);
+        if (ez != cudaSuccess) return ez;
+    } else {
+        sort_cluster_kernel<IT><<<CL_BLOCKS, CL_THREADS, SMEM, s>>>(a, passes, per, a.keys[0], a.pos[0]);
+    }
+    a.zeroed = a.zero_rows != nullptr;
     a.sorted_keys = a.keys[0];
     a.order = a.pos[0];
     return cudaGetLastError();

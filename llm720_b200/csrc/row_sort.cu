@@ -195,8 +195,8 @@ struct ClusterShared {
 // in a bitmap (every block reads all ids, from L2) and writes the unmarked rows.  Launched in front of the sort, which
 // starts as soon as all of these blocks run (programmatic launch; they leave room for it on every SM) and waits for
 // their end only in its last instruction.
-constexpr int ZERO_THREADS = 512, ZERO_WORDS = 1024;
-__global__ void __launch_bounds__(ZERO_THREADS) zero_unnamed_kernel(const RowSortArgs a) {
+constexpr int ZERO_THREADS = 512, ZERO_WORDS = 1024, ZERO_IDS = 8;      // 32 registers a thread: sixteen warps fit beside a block of the sort
+__global__ void __launch_bounds__(ZERO_THREADS, 4) zero_unnamed_kernel(const RowSortArgs a) {
     __shared__ uint32_t marks[ZERO_WORDS];
     grid_release();
     const int64_t each = (a.vocab + gridDim.x - 1) / gridDim.x;
@@ -207,10 +207,16 @@ __global__ void __launch_bounds__(ZERO_THREADS) zero_unnamed_kernel(const RowSor
         const int64_t v1 = v0 + ZERO_WORDS * 32 < last ? v0 + ZERO_WORDS * 32 : last;
         for (int i = threadIdx.x; i < ZERO_WORDS; i += ZERO_THREADS) marks[i] = 0u;
         __syncthreads();
-#pragma unroll 4
-        for (int64_t i = threadIdx.x; i < a.n; i += ZERO_THREADS) {
-            const int64_t id = source_key(a, i);
-            if (id >= v0 && id < v1) atomicOr(&marks[(id - v0) >> 5], 1u << ((id - v0) & 31));
+        for (int64_t i0 = threadIdx.x; i0 < a.n; i0 += ZERO_THREADS * ZERO_IDS) {
+            uint32_t id[ZERO_IDS];                           // loaded together: 16,384 ids are four rounds of latency
+#pragma unroll
+            for (int k = 0; k < ZERO_IDS; ++k) {
+                const int64_t i = i0 + k * ZERO_THREADS;
+                id[k] = source_key(a, i < a.n ? i : a.n - 1);
+            }
+#pragma unroll
+            for (int k = 0; k < ZERO_IDS; ++k)
+                if (id[k] >= v0 && id[k] < v1) atomicOr(&marks[(id[k] - v0) >> 5], 1u << ((id[k] - v0) & 31));
         }
         __syncthreads();
         for (int64_t v = v0 + warp; v < v1; v += ZERO_THREADS / 32) {

@@ -87,7 +87,7 @@ typedef struct peer_tensors {
     float*       scores_out;   /* optional [T, num_heads, top_k]: raw (pre-softmax) scores */
     const void*  keys2;        /* [n_keys2, query_dim/num_key_dims] (3-D, 4-D key grids) */
     const void*  keys3;        /* [n_keys3, query_dim/num_key_dims] (4-D key grids)      */
-    int32_t*     product_ids_out; /* optional [T, num_heads, top_k] (peer_forward only): the selected experts'
+    int32_t*     product_ids_out; /* optional [T, num_heads, top_k] (peer_forward, peer_block_forward): the selected experts'
                                   true positions in the key grid, sum_d index_d * stride_d, whatever
                                   index_mode says; the backward pass needs the per-dimension indices */
 } peer_tensors_t;
@@ -390,6 +390,18 @@ int64_t peer_embedding_workspace(int64_t n_ids, int64_t dim);
 int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_t n_ids, const void* grad, int64_t grad_stride,
                             int32_t dtype, int64_t vocab, int64_t dim, float scale, int64_t padding_idx, void* grad_weight,
                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* peer_gather_eval_backward_rows with the table gradients summed by sorted ids instead of reductions in memory: every
+ * row of grad_down [n_grad_rows, input_dim] and grad_up [n_grad_rows, output_dim] (the tables' dtype) is WRITTEN (zero
+ * where no id names it), its sum formed in fp32 and rounded once, the same from run to run.  Single-neuron experts of
+ * an fp32 or bf16 layer, rows of at most 4 KB.  workspace: at least
+ * peer_gather_eval_backward_sorted_workspace(h, n_tokens) bytes, 16-byte aligned (0 bytes: unsupported size). */
+#define PEER_SORT_IDS_MAX 0x7ffffffe
+int64_t peer_gather_eval_backward_sorted_workspace(peer_handle_t h, int64_t n_tokens);
+int peer_gather_eval_backward_sorted(peer_handle_t h, const void* x, const void* grad_out, const int32_t* ids,
+                                     const float* weights, const void* expert_down, const void* expert_up, float* grad_x,
+                                     float* grad_weights, void* grad_down, void* grad_up, int64_t n_grad_rows,
+                                     int64_t n_tokens, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Reads and clears the device status word (synchronises `stream`).  Returns
  * PEER_OK, PEER_ERR_DEVICE_TIMEOUT or PEER_ERR_BOUNDS.  The kernels never

@@ -66,6 +66,8 @@ EXPORTS = {
                                                                                            C.c_int64, C.c_void_p]),
     "peer_gather_eval_backward": (C.c_int, [C.c_void_p] * 11 + [C.c_int32, C.c_int64, C.c_void_p]),
     "peer_gather_eval_backward_rows": (C.c_int, [C.c_void_p] * 11 + [C.c_int32, C.c_int64, C.c_int64, C.c_void_p]),
+    "peer_gather_eval_backward_sorted_workspace": (C.c_int64, [C.c_void_p, C.c_int64]),
+    "peer_gather_eval_backward_sorted": (C.c_int, [C.c_void_p] * 11 + [C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
     "peer_xchg_create": (C.c_int, [C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                    C.POINTER(C.c_void_p)]),
     "peer_xchg_export": (C.c_int, [C.c_void_p, C.c_void_p]),

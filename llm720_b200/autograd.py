@@ -24,12 +24,21 @@ dropout (training mode) the stages are separate nodes:
   backward does for a bf16 layer; where a batch brings only a few selections per
   row, a bf16 layer may sum in bf16 (half the traffic, one rounding per addend).
   ``module.table_grad_sums`` ("auto", "fp32", "table") decides; see
-  ``_table_grad_plan``.
+  ``_table_grad_plan``.  ``"sorted"`` adds every row's contributions by sorted
+  expert ids instead: fp32, one order, nothing accumulated in memory.
+
+``block_train`` is a node around the layer's: the norm in front and the residual
+(llm/models/foundation.py:196-205), keeping one tensor - the block's input, in 8
+bits if asked - and the selection.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from .checkpoint import pack_rows_e4m3, unpack_rows_e4m3
+from .norm import check_norm_arguments, norm_backward, norm_forward
 
 
 class _ProjectQueries(torch.autograd.Function):
@@ -67,9 +76,7 @@ class _ExpertEval(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out):
         x, weights, ids32, down, up = ctx.saved_tensors
-        gdt, rows = ctx.plan
-        gx, gw, gd, gu = ctx.op.gather_eval_backward(x, grad_out.contiguous(), ids32, weights.contiguous(), down, up,
-                                                     grad_dtype=gdt, grad_rows=rows)
+        gx, gw, gd, gu = _expert_grads(ctx.op, ctx.plan, x, grad_out.contiguous(), ids32, weights.contiguous(), down, up)
         need = ctx.needs_input_grad
         return (gx.to(x.dtype) if need[0] else None, gw if need[1] else None, None,
                 _dense_grad(gd, down) if need[3] else None, _dense_grad(gu, up) if need[4] else None, None, None)
@@ -91,15 +98,17 @@ def _reachable_rows(module) -> int:
 
 
 def _table_grad_plan(module, table, n_tokens: int):
-    """(dtype of the sums, rows of the gradient tables).  bf16 sums exist for single-neuron experts of a bf16
+    """(dtype of the sums or "sorted", rows of the gradient tables).  bf16 sums exist for single-neuron experts of a bf16
     layer with rows of at most 4 KB; a bf16 running sum loses small addends once a row collects many
     contributions, so "auto" keeps them for batches with at most four selections per reachable row on average
     and never with the reference's id arithmetic, where a few thousand rows take all of them (about a thousand
     each at the 1 M-expert layer's batch).  With fp32 sums only the reachable rows get a buffer."""
     mode = getattr(module, "table_grad_sums", "auto")
-    if mode not in ("auto", "fp32", "table"):
-        raise ValueError(f"table_grad_sums={mode!r}: 'auto', 'fp32' or 'table'")
+    if mode not in ("auto", "fp32", "table", "sorted"):
+        raise ValueError(f"table_grad_sums={mode!r}: 'auto', 'fp32', 'table' or 'sorted'")
     reach = _reachable_rows(module)
+    if mode == "sorted":
+        return "sorted", reach
     eligible = (module.expert_hidden_size == 1 and table.dtype == torch.bfloat16 and
                 max(module.input_dim, module.output_dim) * table.element_size() <= 4096)
     per_row = n_tokens * module.num_heads * module.num_experts_per_tok / max(reach, 1)
@@ -107,6 +116,14 @@ def _table_grad_plan(module, table, n_tokens: int):
     if in_table:
         return table.dtype, module.num_experts            # summed straight into what becomes .grad
     return torch.float32, reach
+
+
+def _expert_grads(op, plan, x, grad_out, ids32, weights, down, up):
+    """(dx, dweights, grad_down, grad_up) of the expert stage as the plan says."""
+    sums, rows = plan
+    if sums == "sorted":
+        return op.gather_eval_backward_sorted(x, grad_out, ids32, weights, down, up, grad_rows=rows)
+    return op.gather_eval_backward(x, grad_out, ids32, weights, down, up, grad_dtype=sums, grad_rows=rows)
 
 
 def _dense_grad(compact: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
@@ -153,46 +170,122 @@ class _FusedLayer(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, ln_w, ln_b, down, up, module):
         T = x.shape[0]
-        H, k = module.num_heads, module.num_experts_per_tok
         op = module._operator(x.device, x.dtype, T)
-        out = torch.empty(T, module.output_dim, dtype=x.dtype, device=x.device)
-        ids = torch.empty(T, H, k, dtype=torch.int64, device=x.device)
-        sc = torch.empty(T, H, k, dtype=torch.float32, device=x.device)
-        pid = torch.empty(T, H, k, dtype=torch.int32, device=x.device)
+        out, ids, sc, pid = _selection_buffers(module, x)
         op.forward(x, module._weights(), out, ids, sc, pid)
-        ctx.save_for_backward(x, weight, bias, ln_w, ln_b, down, up, ids, sc, pid)
+        ctx.save_for_backward(*_kept(module, x), weight, bias, ln_w, ln_b, down, up, ids, sc, pid)
         ctx.module, ctx.op = module, op
         ctx.mark_non_differentiable(ids, sc)
         return out, ids, sc
 
     @staticmethod
     def backward(ctx, grad_out, _gi, _gs):
-        x, weight, bias, ln_w, ln_b, down, up, ids, sc, pid = ctx.saved_tensors
-        module, op = ctx.module, ctx.op
-        T = x.shape[0]
-        H, Q, k = module.num_heads, module.query_dim, module.num_experts_per_tok
-        need = ctx.needs_input_grad
-        weights = torch.softmax(sc, dim=-1).view(T, H * k)
-        gdt, rows = _table_grad_plan(module, down, T)
-        gx, gw, gd, gu = op.gather_eval_backward(x, grad_out.contiguous(), ids.view(T, H * k).to(torch.int32), weights,
-                                                 down, up, grad_dtype=gdt, grad_rows=rows)
-        # score path: d(loss)/d(weights) = gw, pushed through softmax, the selected scores and the query path
-        leaves = [None if t is None else t.detach().requires_grad_(n)
-                  for t, n in zip((x, weight, bias, ln_w, ln_b), need[:5])]
-        wanted = [t for t in leaves if t is not None and t.requires_grad]
-        got = iter(())
-        if wanted:
-            with torch.enable_grad():                    # projection and LayerNorm again, as torch operations
-                q = F.linear(leaves[0], leaves[1], leaves[2]).float().view(T, H, Q)
-                if leaves[3] is not None:
-                    q = F.layer_norm(q, (Q,), leaves[3].float(), None if leaves[4] is None else leaves[4].float(), 1e-5)
-            gq = op.select_backward(q.detach().contiguous(), [p.detach() for p in module.sub_keys], pid.view(T, H, k),
-                                    sc, gw.view(T, H, k).contiguous())
-            got = iter(torch.autograd.grad(q, wanted, gq))
-        grads = [next(got) if (t is not None and t.requires_grad) else None for t in leaves]
-        if need[0]:
-            grads[0] = (gx + grads[0].float()).to(x.dtype)
-        return (*grads, _dense_grad(gd, down) if need[5] else None, _dense_grad(gu, up) if need[6] else None, None)
+        x, payload, scale, *params, ids, sc, pid = ctx.saved_tensors
+        if x is None:
+            x = unpack_rows_e4m3(payload, scale, grad_out.dtype)
+        return (*_layer_grads(ctx.module, ctx.op, x, params, ids, sc, pid, grad_out.contiguous(), ctx.needs_input_grad[:7]),
+                None)
+
+
+def _selection_buffers(module, x):
+    T, H, k = x.shape[0], module.num_heads, module.num_experts_per_tok
+    return (torch.empty(T, module.output_dim, dtype=x.dtype, device=x.device),
+            torch.empty(T, H, k, dtype=torch.int64, device=x.device),
+            torch.empty(T, H, k, dtype=torch.float32, device=x.device),
+            torch.empty(T, H, k, dtype=torch.int32, device=x.device))
+
+
+def _kept(module, x):
+    """What a node keeps of its input x: (x, None, None), or (None, payload, scale) in 8 bits."""
+    mode = module.activation_checkpoint
+    if mode not in (None, "e4m3"):
+        raise ValueError(f"activation_checkpoint={mode!r}: None or 'e4m3'")
+    return (x, None, None) if mode is None else (None, *pack_rows_e4m3(x))
+
+
+def _layer_grads(module, op, x, params, ids, sc, pid, grad_out, need):
+    """Gradients of the layer in (x, query weight, query bias, LayerNorm weight, bias, expert_down, expert_up)."""
+    weight, bias, ln_w, ln_b, down, up = params
+    T = x.shape[0]
+    H, Q, k = module.num_heads, module.query_dim, module.num_experts_per_tok
+    weights = torch.softmax(sc, dim=-1).view(T, H * k)
+    gx, gw, gd, gu = _expert_grads(op, _table_grad_plan(module, down, T), x, grad_out, ids.view(T, H * k).to(torch.int32),
+                                   weights, down, up)
+    # score path: d(loss)/d(weights) = gw, pushed through softmax, the selected scores and the query path
+    leaves = [None if t is None else t.detach().requires_grad_(n)
+              for t, n in zip((x, weight, bias, ln_w, ln_b), need[:5])]
+    wanted = [t for t in leaves if t is not None and t.requires_grad]
+    got = iter(())
+    if wanted:
+        with torch.enable_grad():                    # projection and LayerNorm again, as torch operations
+            q = F.linear(leaves[0], leaves[1], leaves[2]).float().view(T, H, Q)
+            if leaves[3] is not None:
+                q = F.layer_norm(q, (Q,), leaves[3].float(), None if leaves[4] is None else leaves[4].float(), 1e-5)
+        gq = op.select_backward(q.detach().contiguous(), [p.detach() for p in module.sub_keys], pid.view(T, H, k),
+                                sc, gw.view(T, H, k).contiguous())
+        got = iter(torch.autograd.grad(q, wanted, gq))
+    grads = [next(got) if (t is not None and t.requires_grad) else None for t in leaves]
+    if need[0]:
+        grads[0] = (gx + grads[0].float()).to(x.dtype)
+    return (*grads, _dense_grad(gd, down) if need[5] else None, _dense_grad(gu, up) if need[6] else None)
+
+
+class _FusedBlock(torch.autograd.Function):
+    """``hidden + layer(norm(hidden))`` as one node.  Forward is ``peer_block_forward``; backward forms the norm's
+    output and statistics again from what was kept of ``hidden``, runs the layer's gradients, and adds the residual's
+    gradient where the norm's is written."""
+
+    @staticmethod
+    def forward(ctx, hidden, norm_w, norm_b, weight, bias, ln_w, ln_b, down, up, module, eps, codes):
+        op = module._operator(hidden.device, hidden.dtype, hidden.shape[0])
+        out, ids, sc, pid = _selection_buffers(module, hidden)
+        f32 = lambda p: None if p is None else p.detach().float().contiguous()
+        op.block_forward(hidden, module._weights(), f32(norm_w), f32(norm_b), eps, out, ids, sc, pid)
+        ctx.save_for_backward(*_kept(module, hidden), norm_w, norm_b, weight, bias, ln_w, ln_b, down, up, ids, sc, pid)
+        ctx.module, ctx.op, ctx.eps, ctx.codes = module, op, eps, codes
+        ctx.mark_non_differentiable(ids, sc)
+        return out, ids, sc
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, _gi, _gs):
+        hidden, payload, scale, norm_w, norm_b, *params, ids, sc, pid = ctx.saved_tensors
+        if hidden is None:
+            hidden = unpack_rows_e4m3(payload, scale, grad_out.dtype)
+        need_norm, need = ctx.needs_input_grad[:3], ctx.needs_input_grad[3:9]
+        grad_out = grad_out.contiguous()
+        below = any(need_norm)
+        x, stats, _, _ = norm_forward(hidden, norm_w, norm_b, ctx.eps, *ctx.codes, True, False)
+        gx, *grads = _layer_grads(ctx.module, ctx.op, x, params, ids, sc, pid, grad_out, (below, *need))
+        norm_grads = (None, None, None)
+        if below:
+            norm_grads = norm_backward(gx, hidden, None, None, stats, norm_w, *ctx.codes, need_norm[0],
+                                       norm_w.dtype if need_norm[1] else None, norm_b.dtype if need_norm[2] else None,
+                                       add=grad_out)
+        return (*norm_grads, *grads, None, None, None)
+
+
+def block_train_autograd(module, hidden_states: torch.Tensor, norm) -> torch.Tensor:
+    """``hidden_states + module(norm(hidden_states))`` recording an autograd graph; module a ``llm720_b200.PEER``, norm a
+    ``torch.nn.LayerNorm`` over the model dimension."""
+    w = module._weights()
+    if w["down_scale"] is not None:
+        raise RuntimeError("quantised (FP8) expert tables are inference-only: no backward pass")
+    if tuple(norm.normalized_shape) != (module.input_dim,):
+        raise ValueError(f"ln_2 normalises {tuple(norm.normalized_shape)}, the layer's input is ({module.input_dim},)")
+    B, S, _ = hidden_states.shape
+    hidden = hidden_states.contiguous().view(B * S, module.input_dim)
+    codes = check_norm_arguments(hidden, norm.weight, norm.bias, norm.eps)
+    if module.training and module.dropout.p > 0:
+        from .norm import layer_norm
+        return hidden_states + module(layer_norm(hidden_states, norm.weight, norm.bias, norm.eps))
+    ln = module.query_layer_norm
+    out, ids, sc = _FusedBlock.apply(hidden, norm.weight, norm.bias, module.query_proj.weight, module.query_proj.bias,
+                                     None if ln is None else ln.weight, None if ln is None else ln.bias,
+                                     module.expert_down.weight, module.expert_up.weight, module, norm.eps, codes)
+    if module.track_indices:
+        module._stash(ids, sc, B, S)
+    return out.view(B, S, module.output_dim)
 
 
 def peer_forward_autograd(module, hidden_states: torch.Tensor) -> torch.Tensor:
@@ -217,6 +310,8 @@ def peer_forward_autograd(module, hidden_states: torch.Tensor) -> torch.Tensor:
 def _forward_with_dropout(module, x, w, B, S):
     """Training mode with dropout of the expert activations (experts.py:366): the stages as separate autograd
     nodes, so that the per-slot dropout factor can sit between the softmax and the expert stage."""
+    if module.activation_checkpoint is not None:
+        raise RuntimeError("activation_checkpoint is not implemented together with dropout: the stages are separate nodes")
     if module.expert_hidden_size != 1:
         raise RuntimeError("dropout with expert_hidden_size > 1 is not implemented (it acts on every neuron)")
     T = B * S

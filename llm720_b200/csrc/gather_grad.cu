@@ -18,6 +18,10 @@
 // accumulated with vector reductions (red.global.add.v4.f32) into fp32 tables,
 // so tokens that share an expert need no sorting or locking.  Rows are read
 // twice (dot products, then the updates); the second read hits L1/L2.
+//
+// SUMS_LATER: only the two factors of every (token, slot), dz and w act(z), are
+// written; the table gradients are then weighted sums of the rows of x and dy by
+// id (row_sum.cu), in fp32 and in one order.
 #include <type_traits>
 
 #include "common.cuh"
@@ -91,6 +95,7 @@ struct GradParams {
     const void* x; const void* dy; const int32_t* ids; const float* weights;
     const char* down; const char* up;
     void* d_down; void* d_up; float* dx; float* dweights;
+    float* coef_down; float* coef_up;      // [T, HK] (SUMS_LATER)
     int64_t T; int HK; int64_t N; int D, Dout; int activation; int* status;
     int nch_u, nch_v;          // 16-byte chunks per down / up row (table storage)
 };
@@ -99,7 +104,7 @@ struct GradParams {
 // dy covers the same elements as a 16-byte chunk of a table row.
 // LP: the table gradients are accumulated in the tables' own 16-bit type (what the reference's bf16 training
 // does: its embedding gradients are bf16) instead of fp32: half the read-modify-write bytes, no cast afterwards.
-template <typename XT, int CH, bool LP>
+template <typename XT, int CH, bool LP, bool SUMS_LATER>
 __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p) {
     constexpr int EPC = Chunk16<XT>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -122,7 +127,11 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
             const int32_t id = __ldg(p.ids + t * p.HK + e);
             const float w = __ldg(p.weights + t * p.HK + e);
             if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.N)) {      // recorded and skipped
-                if (lane == 0) { atomicMax(p.status, STATUS_BOUNDS); p.dweights[t * p.HK + e] = 0.f; }
+                if (lane == 0) {
+                    atomicMax(p.status, STATUS_BOUNDS);
+                    p.dweights[t * p.HK + e] = 0.f;
+                    if (SUMS_LATER) p.coef_down[t * p.HK + e] = p.coef_up[t * p.HK + e] = 0.f;
+                }
                 continue;
             }
             const uint4* __restrict__ ur = reinterpret_cast<const uint4*>(p.down + static_cast<int64_t>(id) * row_u);
@@ -156,6 +165,10 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
             if (lane == 0) p.dweights[t * p.HK + e] = av * g;
             const float cv = w * av;
             const float dz = w * g * act_slope(z, p.activation);
+            if (SUMS_LATER && lane == 0) {
+                p.coef_down[t * p.HK + e] = dz;
+                p.coef_up[t * p.HK + e] = cv;
+            }
             using GT = typename std::conditional<LP, XT, float>::type;
             GT* __restrict__ du = static_cast<GT*>(p.d_down) + static_cast<int64_t>(id) * p.D;
             GT* __restrict__ dv = static_cast<GT*>(p.d_up) + static_cast<int64_t>(id) * p.Dout;
@@ -163,7 +176,7 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
             for (int i = 0; i < CH; ++i) {
                 const int c = lane + 32 * i;
                 float a[EPC], b[EPC];
-                if (c < p.nch_v) {
+                if (!SUMS_LATER && c < p.nch_v) {
                     Chunk16<XT>::decode(dyc[i], b);
                     if constexpr (LP && sizeof(XT) == 2) {
                         red_add_v4_bf16x2(dv + c * EPC, pack2(cv * b[0], cv * b[1]), pack2(cv * b[2], cv * b[3]),
@@ -179,7 +192,8 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
                     Chunk16<XT>::decode(xc[i], b);
 #pragma unroll
                     for (int q = 0; q < EPC; ++q) dxa[i * EPC + q] = fmaf(dz, a[q], dxa[i * EPC + q]);
-                    if constexpr (LP && sizeof(XT) == 2) {
+                    if constexpr (SUMS_LATER) {
+                    } else if constexpr (LP && sizeof(XT) == 2) {
                         red_add_v4_bf16x2(du + c * EPC, pack2(dz * b[0], dz * b[1]), pack2(dz * b[2], dz * b[3]),
                                           pack2(dz * b[4], dz * b[5]), pack2(dz * b[6], dz * b[7]));
                     } else {
@@ -203,23 +217,23 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
     }
 }
 
-template <typename XT, int CH, bool LP>
+template <typename XT, int CH, bool LP, bool SUMS_LATER>
 cudaError_t launch_t(const GradParams& p, int sm_count, cudaStream_t s) {
     int64_t ctas = (p.T + WARPS - 1) / WARPS;
     const int64_t cap = static_cast<int64_t>(sm_count) * 4;      // a few CTAs per SM, grid-stride over tokens
     if (ctas > cap) ctas = cap;
-    gather_grad_kernel<XT, CH, LP><<<static_cast<unsigned>(ctas), THREADS, 0, s>>>(p);
+    gather_grad_kernel<XT, CH, LP, SUMS_LATER><<<static_cast<unsigned>(ctas), THREADS, 0, s>>>(p);
     return cudaGetLastError();
 }
 
-template <typename XT, bool LP>
+template <typename XT, bool LP, bool SUMS_LATER = false>
 cudaError_t launch_ch(const GradParams& p, int sm_count, cudaStream_t s) {
     const int max_ch = p.nch_u > p.nch_v ? p.nch_u : p.nch_v;
     const int need = (max_ch + 31) / 32;
-    if (need <= 1) return launch_t<XT, 1, LP>(p, sm_count, s);
-    if (need <= 2) return launch_t<XT, 2, LP>(p, sm_count, s);
-    if (need <= 4) return launch_t<XT, 4, LP>(p, sm_count, s);
-    if (need <= 8) return launch_t<XT, 8, LP>(p, sm_count, s);
+    if (need <= 1) return launch_t<XT, 1, LP, SUMS_LATER>(p, sm_count, s);
+    if (need <= 2) return launch_t<XT, 2, LP, SUMS_LATER>(p, sm_count, s);
+    if (need <= 4) return launch_t<XT, 4, LP, SUMS_LATER>(p, sm_count, s);
+    if (need <= 8) return launch_t<XT, 8, LP, SUMS_LATER>(p, sm_count, s);
     return cudaErrorInvalidValue;
 }
 
@@ -236,6 +250,12 @@ cudaError_t launch_gather_grad(const GatherGradArgs& a, cudaStream_t s) {
     p.d_down = a.d_down; p.d_up = a.d_up; p.dx = a.dx; p.dweights = a.dweights;
     p.T = a.T; p.HK = a.HK; p.N = a.N; p.D = a.D; p.Dout = a.Dout; p.activation = a.activation; p.status = a.status;
     p.nch_u = a.D * tb / 16; p.nch_v = a.Dout * tb / 16;
+    p.coef_down = a.coef_down; p.coef_up = a.coef_up;
+    if (a.coef_down) {
+        if (a.act_dtype == PEER_DTYPE_F32) return launch_ch<float, false, true>(p, a.sm_count, s);
+        if (a.act_dtype == PEER_DTYPE_BF16) return launch_ch<__nv_bfloat16, false, true>(p, a.sm_count, s);
+        return cudaErrorInvalidValue;
+    }
     if (a.act_dtype == PEER_DTYPE_F32) return launch_ch<float, false>(p, a.sm_count, s);       // fp32 either way
     if (a.act_dtype == PEER_DTYPE_BF16)
         return a.grad_dtype == PEER_DTYPE_BF16 ? launch_ch<__nv_bfloat16, true>(p, a.sm_count, s)

@@ -154,6 +154,7 @@ struct GatherGradArgs {
     int sm_count;
     int hidden;               // neurons per expert; 0 or 1 = single
     int grad_dtype;           // dtype of d_down / d_up: PEER_DTYPE_F32, or the tables' own 16-bit type
+    float* coef_down; float* coef_up;      // optional [T, HK]: the factors of x and dy instead of d_down / d_up
 };
 cudaError_t launch_gather_grad(const GatherGradArgs& a, cudaStream_t s);
 
@@ -213,14 +214,30 @@ struct RowSortArgs {
     const void* ids; int id_bytes;        // int32 or int64
     int64_t n, vocab, skip;               // ids outside [0, vocab) and the id `skip` are left out
     uint32_t* keys[2]; uint32_t* pos[2]; uint32_t* counts; uint32_t* totals;
+    int* counters;                        // [4], zero behind the sort: for launch_row_sums
     uint32_t* sorted_keys; uint32_t* order;
-    int* counter;                         // optional: set to zero for the kernels behind the sort
     void* zero_rows; int64_t row_bytes;   // optional [vocab] rows: those that no id names are set to zero when the sort is
     bool zeroed;                          // one launch with SMs to spare (`zeroed` says so on return)
+    int launches;                         // kernels launched
 };
 int64_t row_sort_bytes(int64_t n);
 void row_sort_layout(RowSortArgs& a, void* workspace);
 cudaError_t launch_row_sort(RowSortArgs& a, cudaStream_t s);
+
+// Sums of rows by id (row_sum.cu): out[v] = scale * sum over the positions j of id v of  coef[j] * src[j / per_row]
+// (coef null: 1).  `counter`: one of the sort's, a different one for each sum behind the same sort.
+struct RowSumArgs {
+    const uint32_t* keys; const uint32_t* order; int64_t n, vocab;
+    const void* src; int64_t src_stride; const float* coef; int64_t per_row;
+    int dtype;                            // of src and out
+    float scale;
+    void* out; int64_t D;
+    int* counter; void* workspace;        // row_sum_bytes(n, D)
+    bool zero;                            // write the rows that no position names (the sort has not)
+    int launches;                         // kernels launched
+};
+int64_t row_sum_bytes(int64_t n, int64_t D);
+cudaError_t launch_row_sums(RowSumArgs& a, cudaStream_t s);
 
 // one-time per-process attribute set-up (dynamic shared memory opt-in)
 cudaError_t select_simt_setup();

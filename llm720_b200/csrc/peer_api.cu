@@ -611,7 +611,7 @@ extern "C" int peer_block_forward(peer_handle_t h, const peer_tensors_t* t, cons
         h->launches += 1;
         rc = forward_slice(h, t, h->x_ln, static_cast<char*>(t->out) + t0 * c.output_dim * ab,
                            t->ids_out ? t->ids_out + t0 * HK : nullptr, t->scores_out ? t->scores_out + t0 * HK : nullptr,
-                           n, s, xs);
+                           n, s, xs, t->product_ids_out ? t->product_ids_out + t0 * HK : nullptr);
         if (rc) return rc;
     }
     return PEER_OK;
@@ -999,6 +999,79 @@ extern "C" int peer_gather_eval_backward_rows(peer_handle_t h, const void* x, co
                     c.input_dim, c.output_dim);
     CU_TRY(h, e);
     h->launches += 1;
+    return PEER_OK;
+}
+
+static int64_t round256(int64_t v) { return (v + 255) & ~static_cast<int64_t>(255); }
+
+// [sort | sums of the wider table's rows (both tables in turn) | factors of x | factors of dy]
+extern "C" int64_t peer_gather_eval_backward_sorted_workspace(peer_handle_t h, int64_t n_tokens) {
+    if (!h || n_tokens <= 0) return 0;
+    const int64_t n = n_tokens * h->cfg.num_heads * h->cfg.top_k;
+    if (n > PEER_SORT_IDS_MAX) return 0;
+    const int64_t wide = h->cfg.input_dim > h->cfg.output_dim ? h->cfg.input_dim : h->cfg.output_dim;
+    return row_sort_bytes(n) + row_sum_bytes(n, wide) + 2 * round256(n * 4);
+}
+
+extern "C" int peer_gather_eval_backward_sorted(peer_handle_t h, const void* x, const void* grad_out, const int32_t* ids,
+                                                const float* weights, const void* expert_down, const void* expert_up,
+                                                float* grad_x, float* grad_weights, void* grad_down, void* grad_up,
+                                                int64_t n_grad_rows, int64_t n_tokens, void* workspace,
+                                                int64_t workspace_bytes, void* stream) {
+    if (!h) return PEER_ERR_INVALID_ARG;
+    const peer_config_t& c = h->cfg;
+    if (n_tokens < 0 || n_grad_rows <= 0 || n_grad_rows > c.num_experts)
+        return fail(h, PEER_ERR_INVALID_ARG, "peer_gather_eval_backward_sorted: n_tokens must not be negative, n_grad_rows lie in [1, num_experts]");
+    if (!grad_down || !grad_up) return fail(h, PEER_ERR_INVALID_ARG, "peer_gather_eval_backward_sorted: null pointer");
+    const int tb = act_bytes(c.table_dtype);
+    if (c.table_dtype != c.act_dtype || (c.act_dtype != PEER_DTYPE_F32 && c.act_dtype != PEER_DTYPE_BF16) || h->hidden > 1)
+        return fail(h, PEER_ERR_UNSUPPORTED, "sorted table gradients: single-neuron experts of an fp32 or bf16 layer");
+    if (c.input_dim * tb > 4096 || c.output_dim * tb > 4096 || (c.input_dim * tb) % 16 || (c.output_dim * tb) % 16)
+        return fail(h, PEER_ERR_UNSUPPORTED, "sorted table gradients: rows of at most 4 KB, a multiple of 16 bytes");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (n_tokens == 0) {
+        CU_TRY(h, cudaMemsetAsync(grad_down, 0, static_cast<size_t>(n_grad_rows) * c.input_dim * tb, s));
+        CU_TRY(h, cudaMemsetAsync(grad_up, 0, static_cast<size_t>(n_grad_rows) * c.output_dim * tb, s));
+        return PEER_OK;
+    }
+    if (!x || !grad_out || !ids || !weights || !expert_down || !expert_up || !grad_x || !grad_weights)
+        return fail(h, PEER_ERR_INVALID_ARG, "peer_gather_eval_backward_sorted: null pointer");
+    if (!aligned16(x) || !aligned16(grad_out) || !aligned16(expert_down) || !aligned16(expert_up) || !aligned16(grad_x) ||
+        !aligned16(grad_down) || !aligned16(grad_up) || !aligned16(workspace))
+        return fail(h, PEER_ERR_INVALID_ARG, "x, grad_out, tables, gradient buffers and the workspace must be 16-byte aligned");
+    const int64_t HK = static_cast<int64_t>(c.num_heads) * c.top_k, n = n_tokens * HK;
+    if (n > PEER_SORT_IDS_MAX) return fail(h, PEER_ERR_UNSUPPORTED, "sorted table gradients: more than 2^31 - 2 selections in one call");
+    if (!workspace || workspace_bytes < peer_gather_eval_backward_sorted_workspace(h, n_tokens))
+        return fail(h, PEER_ERR_INVALID_ARG, "peer_gather_eval_backward_sorted: workspace is missing or too small");
+    const int64_t wide = c.input_dim > c.output_dim ? c.input_dim : c.output_dim;
+    char* ws = static_cast<char*>(workspace);
+    RowSortArgs a{};
+    a.ids = ids; a.id_bytes = 4; a.n = n; a.vocab = n_grad_rows; a.skip = -1;
+    row_sort_layout(a, ws);
+    char* sums = ws + row_sort_bytes(n);
+    float* coef_down = reinterpret_cast<float*>(sums + row_sum_bytes(n, wide));
+    float* coef_up = reinterpret_cast<float*>(sums + row_sum_bytes(n, wide) + round256(n * 4));
+    GatherGradArgs g{};
+    g.x = x; g.dy = grad_out; g.ids = ids; g.weights = weights; g.down = expert_down; g.up = expert_up;
+    g.dx = grad_x; g.dweights = grad_weights; g.coef_down = coef_down; g.coef_up = coef_up;
+    g.T = n_tokens; g.HK = static_cast<int>(HK); g.N = n_grad_rows; g.D = c.input_dim; g.Dout = c.output_dim;
+    g.act_dtype = c.act_dtype; g.table_dtype = c.table_dtype; g.activation = c.activation;
+    g.status = h->status; g.sm_count = h->sm_count; g.hidden = 1; g.grad_dtype = PEER_DTYPE_F32;
+    CU_TRY(h, launch_gather_grad(g, s));
+    a.zero_rows = grad_down;
+    a.row_bytes = static_cast<int64_t>(c.input_dim) * tb;
+    CU_TRY(h, launch_row_sort(a, s));
+    RowSumArgs r{};
+    r.keys = a.sorted_keys; r.order = a.order; r.n = n; r.vocab = n_grad_rows; r.per_row = HK; r.dtype = c.act_dtype; r.scale = 1.f;
+    r.workspace = sums;
+    r.src = x; r.src_stride = c.input_dim; r.coef = coef_down; r.out = grad_down; r.D = c.input_dim;
+    r.counter = a.counters; r.zero = !a.zeroed;
+    CU_TRY(h, launch_row_sums(r, s));
+    h->launches += 1 + a.launches + r.launches;
+    r.src = grad_out; r.src_stride = c.output_dim; r.coef = coef_up; r.out = grad_up; r.D = c.output_dim;
+    r.counter = a.counters + 1; r.zero = true;
+    CU_TRY(h, launch_row_sums(r, s));
+    h->launches += r.launches;
     return PEER_OK;
 }
 

@@ -45,7 +45,7 @@ template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const RowSortArgs a, const uint32_t* __restrict__ keys, int shift,
                                                                   int digits, int items, int tiles) {
     __shared__ uint32_t hist[MAX_DIGITS];
-    if (FIRST && blockIdx.x == 0 && threadIdx.x == 0 && a.counter) *a.counter = 0;
+    if (FIRST && blockIdx.x == 0 && threadIdx.x < 4) a.counters[threadIdx.x] = 0;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0u;
     __syncthreads();
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * SORT_THREADS * items;
@@ -246,7 +246,7 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t local0 = warp * IT * 32 + lane, i0 = rank * EACH + local0;
     const uint32_t n = static_cast<uint32_t>(a.n), digits = 1u << per;
-    if (rank == 0 && tid == 0 && a.counter) *a.counter = 0;
+    if (rank == 0 && tid < 4) a.counters[tid] = 0;
     uint32_t key[IT], pos[IT], slot[IT];
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
@@ -356,7 +356,7 @@ int64_t tiles_for(int64_t n) { const int64_t t = SORT_THREADS * items_for(n); re
 }  // namespace
 
 int64_t row_sort_bytes(int64_t n) {
-    return 4 * round256(n * 4) + round256(tiles_for(n) * MAX_DIGITS * 4) + round256(MAX_DIGITS * 4);
+    return 4 * round256(n * 4) + round256(tiles_for(n) * MAX_DIGITS * 4) + round256(MAX_DIGITS * 4) + 256;
 }
 
 void row_sort_layout(RowSortArgs& a, void* workspace) {
@@ -366,6 +366,7 @@ void row_sort_layout(RowSortArgs& a, void* workspace) {
     a.counts = reinterpret_cast<uint32_t*>(p);
     p += round256(tiles_for(a.n) * MAX_DIGITS * 4);
     a.totals = reinterpret_cast<uint32_t*>(p);
+    a.counters = reinterpret_cast<int*>(p + round256(MAX_DIGITS * 4));
 }
 
 template <int IT>
@@ -382,6 +383,7 @@ static cudaError_t launch_cluster(RowSortArgs& a, int passes, int per, cudaStrea
         sort_cluster_kernel<IT><<<CL_BLOCKS, CL_THREADS, SMEM, s>>>(a, passes, per, a.keys[0], a.pos[0]);
     }
     a.zeroed = a.zero_rows != nullptr;
+    a.launches = a.zeroed ? 2 : 1;
     a.sorted_keys = a.keys[0];
     a.order = a.pos[0];
     return cudaGetLastError();
@@ -399,6 +401,7 @@ cudaError_t launch_row_sort(RowSortArgs& a, cudaStream_t s) {
         if (it <= 4) return launch_cluster<4>(a, passes, per, s);
         return launch_cluster<8>(a, passes, per, s);
     }
+    a.launches = 3 * passes;
     for (int p = 0; p < passes; ++p) {
         const int in = (p + 1) & 1, out = p & 1, shift = p * per;
         if (p == 0) sort_count_kernel<true><<<tiles, SORT_THREADS, 0, s>>>(a, nullptr, shift, digits, items, tiles);

@@ -148,13 +148,14 @@ class PeerOp:
             self._check(self.lib.peer_forward(self.handle, C.byref(t), T, _stream(self.device)))
 
     def block_forward(self, hidden: torch.Tensor, w: dict, ln_w, ln_b, eps: float, out: torch.Tensor,
-                      ids_out=None, scores_out=None):
+                      ids_out=None, scores_out=None, product_ids_out=None):
         """out = hidden + layer(LayerNorm(hidden)); hidden, out [T, D] on the device; ln_w, ln_b fp32 [D] or None."""
         self._dev(ln_w, "ln_w", torch.float32)
         self._dev(ln_b, "ln_b", torch.float32)
         if out.data_ptr() == hidden.data_ptr():
             raise ValueError("out may not alias hidden")
-        t = self._tensors(hidden, w, out, ids_out, scores_out)
+        self._dev(product_ids_out, "product_ids_out", torch.int32)
+        t = self._tensors(hidden, w, out, ids_out, scores_out, product_ids_out=product_ids_out)
         with torch.cuda.device(self.device):
             self._check(self.lib.peer_block_forward(self.handle, C.byref(t), _ptr(ln_w), _ptr(ln_b), float(eps),
                                                     hidden.shape[0], _stream(self.device)))
@@ -373,6 +374,30 @@ class PeerOp:
                 _ptr(gx), _ptr(gw), _ptr(grad_down), _ptr(grad_up), _DT[grad_dtype], n_rows, T, _stream(self.device)))
         return gx, gw, grad_down, grad_up
 
+    def gather_eval_backward_sorted(self, x, grad_out, ids32, weights, down, up, grad_rows: Optional[int] = None):
+        """``gather_eval_backward`` with the table gradients summed by sorted ids: (grad_x fp32, grad_weights fp32,
+        grad_down, grad_up), the last two new tables [grad_rows, .] in the tables' dtype, every row's sum formed in
+        fp32 in one order and rounded once."""
+        self._dev(x, "x", self.act_dtype)
+        self._dev(grad_out, "grad_out", self.act_dtype)
+        self._dev(ids32, "ids", torch.int32)
+        self._dev(weights, "weights", torch.float32)
+        self._dev(down, "expert_down", self.table_dtype)
+        self._dev(up, "expert_up", self.table_dtype)
+        T = x.shape[0]
+        n_rows = down.shape[0] if grad_rows is None else int(grad_rows)
+        gx = torch.empty(T, self.cfg.input_dim, dtype=torch.float32, device=self.device)
+        gw = torch.empty(T, self.cfg.num_heads * self.cfg.top_k, dtype=torch.float32, device=self.device)
+        gd = torch.empty(n_rows, down.shape[1], dtype=self.table_dtype, device=self.device)
+        gu = torch.empty(n_rows, up.shape[1], dtype=self.table_dtype, device=self.device)
+        nbytes = self.lib.peer_gather_eval_backward_sorted_workspace(self.handle, T)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        with torch.cuda.device(self.device):
+            self._check(self.lib.peer_gather_eval_backward_sorted(
+                self.handle, _ptr(x), _ptr(grad_out), _ptr(ids32), _ptr(weights), _ptr(down), _ptr(up), _ptr(gx), _ptr(gw),
+                _ptr(gd), _ptr(gu), n_rows, T, _ptr(ws), nbytes, _stream(self.device)))
+        return gx, gw, gd, gu
+
     def query_status(self):
         """Synchronise and raise if a kernel recorded a timeout or an out-of-range id."""
         with torch.cuda.device(self.device):
@@ -425,6 +450,13 @@ class PEER(nn.Module):
       with ``index_mode="reference"`` (ids stay below n0 + n1; then only those rows
       get fp32 sums, not the whole table) and when a batch brings more than four
       selections per table row on average - else ``"table"``.
+      ``"sorted"`` (single-neuron experts of an fp32 or bf16 layer, rows of at most
+      4 KB): by sorted expert ids, in fp32, rounded once, and the same from run to
+      run; the other modes add in memory, in an order that varies.
+    * ``activation_checkpoint``: what a training step keeps of the layer's input for
+      its backward pass: ``None`` (default) the tensor itself, ``"e4m3"`` its 8-bit
+      form (``checkpoint.pack_rows_e4m3``: a half or a quarter of the memory, the
+      gradients then those of the rounded input).  Not with dropout.
     """
 
     def __init__(self, input_dim: int, output_dim: int, num_experts: int, num_experts_per_tok: int = 16,
@@ -473,6 +505,7 @@ class PEER(nn.Module):
         self.track_indices = True
         self.max_slice_tokens = 16384
         self.table_grad_sums = "auto"
+        self.activation_checkpoint: Optional[str] = None
         self._last_expert_indices: Optional[torch.Tensor] = None
         self._last_expert_scores: Optional[torch.Tensor] = None
         self._op: Optional[PeerOp] = None
@@ -675,6 +708,22 @@ class PEER(nn.Module):
         op.block_forward(x, w, f32(ln_2.weight), f32(ln_2.bias), ln_2.eps, out, ids, sc)
         self._stash(ids, sc, B, S)
         return out.view(B, S, self.output_dim)
+
+    def block_train(self, hidden_states: torch.Tensor, ln_2: nn.LayerNorm) -> torch.Tensor:
+        """``hidden_states + self(ln_2(hidden_states))`` with a gradient: the training form of ``block_forward``,
+        same values.  One autograd node that keeps ``hidden_states`` (in 8 bits with ``activation_checkpoint =
+        "e4m3"``) and the selection; the norm's output and statistics are formed anew in the backward pass.
+        ``ln_2``'s parameters are fp32 or of the layer's dtype."""
+        w, dt = self._prepare(hidden_states)
+        if self.input_dim != self.output_dim:
+            raise ValueError(f"a block adds its input back: input_dim {self.input_dim} must equal output_dim {self.output_dim}")
+        if not (self._needs_grad(hidden_states) or
+                (torch.is_grad_enabled() and any(p.requires_grad for p in ln_2.parameters()))):
+            return self.block_forward(hidden_states, ln_2)
+        if hidden_states.device.type != "cuda":
+            raise RuntimeError("peer_b200 runs on CUDA devices only (sm_100a); there is no CPU path")
+        from .autograd import block_train_autograd
+        return block_train_autograd(self, hidden_states, ln_2)
 
     def forward_host(self, hidden_states: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Same layer for a HOST tensor (pinned for full speed): slices are copied to the device,

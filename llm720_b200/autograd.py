@@ -37,8 +37,8 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
+from . import _ext
 from .checkpoint import pack_rows_e4m3, unpack_rows_e4m3
-from .norm import check_norm_arguments, norm_backward, norm_forward
 
 
 class _ProjectQueries(torch.autograd.Function):
@@ -236,13 +236,13 @@ class _FusedBlock(torch.autograd.Function):
     gradient where the norm's is written."""
 
     @staticmethod
-    def forward(ctx, hidden, norm_w, norm_b, weight, bias, ln_w, ln_b, down, up, module, eps, codes):
+    def forward(ctx, hidden, norm_w, norm_b, weight, bias, ln_w, ln_b, down, up, module, eps):
         op = module._operator(hidden.device, hidden.dtype, hidden.shape[0])
         out, ids, sc, pid = _selection_buffers(module, hidden)
         f32 = lambda p: None if p is None else p.detach().float().contiguous()
         op.block_forward(hidden, module._weights(), f32(norm_w), f32(norm_b), eps, out, ids, sc, pid)
         ctx.save_for_backward(*_kept(module, hidden), norm_w, norm_b, weight, bias, ln_w, ln_b, down, up, ids, sc, pid)
-        ctx.module, ctx.op, ctx.eps, ctx.codes = module, op, eps, codes
+        ctx.module, ctx.op, ctx.eps = module, op, eps
         ctx.mark_non_differentiable(ids, sc)
         return out, ids, sc
 
@@ -255,14 +255,13 @@ class _FusedBlock(torch.autograd.Function):
         need_norm, need = ctx.needs_input_grad[:3], ctx.needs_input_grad[3:9]
         grad_out = grad_out.contiguous()
         below = any(need_norm)
-        x, stats, _, _ = norm_forward(hidden, norm_w, norm_b, ctx.eps, *ctx.codes, True, False)
+        ops = _ext.load()
+        x, stats = ops.block_norm(hidden, norm_w, norm_b, ctx.eps)
         gx, *grads = _layer_grads(ctx.module, ctx.op, x, params, ids, sc, pid, grad_out, (below, *need))
         norm_grads = (None, None, None)
         if below:
-            norm_grads = norm_backward(gx, hidden, None, None, stats, norm_w, *ctx.codes, need_norm[0],
-                                       norm_w.dtype if need_norm[1] else None, norm_b.dtype if need_norm[2] else None,
-                                       add=grad_out)
-        return (*norm_grads, *grads, None, None, None)
+            norm_grads = ops.block_norm_grad(gx, hidden, stats, norm_w, norm_b, grad_out, *need_norm)
+        return (*norm_grads, *grads, None, None)
 
 
 def block_train_autograd(module, hidden_states: torch.Tensor, norm) -> torch.Tensor:
@@ -275,14 +274,14 @@ def block_train_autograd(module, hidden_states: torch.Tensor, norm) -> torch.Ten
         raise ValueError(f"ln_2 normalises {tuple(norm.normalized_shape)}, the layer's input is ({module.input_dim},)")
     B, S, _ = hidden_states.shape
     hidden = hidden_states.contiguous().view(B * S, module.input_dim)
-    codes = check_norm_arguments(hidden, norm.weight, norm.bias, norm.eps)
+    _ext.load().check_norm_arguments(hidden, norm.weight, norm.bias, norm.eps)
     if module.training and module.dropout.p > 0:
         from .norm import layer_norm
         return hidden_states + module(layer_norm(hidden_states, norm.weight, norm.bias, norm.eps))
     ln = module.query_layer_norm
     out, ids, sc = _FusedBlock.apply(hidden, norm.weight, norm.bias, module.query_proj.weight, module.query_proj.bias,
                                      None if ln is None else ln.weight, None if ln is None else ln.bias,
-                                     module.expert_down.weight, module.expert_up.weight, module, norm.eps, codes)
+                                     module.expert_down.weight, module.expert_up.weight, module, norm.eps)
     if module.track_indices:
         module._stash(ids, sc, B, S)
     return out.view(B, S, module.output_dim)

@@ -4,6 +4,10 @@ Every ``csrc/*.cu`` is compiled for sm_100a only and linked into
 ``llm720_b200/lib/libpeer_b200.so`` (a plain C-ABI shared object, no Python or
 torch symbols).  Sources are compiled in parallel; an object is rebuilt only
 when it is older than its source or any header.
+
+``csrc/torch/row_ops.cpp``, the torch binding of the row-wise operators, becomes
+``llm720_b200/lib/_row_ops.so``, a Python extension that links against the
+library beside it.
 """
 from __future__ import annotations
 
@@ -19,6 +23,8 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libpeer_b200.so")
+EXT = os.path.join(LIBDIR, "_row_ops.so")
+EXT_SRC = os.path.join(CSRC, "torch", "row_ops.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -38,6 +44,33 @@ def _stale(target: str, deps) -> bool:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _extension_command():
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ce
+    includes = ce.include_paths("cuda") + [sysconfig.get_paths()["include"],
+                                           os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_row_ops",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{p}" for p in includes]
+            + [EXT_SRC, "-o", EXT] + [f"-L{p}" for p in ce.library_paths("cuda")]
+            + [f"-L{LIBDIR}", "-lpeer_b200", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+               "-ltorch_python"])
+
+
+def build_extension(force: bool = False, verbose: bool = False) -> str:
+    """The torch binding; rebuilt when its source, the C header or the installed torch is newer."""
+    import torch
+    deps = [EXT_SRC, os.path.join(os.path.dirname(PKG), "include", "peer_b200.h"), torch.version.__file__]
+    if force or _stale(EXT, deps):
+        r = subprocess.run(_extension_command(), capture_output=True, text=True)
+        if verbose or r.returncode:
+            sys.stderr.write(f"[{os.path.basename(EXT_SRC)}]\n{r.stdout}{r.stderr}")
+        if r.returncode:
+            raise RuntimeError(f"g++ failed on {EXT_SRC}")
+    return EXT
 
 
 def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
@@ -72,6 +105,7 @@ def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool =
         if r.returncode:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    build_extension(force, verbose)
     return LIB
 
 

@@ -14,6 +14,7 @@
 
 #include "kernels.h"
 #include "row_ops.cuh"
+#include "row_shift.cuh"
 
 namespace peer {
 void set_global_error(const char* msg);
@@ -444,8 +445,6 @@ __device__ __forceinline__ float inverse_sqrt(float v) {
     return (v > 0.f && v < __uint_as_float(F32_INF_BITS)) ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
 }
 
-constexpr int RING_COLUMNS = 16, RING_THREADS = 512;      // columns per thread; one block per SM
-
 template <typename T, int NV, int N>
 __device__ __forceinline__ void load_param_pairs(const void* p, bool f32, const bool (&in)[NV], int gt, int threads, float absent,
                                                  float2 (&out)[NV][N / 2]) {
@@ -458,24 +457,6 @@ __device__ __forceinline__ void load_param_pairs(const void* p, bool f32, const 
 #pragma unroll
         for (int h = 0; h < N / 2; ++h) out[i][h] = make_float2(f[2 * h], f[2 * h + 1]);
     }
-}
-
-// 16, 8 or 4 bytes of this thread's shared memory
-template <typename V> __device__ __forceinline__ V shared_at(uint32_t at);
-template <> __device__ __forceinline__ uint4 shared_at<uint4>(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
-template <> __device__ __forceinline__ uint2 shared_at<uint2>(uint32_t at) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-    return v;
-}
-template <> __device__ __forceinline__ uint32_t shared_at<uint32_t>(uint32_t at) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
 }
 
 template <typename T, int W, bool PACK, int STAGES>
@@ -804,6 +785,335 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const N
     }
 }
 
+// ---------------------------------------------------------------------------
+// The same for rows that are not whole 16-byte pieces at 16-byte addresses (an odd width, an odd stride, a view that
+// begins anywhere), brought and stored as the granules that cover them (row_shift.cuh).  A granule is another thread's,
+// so a row has a barrier behind its arrival and one before its results leave.  16384 x 2001 bf16: forward 56 us, all
+// gradients 67 us, against 172 and 187 us one value at a time.
+// ---------------------------------------------------------------------------
+// parameters of this thread's columns, `absent` beyond the row's end
+template <typename T, int NV, int N>
+__device__ __forceinline__ void load_param_values(const void* p, bool f32, int D, int gt, int threads, float absent, float2 (&out)[NV][N / 2]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const int c = (gt + i * threads) * N + q;
+            f[q] = p && c < D ? param_at<T>(p, f32, c) : absent;
+        }
+#pragma unroll
+        for (int h = 0; h < N / 2; ++h) out[i][h] = make_float2(f[2 * h], f[2 * h + 1]);
+    }
+}
+
+template <typename T, bool PACK, int STAGES>
+__global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormParams p, int warps) {
+    using P = Piece<T, true>;
+    constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2, XB = static_cast<int>(sizeof(typename P::Packed));
+    extern __shared__ __align__(16) unsigned char ring_smem[];
+    __shared__ float2 part[2 * MAX_WARPS];
+    __shared__ uint32_t part_top[2 * MAX_WARPS];
+    __shared__ float held[MAX_WARPS];                       // columns of each of the group's warps
+    const int lane = threadIdx.x & 31, threads = warps * 32;
+    const int group = threadIdx.x / threads, gt = threadIdx.x - group * threads, gw = gt >> 5;
+    const int groups = blockDim.x / threads, D = static_cast<int>(p.D), bytes = D * static_cast<int>(sizeof(T));
+    // a group's memory: STAGES rows of x, 16 bytes, a row of y, 16 bytes, a row of payload
+    const int room = row_room(threads * RING_COLUMNS, sizeof(T)), room8 = row_room(threads * RING_COLUMNS, 1);
+    const uint32_t slot0 = smem_u32(ring_smem) + group * ((STAGES + 1) * room + room8 + 32), slot_end = slot0 + STAGES * room;
+    const uint32_t out = slot_end + 16, out8 = out + room + 16;
+    auto sync = [&]() { if (warps > 1) group_sync(group, threads); else __syncwarp(); };
+    int valid[NV], mine = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        valid[i] = min(max(D - (gt + i * threads) * N, 0), N);
+        mine += min(max(D - (i * threads + gw * 32) * N, 0), 32 * N);
+    }
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * groups + group, step = static_cast<int64_t>(gridDim.x) * groups;
+    int rows = first < p.rows ? static_cast<int>((p.rows - first + step - 1) / step) : 0;      // of this group
+    int to_fetch = rows;
+    const T* src = static_cast<const T*>(p.x) + first * p.x_stride;
+    const T* cur = src;
+    const int64_t src_step = step * p.x_stride;
+    uint32_t slot = slot0, fetch_slot = slot0;
+    auto fetch = [&]() {
+        if (to_fetch > 0) fetch_row(fetch_slot, src, bytes, gt, threads);
+        src += src_step;
+        --to_fetch;
+        fetch_slot += room;
+        if (fetch_slot == slot_end) fetch_slot = slot0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    float2 w[NV][H], b[NV][H];
+    load_param_values<T, NV, N>(p.w, p.param_f32, D, gt, threads, 1.f, w);
+    load_param_values<T, NV, N>(p.b, p.param_f32, D, gt, threads, 0.f, b);
+    if (group == 0 && lane == 0) held[gw] = static_cast<float>(mine);
+    __syncthreads();
+    const float inv_mine = mine > 0 ? 1.f / static_cast<float>(mine) : 0.f, inv_d = 1.f / static_cast<float>(D);
+    int64_t r = first;
+    int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
+    for (; rows > 0; --rows) {
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        sync();                                             // the other threads' granules
+        const uint32_t shift = offset16(cur);
+        cur += src_step;
+        typename P::Raw raw[NV];
+        float2 x[NV][H], s2 = splat(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            raw[i] = valid[i] ? shared_shifted(slot + (gt + i * threads) * 16, shift) : P::zero();      // zeros behind the row
+            float f[N];
+            P::decode(raw[i], f);
+#pragma unroll
+            for (int h = 0; h < H; ++h) { x[i][h] = make_float2(f[2 * h], f[2 * h + 1]); s2 = __fadd2_rn(s2, x[i][h]); }
+        }
+        slot += room;
+        if (slot == slot_end) slot = slot0;
+        bool odd = false;
+        uint32_t top = 0u;
+        if (PACK) top = warp_top<T, true, NV>(raw, odd);
+        float mean = warp_sum(s2.x + s2.y) * inv_mine;
+        const float2 neg = splat(-mean);
+        s2 = splat(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                float2 d = __fadd2_rn(x[i][h], neg);
+                if (valid[i] < N) {                         // the row's last piece, and those behind it
+                    if (2 * h >= valid[i]) d.x = 0.f;
+                    if (2 * h + 1 >= valid[i]) d.y = 0.f;
+                }
+                s2 = __ffma2_rn(d, d, s2);
+            }
+        }
+        float m2 = warp_sum(s2.x + s2.y);
+        if (warps > 1) {
+            if (lane == 0) {
+                part[exchange + gw] = make_float2(mean, m2);
+                if (PACK) part_top[exchange + gw] = top;
+            }
+            group_sync(group, threads);
+            mean = 0.f;
+            for (int k = 0; k < warps; ++k) {
+                mean = fmaf(held[k], part[exchange + k].x, mean);
+                if (PACK) top = max(top, part_top[exchange + k]);
+            }
+            mean *= inv_d;
+            m2 = 0.f;
+            for (int k = 0; k < warps; ++k) {
+                const float2 v = part[exchange + k];
+                const float d = v.x - mean;
+                m2 += fmaf(held[k] * d, d, v.y);
+            }
+            exchange += other;
+            other = -other;
+        }
+        const float rstd = inverse_sqrt(m2 * inv_d + p.eps);
+        const float2 r2 = splat(rstd), c2 = splat(-mean * rstd);
+        const int e = PACK ? e4m3_scale_exponent(top) : 0;
+        const float inv = exp2_int(-e);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (valid[i]) {
+                float f[N];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const float2 v = __ffma2_rn(__ffma2_rn(x[i][h], r2, c2), w[i][h], b[i][h]);
+                    f[2 * h] = v.x;
+                    f[2 * h + 1] = v.y;
+                }
+                store_shared(out + (gt + i * threads) * 16, P::encode(f));
+                if constexpr (PACK) store_shared(out8 + (gt + i * threads) * XB, pack_piece<T, true>(raw[i], inv, odd));
+            }
+        sync();
+        store_row<T>(static_cast<T*>(p.y) + r * p.D, out, bytes, gt, threads);
+        if (PACK) store_row<uint8_t>(p.payload + r * p.D, out8, D, gt, threads);
+        if (gt == 0) {
+            if (p.mean) p.mean[r] = mean;
+            if (p.rstd) p.rstd[r] = rstd;
+            if (PACK) p.scale[r] = exp2_int(e);
+        }
+        r += step;
+    }
+}
+
+template <typename T, bool KEPT, int STAGES>
+__global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const NormGradParams p, int warps) {
+    using P = Piece<T, true>;
+    using X = typename std::conditional<KEPT, typename P::Packed, uint4>::type;
+    constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2, XB = static_cast<int>(sizeof(X));
+    extern __shared__ __align__(16) unsigned char ring_smem[];
+    __shared__ float2 part[2 * MAX_WARPS];
+    const int lane = threadIdx.x & 31, threads = warps * 32;
+    const int group = threadIdx.x / threads, gt = threadIdx.x - group * threads, gw = gt >> 5;
+    const int groups = blockDim.x / threads, D = static_cast<int>(p.D), bytes = D * static_cast<int>(sizeof(T));
+    const int x_bytes = KEPT ? D : bytes;
+    // a group's memory: STAGES of {dy, x or payload, {mean, 1/deviation, scale, -}}, 16 bytes, a row of dx
+    const int room = row_room(threads * RING_COLUMNS, sizeof(T)), room_x = row_room(threads * RING_COLUMNS, KEPT ? 1 : sizeof(T));
+    const int stage = room + room_x + 16;
+    const uint32_t slot0 = smem_u32(ring_smem) + group * (STAGES * stage + 16 + room), slot_end = slot0 + STAGES * stage;
+    const uint32_t out = slot_end + 16;
+    auto sync = [&]() { if (warps > 1) group_sync(group, threads); else __syncwarp(); };
+    bool in[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) in[i] = (gt + i * threads) * N < D;
+    const float inv_d = 1.f / static_cast<float>(D);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * groups + group, step = static_cast<int64_t>(gridDim.x) * groups;
+    int rows = first < p.rows ? static_cast<int>((p.rows - first + step - 1) / step) : 0;      // of this group
+    int to_fetch = rows;
+    const T* src_dy = static_cast<const T*>(p.dy) + first * p.dy_stride;
+    const char* src_x = KEPT ? reinterpret_cast<const char*>(p.payload) + first * p.D
+                             : reinterpret_cast<const char*>(static_cast<const T*>(p.x) + first * p.x_stride);
+    const float* src_stat = (gt == 0 ? p.mean : gt == 1 ? p.rstd : p.scale) + first;
+    const bool brings = gt < (KEPT ? 3 : 2);
+    const T* cur_dy = src_dy;
+    const char* cur_x = src_x;
+    const int64_t dy_step = step * p.dy_stride, x_step = step * (KEPT ? p.D : p.x_stride * static_cast<int64_t>(sizeof(T)));
+    uint32_t slot = slot0, fetch_slot = slot0;
+    auto fetch = [&]() {
+        if (to_fetch > 0) {
+            if (brings) copy_async<4>(fetch_slot + room + room_x + gt * 4, src_stat);
+            fetch_row(fetch_slot, src_dy, bytes, gt, threads);
+            fetch_row(fetch_slot + room, src_x, x_bytes, gt, threads);
+        }
+        src_dy += dy_step;
+        src_x += x_step;
+        src_stat += step;
+        --to_fetch;
+        fetch_slot += stage;
+        if (fetch_slot == slot_end) fetch_slot = slot0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    float2 w[NV][H], aw[NV][H], ab[NV][H];
+    load_param_values<T, NV, N>(p.w, p.param_f32, D, gt, threads, 1.f, w);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int h = 0; h < H; ++h) aw[i][h] = ab[i][h] = splat(0.f);
+    int64_t r = first;
+    int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
+    for (; rows > 0; --rows) {
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        sync();                                             // the other threads' granules
+        const uint4 st = shared_at<uint4>(slot + room + room_x);
+        const float mean = __uint_as_float(st.x), rstd = __uint_as_float(st.y), sc = KEPT ? __uint_as_float(st.z) : 1.f;
+        const bool clamp = KEPT && may_clamp<T>(sc);
+        const float2 r2 = splat(rstd), rx = splat(KEPT && !clamp ? rstd * sc : rstd), c2 = splat(-mean * rstd);
+        const uint32_t dy_shift = offset16(cur_dy), x_shift = offset16(cur_x);
+        cur_dy += dy_step;
+        cur_x += x_step;
+        float2 n[NV][H], g[NV][H], s1 = splat(0.f), s2 = splat(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = gt + i * threads;
+            float f[N], d[N];
+            if constexpr (KEPT) {
+                P::decode_packed(in[i] ? shared_unaligned<X>(slot + room + x_shift + c * XB) : X{}, f);
+                if (clamp) {
+#pragma unroll
+                    for (int q = 0; q < N; ++q) f[q] = unpacked<T>(f[q], sc);
+                }
+            } else {
+                P::decode(in[i] ? shared_shifted(slot + room + c * 16, x_shift) : X{}, f);
+            }
+            P::decode(in[i] ? shared_shifted(slot + c * 16, dy_shift) : P::zero(), d);      // zeros behind the row
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const float2 dv = make_float2(d[2 * h], d[2 * h + 1]);
+                n[i][h] = __ffma2_rn(make_float2(f[2 * h], f[2 * h + 1]), rx, c2);
+                g[i][h] = __fmul2_rn(dv, w[i][h]);
+                s1 = __fadd2_rn(s1, g[i][h]);
+                s2 = __ffma2_rn(g[i][h], n[i][h], s2);
+                aw[i][h] = __ffma2_rn(dv, n[i][h], aw[i][h]);
+                ab[i][h] = __fadd2_rn(ab[i][h], dv);
+            }
+        }
+        slot += stage;
+        if (slot == slot_end) slot = slot0;
+        if (p.dx) {
+            float s[2] = {s1.x + s1.y, s2.x + s2.y};
+            const float total = warp_sums<2>(s);            // lane 0: the first sum, lane 16: the second
+            float m1 = 0.f, m2 = 0.f;
+            if (warps == 1) {
+                m1 = __shfl_sync(FULL_MASK, total, 0);
+                m2 = __shfl_sync(FULL_MASK, total, 16);
+            } else {
+                if ((lane & 15) == 0) reinterpret_cast<float*>(part + exchange + gw)[lane >> 4] = total;
+                group_sync(group, threads);
+                for (int k = 0; k < warps; ++k) {
+                    const float2 v = part[exchange + k];
+                    m1 += v.x;
+                    m2 += v.y;
+                }
+                exchange += other;
+                other = -other;
+            }
+            const float scaled = -inv_d * rstd;
+            const float2 m1p = splat(m1 * scaled), m2p = splat(m2 * scaled);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (in[i]) {
+                    float f[N];
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const float2 v = __ffma2_rn(g[i][h], r2, __ffma2_rn(n[i][h], m2p, m1p));
+                        f[2 * h] = v.x;
+                        f[2 * h + 1] = v.y;
+                    }
+                    store_shared(out + (gt + i * threads) * 16, P::encode(f));
+                }
+            sync();
+            store_row<T>(static_cast<T*>(p.dx) + r * p.D, out, bytes, gt, threads);
+        } else {
+            sync();                                         // before a fetch overwrites what another thread still reads
+        }
+        r += step;
+    }
+    if (!p.dw && !p.db) return;
+    grid_release();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                        // the ring is free: the groups add up in order through it
+    float2* columns = reinterpret_cast<float2*>(ring_smem);      // [2 * NV * H][threads]
+    for (int q = 0; q + 1 < groups; ++q) {
+        if (group == q) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    columns[(i * H + h) * threads + gt] = aw[i][h];
+                    columns[((NV + i) * H + h) * threads + gt] = ab[i][h];
+                }
+        }
+        __syncthreads();
+        if (group == q + 1) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    aw[i][h] = __fadd2_rn(aw[i][h], columns[(i * H + h) * threads + gt]);
+                    ab[i][h] = __fadd2_rn(ab[i][h], columns[((NV + i) * H + h) * threads + gt]);
+                }
+        }
+        __syncthreads();
+    }
+    if (group == groups - 1) {
+        float* sums = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.D;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int c = (gt + i * threads) * N + 2 * h;
+                if (c < D) { sums[c] = aw[i][h].x; sums[p.D + c] = ab[i][h].x; }
+                if (c + 1 < D) { sums[c + 1] = aw[i][h].y; sums[p.D + c + 1] = ab[i][h].y; }
+            }
+    }
+}
+
 // `splits` partial rows to the gradients: 32 columns by 32 lanes of partials per block, so that a lane's few loads are
 // all in flight at once
 constexpr int JOIN_LANES = 32;
@@ -846,6 +1156,10 @@ int splits_for(int64_t rows) {
 unsigned row_blocks(int64_t rows) { return static_cast<unsigned>(rows < 148 * 64 ? rows : 148 * 64); }
 
 constexpr int64_t RING_ROWS = 1024;   // below, a block sees too few rows for a ring to run ahead
+// rows at any address: a warp's 512 columns are too many for narrower ones (32768 x 129 bf16: 23 us forward, 21 us one
+// value at a time; 16384 x 2001: 56 and 172); the backward pass needs more rows (1500 x 1001 fp32: 14 us, 12 one value
+// at a time; 5003 x 1537 fp16: 27 and 41)
+constexpr int64_t SHIFT_DIM = 256, SHIFT_GRAD_ROWS = 2048;
 
 // the width a ring kernel is built for: W full warps when the row is exactly that, else 0
 inline int ring_width(int64_t D) {
@@ -853,7 +1167,6 @@ inline int ring_width(int64_t D) {
         if (D == static_cast<int64_t>(w) * 32 * RING_COLUMNS) return w;
     return 0;
 }
-inline int ring_warps(int64_t D) { return static_cast<int>((D + 32 * RING_COLUMNS - 1) / (32 * RING_COLUMNS)); }
 
 template <typename T, int W, bool PACK>
 cudaError_t norm_ring_width(const NormParams& p, cudaStream_t s) {
@@ -879,6 +1192,19 @@ cudaError_t norm_ring_launch(const NormParams& p, cudaStream_t s) {
     }
 }
 
+template <typename T, bool PACK>
+cudaError_t norm_shift_launch(const NormParams& p, cudaStream_t s) {
+    constexpr int STAGES = sizeof(T) == 4 ? 3 : 5;           // with the results' rows at most 160 KB
+    auto* kernel = norm_shift_kernel<T, PACK, STAGES>;
+    const int warps = ring_warps(p.D), groups = MAX_WARPS / warps, columns = warps * 32 * RING_COLUMNS;
+    const int smem = groups * ((STAGES + 1) * row_room(columns, sizeof(T)) + row_room(columns, 1) + 32);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const int64_t need = (p.rows + groups - 1) / groups;
+    kernel<<<static_cast<unsigned>(need < GRID_SMS ? need : GRID_SMS), groups * warps * 32, smem, s>>>(p, warps);
+    return cudaGetLastError();
+}
+
 template <typename T, bool WIDE, int NV, bool PACK>
 cudaError_t norm_launch(const NormParams& p, const RowShape& h, cudaStream_t s) {
     const int64_t need = (p.rows + h.groups - 1) / h.groups;
@@ -893,7 +1219,10 @@ cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
     const bool wide = p.D % N == 0 && p.x_stride % N == 0 && aligned16(p.x) && aligned16(p.y) && (!p.w || aligned16(p.w)) &&
                       (!p.b || aligned16(p.b)) && (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0;
-    if (wide && p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) return norm_ring_launch<T, PACK>(p, s);
+    if (p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) {
+        if (wide) return norm_ring_launch<T, PACK>(p, s);
+        if (p.D > SHIFT_DIM) return norm_shift_launch<T, PACK>(p, s);
+    }
     const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8, 1) : narrow_shape(p.rows, p.D, 8);
     if (h.warps == 0) {
         norm_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
@@ -951,6 +1280,21 @@ cudaError_t norm_grad_ring_launch(NormGradParams& p, cudaStream_t s) {
 }
 
 template <typename T, bool KEPT>
+cudaError_t norm_grad_shift_launch(NormGradParams& p, cudaStream_t s) {
+    constexpr int STAGES = sizeof(T) == 4 ? (KEPT ? 3 : 2) : (KEPT ? 5 : 4);          // at most 170 KB
+    auto* kernel = norm_grad_shift_kernel<T, KEPT, STAGES>;
+    const int warps = ring_warps(p.D), groups = MAX_WARPS / warps, columns = warps * 32 * RING_COLUMNS;
+    const int smem = groups * (STAGES * (row_room(columns, sizeof(T)) + row_room(columns, KEPT ? 1 : sizeof(T)) + 16) + 16 +
+                               row_room(columns, sizeof(T)));
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const int64_t need = (p.rows + groups - 1) / groups;
+    p.splits = static_cast<int>(need < MAX_SPLITS ? need : MAX_SPLITS);
+    kernel<<<p.splits, groups * warps * 32, smem, s>>>(p, warps);
+    return cudaGetLastError();
+}
+
+template <typename T, bool KEPT>
 cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
     bool wide = p.D % N == 0 && p.dy_stride % N == 0 && aligned16(p.dy) && (!p.dx || aligned16(p.dx)) && (!p.add || aligned16(p.add)) &&
@@ -958,8 +1302,8 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     wide = wide && (KEPT ? (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0 : p.x_stride % N == 0 && aligned16(p.x));
     const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16, 1) : narrow_shape(p.rows, p.D, 16);
     const bool sums = p.dw || p.db;
-    if (wide && p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) {
-        const cudaError_t e = norm_grad_ring_launch<T, KEPT>(p, s);
+    if (p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS && (wide || (!p.add && p.D > SHIFT_DIM && p.rows >= SHIFT_GRAD_ROWS))) {
+        const cudaError_t e = wide ? norm_grad_ring_launch<T, KEPT>(p, s) : norm_grad_shift_launch<T, KEPT>(p, s);
         if (e != cudaSuccess) return e;
     } else if (h.warps == 0 || p.rows == 0) {
         p.splits = splits_for(p.rows);

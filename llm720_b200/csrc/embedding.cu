@@ -21,27 +21,27 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int id_bytes, int64_t 
     return id_bytes == 8 ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
 }
 
-// one warp per token
+// `group` threads (a warp, or the block when there are few tokens) per token
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) embed_kernel(const void* __restrict__ ids, int id_bytes, int64_t n, const T* __restrict__ w,
                                                     int64_t vocab, int64_t D, float scale, T* __restrict__ out,
-                                                    unsigned long long* dropped) {
+                                                    unsigned long long* dropped, int group) {
     using P = Piece<T, WIDE>;
     constexpr int N = P::N;
-    const int lane = threadIdx.x & 31;
-    const int64_t stride = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-    for (int64_t t = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; t < n; t += stride) {
+    const int gt = threadIdx.x & (group - 1), per_block = blockDim.x / group;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / group; t < n; t += static_cast<int64_t>(gridDim.x) * per_block) {
         const int64_t id = id_at(ids, id_bytes, t);
         const bool inside = id >= 0 && id < vocab;
-        if (!inside && dropped && lane == 0) atomicAdd(dropped, 1ULL);
-        const T* row = w + (inside ? id : 0) * D;
+        if (!inside && dropped && gt == 0) atomicAdd(dropped, 1ULL);
+        const T* row = w + (inside ? id : 0) * D;          // row 0 is read in place of none: no test between the loads
+        T* dst = out + t * D;
 #pragma unroll 4
-        for (int64_t c = static_cast<int64_t>(lane) * N; c < D; c += 32 * N) {
+        for (int64_t c = static_cast<int64_t>(gt) * N; c < D; c += group * N) {
             float f[N];
-            P::decode(inside ? P::load(row + c) : P::zero(), f);
+            P::decode(P::load(row + c), f);
 #pragma unroll
             for (int q = 0; q < N; ++q) f[q] = inside ? f[q] * scale : 0.f;
-            P::store(out + t * D + c, P::encode(f));
+            P::store(dst + c, P::encode(f));
         }
     }
 }
@@ -50,12 +50,13 @@ template <typename T>
 cudaError_t embed_t(const void* ids, int id_bytes, int64_t n, const void* w, int64_t vocab, int64_t D, float scale, void* out,
                     int64_t* dropped, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    const int64_t blocks = (n + 7) / 8;
+    const int group = n < GRID_SMS * 8 ? 256 : 32;          // fewer tokens than a warp each would need to fill the SMs
+    const int64_t blocks = (n * group + 255) / 256;
     const unsigned grid = static_cast<unsigned>(blocks < 148 * 32 ? blocks : 148 * 32);
     const bool vec = D % V == 0 && ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
     auto* d = reinterpret_cast<unsigned long long*>(dropped);
-    if (vec) embed_kernel<T, true><<<grid, 256, 0, s>>>(ids, id_bytes, n, static_cast<const T*>(w), vocab, D, scale, static_cast<T*>(out), d);
-    else embed_kernel<T, false><<<grid, 256, 0, s>>>(ids, id_bytes, n, static_cast<const T*>(w), vocab, D, scale, static_cast<T*>(out), d);
+    if (vec) embed_kernel<T, true><<<grid, 256, 0, s>>>(ids, id_bytes, n, static_cast<const T*>(w), vocab, D, scale, static_cast<T*>(out), d, group);
+    else embed_kernel<T, false><<<grid, 256, 0, s>>>(ids, id_bytes, n, static_cast<const T*>(w), vocab, D, scale, static_cast<T*>(out), d, group);
     return cudaGetLastError();
 }
 

@@ -6,7 +6,7 @@
 //
 // Up to 65,536 ids (a training batch): one launch.  A cluster of eight blocks holds all pairs in registers and
 // shared memory; per digit the blocks tell one another their counts and send every pair to its place in distributed
-// shared memory.  16,384 ids below 32,000: SORT_US.
+// shared memory.  16,384 ids below 32,000: 12 us.
 //
 // More ids: three launches per digit.  (1) every tile of keys counts its digits, (2) every digit scans its
 // counts over the tiles, (3) every tile scatters its keys; the rank of a key
@@ -29,7 +29,7 @@ __device__ __forceinline__ uint32_t source_key(const RowSortArgs& a, int64_t i) 
 }
 
 // Lanes of the warp whose digit equals this lane's: one vote per bit.  (match.any does the same in one instruction,
-// but takes about a microsecond when the digits differ: 17 us instead of SORT16_US for 16,384 ids.)
+// but takes about a microsecond when the digits differ: a scatter of 131,072 keys took 21 us with it, 8 us without.)
 __device__ __forceinline__ unsigned same_digit(uint32_t digit) {
     unsigned same = FULL_MASK;
 #pragma unroll
@@ -45,6 +45,7 @@ template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const RowSortArgs a, const uint32_t* __restrict__ keys, int shift,
                                                                   int digits, int items, int tiles) {
     __shared__ uint32_t hist[MAX_DIGITS];
+    if (!FIRST) grid_wait();
     if (FIRST && blockIdx.x == 0 && threadIdx.x < 4) a.counters[threadIdx.x] = 0;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0u;
     __syncthreads();
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scan_kernel(const RowSortAr
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t* row = a.counts + static_cast<int64_t>(blockIdx.x) * tiles;
     uint32_t carry = 0u;
+    grid_wait();
     for (int t0 = 0; t0 < tiles; t0 += SORT_THREADS) {
         const int t = t0 + threadIdx.x;
         const uint32_t v = t < tiles ? row[t] : 0u;
@@ -103,6 +105,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const RowSor
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int d = threadIdx.x; d < SORT_WARPS * MAX_DIGITS; d += SORT_THREADS) (&seen[0][0])[d] = 0u;
     __syncthreads();
+    grid_wait();
     // a warp owns `items` consecutive groups of 32 keys, in order
     const int64_t w0 = (static_cast<int64_t>(blockIdx.x) * SORT_WARPS + warp) * items * 32;
     uint32_t key[16], rank[16];
@@ -188,6 +191,8 @@ __device__ __forceinline__ void store_remote(uint32_t addr, uint32_t a, uint32_t
 struct ClusterShared {
     uint32_t seen[CL_WARPS][MAX_DIGITS];      // per warp and digit: count, then first slot
     uint32_t totals[CL_BLOCKS][MAX_DIGITS];   // every block's count per digit
+    uint32_t quarter[4][MAX_DIGITS];          // this block's count per digit in eight warps each
+    uint32_t first[MAX_DIGITS];               // this block's first slot per digit
     uint32_t warp_total[CL_WARPS];
 };
 
@@ -195,8 +200,8 @@ struct ClusterShared {
 // in a bitmap (every block reads all ids, from L2) and writes the unmarked rows.  Launched in front of the sort, which
 // starts as soon as all of these blocks run (programmatic launch; they leave room for it on every SM) and waits for
 // their end only in its last instruction.
-constexpr int ZERO_THREADS = 512, ZERO_WORDS = 1024, ZERO_IDS = 8;      // 32 registers a thread: sixteen warps fit beside a block of the sort
-__global__ void __launch_bounds__(ZERO_THREADS, 4) zero_unnamed_kernel(const RowSortArgs a) {
+constexpr int ZERO_THREADS = 256, ZERO_WORDS = 1024, ZERO_IDS = 8;      // 32 registers a thread: eight warps fit beside a block of the sort
+__global__ void __launch_bounds__(ZERO_THREADS, 8) zero_unnamed_kernel(const RowSortArgs a) {
     __shared__ uint32_t marks[ZERO_WORDS];
     grid_release();
     const int64_t each = (a.vocab + gridDim.x - 1) / gridDim.x;
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(ZERO_THREADS, 4) zero_unnamed_kernel(const Row
         for (int i = threadIdx.x; i < ZERO_WORDS; i += ZERO_THREADS) marks[i] = 0u;
         __syncthreads();
         for (int64_t i0 = threadIdx.x; i0 < a.n; i0 += ZERO_THREADS * ZERO_IDS) {
-            uint32_t id[ZERO_IDS];                           // loaded together: 16,384 ids are four rounds of latency
+            uint32_t id[ZERO_IDS];                           // loaded together: 16,384 ids are eight rounds of latency
 #pragma unroll
             for (int k = 0; k < ZERO_IDS; ++k) {
                 const int64_t i = i0 + k * ZERO_THREADS;
@@ -273,57 +278,52 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 
         }
         __syncthreads();
         // thread (digit, quarter): the quarter's warps of one digit, turned into running sums within the quarter
-        {
-            const int d = tid & (MAX_DIGITS - 1), q = tid >> 8;
-            uint32_t run = 0u;
+        const int d = tid & (MAX_DIGITS - 1), q = tid >> 8;
+        uint32_t run = 0u;
 #pragma unroll
-            for (int w = 0; w < CL_WARPS / 4; ++w) {
-                const uint32_t v = sh.seen[q * (CL_WARPS / 4) + w][d];
-                sh.seen[q * (CL_WARPS / 4) + w][d] = run;
-                run += v;
-            }
-            // quarters' totals meet in `totals` rows 0-3 of this block for a moment
-            sh.totals[q][d] = run;
-            __syncthreads();
-            const uint32_t t0 = sh.totals[0][d], t1 = sh.totals[1][d], t2 = sh.totals[2][d], t3 = sh.totals[3][d];
-            const uint32_t ahead = (q > 0 ? t0 : 0u) + (q > 1 ? t1 : 0u) + (q > 2 ? t2 : 0u);
+        for (int w = 0; w < CL_WARPS / 4; ++w) {
+            const uint32_t v = sh.seen[q * (CL_WARPS / 4) + w][d];
+            sh.seen[q * (CL_WARPS / 4) + w][d] = run;
+            run += v;
+        }
+        sh.quarter[q][d] = run;
+        __syncthreads();
+        const uint32_t t0 = sh.quarter[0][d], t1 = sh.quarter[1][d], t2 = sh.quarter[2][d], t3 = sh.quarter[3][d];
+        {                                               // this block's count of digit d to all eight blocks
+            const uint32_t at = smem_u32(&sh.totals[rank][d]);
 #pragma unroll
-            for (int w = 0; w < CL_WARPS / 4; ++w) sh.seen[q * (CL_WARPS / 4) + w][d] += ahead;
-            cluster_sync();                             // every block is done with the scratch rows
-            if (q < 2) {                                // this block's count of digit d to all eight blocks
-                const uint32_t mine = t0 + t1 + t2 + t3, at = smem_u32(&sh.totals[rank][d]);
-#pragma unroll
-                for (int b = 0; b < CL_BLOCKS / 2; ++b) store_remote(remote(at, q * (CL_BLOCKS / 2) + b), mine);
-            }
+            for (int b = 0; b < CL_BLOCKS / 4; ++b) store_remote(remote(at, q * (CL_BLOCKS / 4) + b), t0 + t1 + t2 + t3);
         }
         cluster_sync();
         // first slot of a digit: smaller digits of all blocks, then this digit of earlier blocks
-        {
-            uint32_t all = 0u, earlier = 0u;
-            if (tid < MAX_DIGITS) {
+        uint32_t all = 0u, earlier = 0u;
+        if (tid < MAX_DIGITS) {
 #pragma unroll
-                for (int b = 0; b < CL_BLOCKS; ++b) {
-                    const uint32_t v = sh.totals[b][tid];
-                    all += v;
-                    if (b < static_cast<int>(rank)) earlier += v;
-                }
+            for (int b = 0; b < CL_BLOCKS; ++b) {
+                const uint32_t v = sh.totals[b][tid];
+                all += v;
+                if (b < static_cast<int>(rank)) earlier += v;
             }
-            uint32_t inc = all;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t u = __shfl_up_sync(FULL_MASK, inc, o);
-                if (lane >= o) inc += u;
-            }
-            if (lane == 31) sh.warp_total[warp] = inc;
-            __syncthreads();
-            if (tid < MAX_DIGITS) {
-                uint32_t first = inc - all + earlier;
-                for (int w = 0; w < warp; ++w) first += sh.warp_total[w];
-#pragma unroll 8
-                for (int w = 0; w < CL_WARPS; ++w) sh.seen[w][tid] += first;
-            }
-            __syncthreads();
         }
+        uint32_t inc = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(FULL_MASK, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (tid < MAX_DIGITS && lane == 31) sh.warp_total[warp] = inc;
+        __syncthreads();
+        if (tid < MAX_DIGITS) {
+            uint32_t f = inc - all + earlier;
+#pragma unroll
+            for (int w = 0; w < MAX_DIGITS / 32; ++w) f += w < warp ? sh.warp_total[w] : 0u;
+            sh.first[tid] = f;
+        }
+        __syncthreads();
+        const uint32_t base = sh.first[d] + (q > 0 ? t0 : 0u) + (q > 1 ? t1 : 0u) + (q > 2 ? t2 : 0u);
+#pragma unroll
+        for (int w = 0; w < CL_WARPS / 4; ++w) sh.seen[q * (CL_WARPS / 4) + w][d] += base;
+        __syncthreads();
         const bool last = p + 1 == passes;
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
@@ -342,9 +342,10 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 
             key[k] = v.x;
             pos[k] = v.y;
         }
-        // the next pass's first cluster_sync lies behind these reads and before the next writes to `pairs`
+        // the next pass's counts are exchanged behind these reads and before the next writes to `pairs`; this pass's
+        // `totals` were read before the cluster_sync above, so other blocks may write the next ones
     }
-    cluster_sync();                                      // no block leaves while another may still write to it
+    // (the last pass writes to other blocks only before its one cluster_sync: a block may leave when it is done)
     grid_wait();                                         // the zeros of the kernel in front belong to the result
 }
 
@@ -374,7 +375,7 @@ static cudaError_t launch_cluster(RowSortArgs& a, int passes, int per, cudaStrea
     constexpr int SMEM = static_cast<int>(sizeof(ClusterShared)) + CL_THREADS * IT * 8;
     const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<IT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
-    if (a.zero_rows) {
+    if (a.zero_rows && IT <= 2) {                        // four and more pairs a thread: the registers of a whole SM
         const int64_t blocks = a.vocab < GRID_SMS ? a.vocab : GRID_SMS;
         zero_unnamed_kernel<<<static_cast<unsigned>(blocks), ZERO_THREADS, 0, s>>>(a);
         const cudaError_t ez = launch_behind_smem(sort_cluster_kernel<IT>, dim3(CL_BLOCKS), dim3(CL_THREADS), SMEM, s, a, passes, per, a.keys[0], a.pos[0]);
@@ -382,7 +383,7 @@ static cudaError_t launch_cluster(RowSortArgs& a, int passes, int per, cudaStrea
     } else {
         sort_cluster_kernel<IT><<<CL_BLOCKS, CL_THREADS, SMEM, s>>>(a, passes, per, a.keys[0], a.pos[0]);
     }
-    a.zeroed = a.zero_rows != nullptr;
+    a.zeroed = a.zero_rows && IT <= 2;
     a.launches = a.zeroed ? 2 : 1;
     a.sorted_keys = a.keys[0];
     a.order = a.pos[0];
@@ -404,13 +405,16 @@ cudaError_t launch_row_sort(RowSortArgs& a, cudaStream_t s) {
     a.launches = 3 * passes;
     for (int p = 0; p < passes; ++p) {
         const int in = (p + 1) & 1, out = p & 1, shift = p * per;
+        const uint32_t *keys = a.keys[in], *pos = a.pos[in];
+        const dim3 block(SORT_THREADS);
+        cudaError_t e = cudaSuccess;
         if (p == 0) sort_count_kernel<true><<<tiles, SORT_THREADS, 0, s>>>(a, nullptr, shift, digits, items, tiles);
-        else sort_count_kernel<false><<<tiles, SORT_THREADS, 0, s>>>(a, a.keys[in], shift, digits, items, tiles);
-        sort_scan_kernel<<<digits, SORT_THREADS, 0, s>>>(a, tiles);
-        if (p == 0)
-            sort_scatter_kernel<true><<<tiles, SORT_THREADS, 0, s>>>(a, nullptr, nullptr, a.keys[out], a.pos[out], shift, digits, items, tiles);
-        else
-            sort_scatter_kernel<false><<<tiles, SORT_THREADS, 0, s>>>(a, a.keys[in], a.pos[in], a.keys[out], a.pos[out], shift, digits, items, tiles);
+        else e = launch_behind(sort_count_kernel<false>, dim3(tiles), block, s, a, keys, shift, digits, items, tiles);
+        if (e == cudaSuccess) e = launch_behind(sort_scan_kernel, dim3(digits), block, s, a, tiles);
+        if (e == cudaSuccess)
+            e = p == 0 ? launch_behind(sort_scatter_kernel<true>, dim3(tiles), block, s, a, keys, pos, a.keys[out], a.pos[out], shift, digits, items, tiles)
+                       : launch_behind(sort_scatter_kernel<false>, dim3(tiles), block, s, a, keys, pos, a.keys[out], a.pos[out], shift, digits, items, tiles);
+        if (e != cudaSuccess) return e;
         a.sorted_keys = a.keys[out];
         a.order = a.pos[out];
     }

@@ -19,13 +19,13 @@
 // so tokens that share an expert need no sorting or locking.  Rows are read
 // twice (dot products, then the updates); the second read hits L1/L2.
 //
-// SUMS_LATER: only the two factors of every (token, slot), dz and w act(z), are
-// written; the table gradients are then weighted sums of the rows of x and dy by
-// id (row_sum.cu), in fp32 and in one order.
+// With the table gradients left to sums by sorted id (row_sum.cu) a second
+// kernel writes only the two factors of every (token, slot), dz and w act(z).
 #include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "row_ops.cuh"
 
 namespace peer {
 
@@ -104,7 +104,7 @@ struct GradParams {
 // dy covers the same elements as a 16-byte chunk of a table row.
 // LP: the table gradients are accumulated in the tables' own 16-bit type (what the reference's bf16 training
 // does: its embedding gradients are bf16) instead of fp32: half the read-modify-write bytes, no cast afterwards.
-template <typename XT, int CH, bool LP, bool SUMS_LATER>
+template <typename XT, int CH, bool LP>
 __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p) {
     constexpr int EPC = Chunk16<XT>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -127,11 +127,7 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
             const int32_t id = __ldg(p.ids + t * p.HK + e);
             const float w = __ldg(p.weights + t * p.HK + e);
             if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.N)) {      // recorded and skipped
-                if (lane == 0) {
-                    atomicMax(p.status, STATUS_BOUNDS);
-                    p.dweights[t * p.HK + e] = 0.f;
-                    if (SUMS_LATER) p.coef_down[t * p.HK + e] = p.coef_up[t * p.HK + e] = 0.f;
-                }
+                if (lane == 0) { atomicMax(p.status, STATUS_BOUNDS); p.dweights[t * p.HK + e] = 0.f; }
                 continue;
             }
             const uint4* __restrict__ ur = reinterpret_cast<const uint4*>(p.down + static_cast<int64_t>(id) * row_u);
@@ -165,10 +161,6 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
             if (lane == 0) p.dweights[t * p.HK + e] = av * g;
             const float cv = w * av;
             const float dz = w * g * act_slope(z, p.activation);
-            if (SUMS_LATER && lane == 0) {
-                p.coef_down[t * p.HK + e] = dz;
-                p.coef_up[t * p.HK + e] = cv;
-            }
             using GT = typename std::conditional<LP, XT, float>::type;
             GT* __restrict__ du = static_cast<GT*>(p.d_down) + static_cast<int64_t>(id) * p.D;
             GT* __restrict__ dv = static_cast<GT*>(p.d_up) + static_cast<int64_t>(id) * p.Dout;
@@ -176,7 +168,7 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
             for (int i = 0; i < CH; ++i) {
                 const int c = lane + 32 * i;
                 float a[EPC], b[EPC];
-                if (!SUMS_LATER && c < p.nch_v) {
+                if (c < p.nch_v) {
                     Chunk16<XT>::decode(dyc[i], b);
                     if constexpr (LP && sizeof(XT) == 2) {
                         red_add_v4_bf16x2(dv + c * EPC, pack2(cv * b[0], cv * b[1]), pack2(cv * b[2], cv * b[3]),
@@ -192,8 +184,7 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
                     Chunk16<XT>::decode(xc[i], b);
 #pragma unroll
                     for (int q = 0; q < EPC; ++q) dxa[i * EPC + q] = fmaf(dz, a[q], dxa[i * EPC + q]);
-                    if constexpr (SUMS_LATER) {
-                    } else if constexpr (LP && sizeof(XT) == 2) {
+                    if constexpr (LP && sizeof(XT) == 2) {
                         red_add_v4_bf16x2(du + c * EPC, pack2(dz * b[0], dz * b[1]), pack2(dz * b[2], dz * b[3]),
                                           pack2(dz * b[4], dz * b[5]), pack2(dz * b[6], dz * b[7]));
                     } else {
@@ -217,23 +208,161 @@ __global__ void __launch_bounds__(THREADS) gather_grad_kernel(const GradParams p
     }
 }
 
-template <typename XT, int CH, bool LP, bool SUMS_LATER>
+template <typename XT, int CH, bool LP>
 cudaError_t launch_t(const GradParams& p, int sm_count, cudaStream_t s) {
     int64_t ctas = (p.T + WARPS - 1) / WARPS;
     const int64_t cap = static_cast<int64_t>(sm_count) * 4;      // a few CTAs per SM, grid-stride over tokens
     if (ctas > cap) ctas = cap;
-    gather_grad_kernel<XT, CH, LP, SUMS_LATER><<<static_cast<unsigned>(ctas), THREADS, 0, s>>>(p);
+    gather_grad_kernel<XT, CH, LP><<<static_cast<unsigned>(ctas), THREADS, 0, s>>>(p);
     return cudaGetLastError();
 }
 
-template <typename XT, bool LP, bool SUMS_LATER = false>
+template <typename XT, bool LP>
 cudaError_t launch_ch(const GradParams& p, int sm_count, cudaStream_t s) {
     const int max_ch = p.nch_u > p.nch_v ? p.nch_u : p.nch_v;
     const int need = (max_ch + 31) / 32;
-    if (need <= 1) return launch_t<XT, 1, LP, SUMS_LATER>(p, sm_count, s);
-    if (need <= 2) return launch_t<XT, 2, LP, SUMS_LATER>(p, sm_count, s);
-    if (need <= 4) return launch_t<XT, 4, LP, SUMS_LATER>(p, sm_count, s);
-    if (need <= 8) return launch_t<XT, 8, LP, SUMS_LATER>(p, sm_count, s);
+    if (need <= 1) return launch_t<XT, 1, LP>(p, sm_count, s);
+    if (need <= 2) return launch_t<XT, 2, LP>(p, sm_count, s);
+    if (need <= 4) return launch_t<XT, 4, LP>(p, sm_count, s);
+    if (need <= 8) return launch_t<XT, 8, LP>(p, sm_count, s);
+    return cudaErrorInvalidValue;
+}
+
+// The factors of the sorted form: dweights, dx, dz and w act(z), no table gradients.  What is left to move are the rows
+// themselves, so as in the forward pass they are kept on their way: every lane copies its own chunks of the next entries'
+// rows into shared memory (cp.async, nobody else reads them, so no barrier), FACTOR_DEPTH - 1 entries ahead; u is read from
+// there once and stays in registers for dx.  Ids, weights and results are held by the lanes, 32 entries at a time.
+// 16,384 tokens x 128 pairs of 4 KB rows: 2.5 ms = 6.9 TB/s; reading rows where they are used 7.5 ms.
+constexpr int FACTOR_WARPS = 8, FACTOR_DEPTH = 3;
+
+template <typename XT, int CH>
+__global__ void __launch_bounds__(FACTOR_WARPS * 32, 1) gather_factors_kernel(const GradParams p) {
+    constexpr int EPC = Chunk16<XT>::N, THREADS_F = FACTOR_WARPS * 32;
+    extern __shared__ __align__(16) unsigned char factor_smem[];      // [depth][u, v][chunk][thread] of 16 bytes
+    uint4* const mine = reinterpret_cast<uint4*>(factor_smem) + threadIdx.x;
+    auto at = [&](int slot, int which, int i) { return mine + ((slot * 2 + which) * CH + i) * THREADS_F; };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t row_u = static_cast<uint32_t>(p.nch_u) * 16u, row_v = static_cast<uint32_t>(p.nch_v) * 16u;
+    const int64_t nwarps = static_cast<int64_t>(gridDim.x) * FACTOR_WARPS;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * FACTOR_WARPS + warp; t < p.T; t += nwarps) {
+        const int32_t* __restrict__ ids = p.ids + t * p.HK;
+        const float* __restrict__ wts = p.weights + t * p.HK;
+        // lane l holds entry base + l of this block of 32 entries and of the next
+        int32_t id_now = lane < p.HK ? __ldg(ids + lane) : -1, id_next = 32 + lane < p.HK ? __ldg(ids + 32 + lane) : -1;
+        float w_now = lane < p.HK ? __ldg(wts + lane) : 0.f;
+        auto fetch = [&](int e, int base) {                 // entry e of blocks base, base + 32
+            const int32_t id = __shfl_sync(FULL_MASK, e - base < 32 ? id_now : id_next, e & 31);
+            if (e < p.HK && static_cast<uint32_t>(id) < static_cast<uint64_t>(p.N)) {
+                const int slot = e % FACTOR_DEPTH;
+                const char* u = p.down + static_cast<int64_t>(id) * row_u;
+                const char* v = p.up + static_cast<int64_t>(id) * row_v;
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const int c = lane + 32 * i;
+                    if (c < p.nch_u) copy_async<16>(smem_u32(at(slot, 0, i)), u + c * 16);
+                    if (c < p.nch_v) copy_async<16>(smem_u32(at(slot, 1, i)), v + c * 16);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int e = 0; e < FACTOR_DEPTH - 1; ++e) fetch(e, 0);
+        uint4 xc[CH], dyc[CH];
+        float dxa[CH * EPC];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int c = lane + 32 * i;
+            xc[i] = c < p.nch_u ? __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.x) + t * row_u) + c) : make_uint4(0u, 0u, 0u, 0u);
+            dyc[i] = c < p.nch_v ? __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.dy) + t * row_v) + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int q = 0; q < EPC; ++q) dxa[i * EPC + q] = 0.f;
+        }
+        float r_dw = 0.f, r_dz = 0.f, r_cv = 0.f;           // results of entry base + lane
+        for (int base = 0; base < p.HK; base += 32) {
+            const int count = min(32, p.HK - base);
+            for (int k = 0; k < count; ++k) {
+                const int e = base + k, slot = e % FACTOR_DEPTH;
+                fetch(e + FACTOR_DEPTH - 1, base);
+                asm volatile("cp.async.wait_group %0;" ::"n"(FACTOR_DEPTH - 1) : "memory");
+                const int32_t id = __shfl_sync(FULL_MASK, id_now, k);
+                const float w = __shfl_sync(FULL_MASK, w_now, k);
+                if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.N)) {      // recorded and skipped
+                    if (lane == 0) atomicMax(p.status, STATUS_BOUNDS);
+                    if (lane == k) r_dw = r_dz = r_cv = 0.f;
+                    continue;
+                }
+                uint4 u[CH];
+                float s[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const int c = lane + 32 * i;
+                    u[i] = c < p.nch_u ? *at(slot, 0, i) : make_uint4(0u, 0u, 0u, 0u);
+                    const uint4 v = c < p.nch_v ? *at(slot, 1, i) : make_uint4(0u, 0u, 0u, 0u);
+                    if constexpr (sizeof(XT) == 2) {
+                        dot8_bf16(u[i], xc[i], s[0]);
+                        dot8_bf16(v, dyc[i], s[1]);
+                    } else {
+                        float a[EPC], b[EPC];
+                        Chunk16<XT>::decode(u[i], a);
+                        Chunk16<XT>::decode(xc[i], b);
+#pragma unroll
+                        for (int q = 0; q < EPC; ++q) s[0] = fmaf(a[q], b[q], s[0]);
+                        Chunk16<XT>::decode(v, a);
+                        Chunk16<XT>::decode(dyc[i], b);
+#pragma unroll
+                        for (int q = 0; q < EPC; ++q) s[1] = fmaf(a[q], b[q], s[1]);
+                    }
+                }
+                const float z = warp_sum(s[0]), g = warp_sum(s[1]);
+                const float av = act_value(z, p.activation), dz = w * g * act_slope(z, p.activation);
+                if (lane == k) { r_dw = av * g; r_dz = dz; r_cv = w * av; }
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    float a[EPC];
+                    Chunk16<XT>::decode(u[i], a);
+#pragma unroll
+                    for (int q = 0; q < EPC; ++q) dxa[i * EPC + q] = fmaf(dz, a[q], dxa[i * EPC + q]);
+                }
+            }
+            if (lane < count) {
+                const int64_t at_e = t * p.HK + base + lane;
+                p.dweights[at_e] = r_dw;
+                p.coef_down[at_e] = r_dz;
+                p.coef_up[at_e] = r_cv;
+            }
+            id_now = id_next;
+            id_next = base + 64 + lane < p.HK ? __ldg(ids + base + 64 + lane) : -1;
+            w_now = base + 32 + lane < p.HK ? __ldg(wts + base + 32 + lane) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int c = lane + 32 * i;
+            if (c < p.nch_u) {
+#pragma unroll
+                for (int q = 0; q < EPC; q += 4)
+                    *reinterpret_cast<float4*>(p.dx + t * p.D + c * EPC + q) =
+                        make_float4(dxa[i * EPC + q], dxa[i * EPC + q + 1], dxa[i * EPC + q + 2], dxa[i * EPC + q + 3]);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");    // only empty groups are left
+    }
+}
+
+template <typename XT, int CH>
+cudaError_t launch_factors(const GradParams& p, int sm_count, cudaStream_t s) {
+    constexpr int SMEM = FACTOR_DEPTH * 2 * CH * FACTOR_WARPS * 32 * 16;
+    const cudaError_t e = cudaFuncSetAttribute(gather_factors_kernel<XT, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t need = (p.T + FACTOR_WARPS - 1) / FACTOR_WARPS, cap = static_cast<int64_t>(sm_count) * (CH == 8 ? 1 : 2);
+    gather_factors_kernel<XT, CH><<<static_cast<unsigned>(need < cap ? need : cap), FACTOR_WARPS * 32, SMEM, s>>>(p);
+    return cudaGetLastError();
+}
+template <typename XT>
+cudaError_t launch_factors_ch(const GradParams& p, int sm_count, cudaStream_t s) {
+    const int need = ((p.nch_u > p.nch_v ? p.nch_u : p.nch_v) + 31) / 32;
+    if (need <= 1) return launch_factors<XT, 1>(p, sm_count, s);
+    if (need <= 2) return launch_factors<XT, 2>(p, sm_count, s);
+    if (need <= 4) return launch_factors<XT, 4>(p, sm_count, s);
+    if (need <= 8) return launch_factors<XT, 8>(p, sm_count, s);
     return cudaErrorInvalidValue;
 }
 
@@ -252,8 +381,8 @@ cudaError_t launch_gather_grad(const GatherGradArgs& a, cudaStream_t s) {
     p.nch_u = a.D * tb / 16; p.nch_v = a.Dout * tb / 16;
     p.coef_down = a.coef_down; p.coef_up = a.coef_up;
     if (a.coef_down) {
-        if (a.act_dtype == PEER_DTYPE_F32) return launch_ch<float, false, true>(p, a.sm_count, s);
-        if (a.act_dtype == PEER_DTYPE_BF16) return launch_ch<__nv_bfloat16, false, true>(p, a.sm_count, s);
+        if (a.act_dtype == PEER_DTYPE_F32) return launch_factors_ch<float>(p, a.sm_count, s);
+        if (a.act_dtype == PEER_DTYPE_BF16) return launch_factors_ch<__nv_bfloat16>(p, a.sm_count, s);
         return cudaErrorInvalidValue;
     }
     if (a.act_dtype == PEER_DTYPE_F32) return launch_ch<float, false>(p, a.sm_count, s);       // fp32 either way

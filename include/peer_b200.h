@@ -340,7 +340,8 @@ int peer_usage_histogram(const int64_t* ids, int64_t n_ids, int64_t* counts, int
  * No handle: every buffer, workspaces included, is the caller's, so calls on different streams or in
  * different captured graphs never share memory.  All are asynchronous on `stream` of the current device.
  * Rows are `dim` consecutive values (1 <= dim <= PEER_ROW_DIM_MAX); inputs may have a row stride (in
- * elements) of their own, outputs are contiguous.  dtype: F32, BF16 or F16; sums and statistics are fp32.
+ * elements) of their own, outputs are contiguous and overlap no input; pointers are aligned to their type.
+ * dtype: F32, BF16 or F16; sums and statistics are fp32.
  * Results do not vary from run to run (no accumulation in memory). */
 #define PEER_ROW_DIM_MAX (1 << 20)
 

@@ -85,6 +85,9 @@ extern "C" int peer_embedding(const void* ids, int32_t id_bytes, int64_t n_ids, 
     if (id_bytes != 4 && id_bytes != 8) return refuse("peer_embedding: ids are int32 or int64");
     if (n_ids == 0) return PEER_OK;
     if (!ids || !weight || !out) return refuse("peer_embedding: null pointer");
+    if ((reinterpret_cast<uintptr_t>(ids) & (id_bytes - 1)) || !aligned_to(weight, dtype) || !aligned_to(out, dtype) ||
+        (reinterpret_cast<uintptr_t>(dropped) & 7u))
+        return refuse("peer_embedding: a pointer is not aligned to its type");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PEER_DTYPE_F32) return report("peer_embedding", embed_t<float>(ids, id_bytes, n_ids, weight, vocab, dim, scale, out, dropped, s));
     if (dtype == PEER_DTYPE_BF16) return report("peer_embedding", embed_t<__nv_bfloat16>(ids, id_bytes, n_ids, weight, vocab, dim, scale, out, dropped, s));
@@ -108,6 +111,9 @@ extern "C" int peer_embedding_backward(const void* ids, int32_t id_bytes, int64_
     if (!grad_weight || (n_ids > 0 && (!ids || !grad))) return refuse("peer_embedding_backward: null pointer");
     if (n_ids > 0 && (!workspace || workspace_bytes < peer_embedding_workspace(n_ids, dim)))
         return refuse("peer_embedding_backward: workspace is missing or smaller than peer_embedding_workspace says");
+    if ((reinterpret_cast<uintptr_t>(ids) & (id_bytes - 1)) || !aligned_to(grad, dtype) || !aligned_to(grad_weight, dtype) ||
+        !aligned16(workspace))
+        return refuse("peer_embedding_backward: a pointer is not aligned to its type, or the workspace to 16 bytes");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (n_ids == 0)
         return report("peer_embedding_backward",

@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
             other = -other;
         }
         const float rstd = inverse_sqrt(m2 * inv_d + p.eps);
-        const float2 r2 = splat(rstd), c2 = splat(-mean * rstd);
+        const float2 r2 = splat(rstd), m2p = splat(-mean);
         const int e = PACK ? e4m3_scale_exponent(top) : 0;
         const float inv = exp2_int(-e);
 #pragma unroll
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
                 float f[N];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    const float2 v = __ffma2_rn(__ffma2_rn(x[i][h], r2, c2), w[i][h], b[i][h]);
+                    const float2 v = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[i][h], m2p), r2), w[i][h], b[i][h]);
                     f[2 * h] = v.x;
                     f[2 * h + 1] = v.y;
                 }
@@ -912,7 +912,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
             other = -other;
         }
         const float rstd = inverse_sqrt(m2 * inv_d + p.eps);
-        const float2 r2 = splat(rstd), c2 = splat(-mean * rstd);
+        const float2 r2 = splat(rstd), m2p = splat(-mean);
         const int e = PACK ? e4m3_scale_exponent(top) : 0;
         const float inv = exp2_int(-e);
 #pragma unroll
@@ -921,7 +921,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
                 float f[N];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    const float2 v = __ffma2_rn(__ffma2_rn(x[i][h], r2, c2), w[i][h], b[i][h]);
+                    const float2 v = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[i][h], m2p), r2), w[i][h], b[i][h]);
                     f[2 * h] = v.x;
                     f[2 * h + 1] = v.y;
                 }
@@ -1359,6 +1359,9 @@ extern "C" int peer_layer_norm(const void* x, int64_t x_stride, int32_t dtype, c
     if ((payload == nullptr) != (scale == nullptr)) return refuse("peer_layer_norm: payload and scale come together");
     if (rows == 0) return PEER_OK;
     if (!x || !y) return refuse("peer_layer_norm: null pointer");
+    if (!aligned_to(x, dtype) || !aligned_to(y, dtype) || !aligned_to(weight, param_dtype) || !aligned_to(bias, param_dtype) ||
+        !aligned_to(mean, PEER_DTYPE_F32) || !aligned_to(rstd, PEER_DTYPE_F32) || !aligned_to(scale, PEER_DTYPE_F32))
+        return refuse("peer_layer_norm: a pointer is not aligned to its type");
     NormParams p{x, x_stride, weight, bias, param_dtype == PEER_DTYPE_F32, eps, rows, dim, y, mean, rstd,
                  static_cast<uint8_t*>(payload), scale};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1388,6 +1391,11 @@ extern "C" int peer_layer_norm_backward(const void* grad_y, int64_t grad_stride,
         return refuse("peer_layer_norm_backward: grad_y, mean, rstd and x (or its packed form) are required");
     if ((grad_weight || grad_bias) && (!workspace || workspace_bytes < peer_layer_norm_workspace(rows, dim)))
         return refuse("peer_layer_norm_backward: workspace is missing or smaller than peer_layer_norm_workspace says");
+    if (!aligned_to(grad_y, dtype) || !aligned_to(x, dtype) || !aligned_to(add, dtype) || !aligned_to(grad_x, dtype) ||
+        !aligned_to(weight, param_dtype) || !aligned_to(grad_weight, param_dtype) || !aligned_to(grad_bias, param_dtype) ||
+        !aligned_to(mean, PEER_DTYPE_F32) || !aligned_to(rstd, PEER_DTYPE_F32) || !aligned_to(scale, PEER_DTYPE_F32) ||
+        !aligned16(workspace))
+        return refuse("peer_layer_norm_backward: a pointer is not aligned to its type, or the workspace to 16 bytes");
     if (rows == 0 && !grad_weight && !grad_bias) return PEER_OK;
     NormGradParams p{grad_y, grad_stride, x, x_stride, static_cast<const uint8_t*>(payload), scale, mean, rstd, weight,
                      param_dtype == PEER_DTYPE_F32, add, rows, dim, rows ? grad_x : nullptr, grad_weight, grad_bias,

@@ -325,6 +325,7 @@ constexpr int GRID_SMS = 148;
 struct RowShape { int warps, groups, nv, u_rows; };
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned_to(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == PEER_DTYPE_F32 ? 3u : 1u)) == 0; }
 
 // Many rows: up to nv_max pieces per thread (doubling from nv_min until one warp takes the row), so that a row needs
 // few warps and few exchanges between them.  Fewer than 1024 rows (under seven per SM): nv_min, a row is then spread

@@ -312,6 +312,7 @@ extern "C" int peer_pack_rows(const void* x, int64_t x_stride, int32_t dtype, in
         return refuse("peer_pack_rows: negative row count or stride, or dim outside [1, 2^20]");
     if (rows == 0) return PEER_OK;
     if (!x || !payload || !scale) return refuse("peer_pack_rows: null pointer");
+    if (!aligned_to(x, dtype) || !aligned_to(scale, PEER_DTYPE_F32)) return refuse("peer_pack_rows: a pointer is not aligned to its type");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* p = static_cast<uint8_t*>(payload);
     if (dtype == PEER_DTYPE_F32) return report("peer_pack_rows", pack_t<float>(x, x_stride, rows, dim, p, scale, s));
@@ -326,6 +327,7 @@ extern "C" int peer_unpack_rows(const void* payload, const float* scale, int32_t
         return refuse("peer_unpack_rows: negative row count, or dim outside [1, 2^20]");
     if (rows == 0) return PEER_OK;
     if (!payload || !scale || !out) return refuse("peer_unpack_rows: null pointer");
+    if (!aligned_to(out, dtype) || !aligned_to(scale, PEER_DTYPE_F32)) return refuse("peer_unpack_rows: a pointer is not aligned to its type");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint8_t* p = static_cast<const uint8_t*>(payload);
     if (dtype == PEER_DTYPE_F32) return report("peer_unpack_rows", unpack_t<float>(p, scale, rows, dim, out, s));

@@ -225,11 +225,49 @@ def test_layer_norm_keeps_rows_apart(cuda_device):
 
 def test_layer_norm_of_a_large_mean(cuda_device):
     """Values near 1000 with a deviation of 0.5: the variance is not lost to cancellation."""
-    x = 1000 + 0.5 * torch.randn(64, 2048, device=cuda_device)
-    y = lib.layer_norm(x)
-    ref, err = norm_reference(x, None, None, 1e-5, x)
-    close(y, ref[0], err[0], "y")
-    assert (y - ref[0]).abs().max() < 2e-3                     # mean rounded to fp32: 1000 * 2^-24 / 0.5 and its sums
+    for R, D in ((64, 2048), (1100, 2048), (1100, 1999), (1030, 530)):
+        x = (1000 + 0.5 * torch.randn(R, D, device=cuda_device)).requires_grad_()
+        dy = torch.randn(R, D, device=cuda_device)
+        y = lib.layer_norm(x)
+        dx, = torch.autograd.grad(y, (x,), dy)
+        ref, err = norm_reference(x.detach(), None, None, 1e-5, dy)
+        close(y.detach(), ref[0], err[0], "y")
+        close(dx, ref[1], err[1], "dx")
+        assert (y - ref[0]).abs().max() < 2e-3                 # mean rounded to fp32: 1000 * 2^-24 / 0.5 and its sums
+
+
+def test_rows_behind_two_to_the_31_elements(cuda_device):
+    """Rows whose offsets pass 32 bits: the last 3000 of 1.1 million rows of 2048 (and of 2047) against a call on them
+    alone, and table rows at the end of a table of that size."""
+    n, tail = 1_100_000, 3000                                  # enough rows for the kernels of many rows
+    for D in (2048, 2047):
+        base = torch.randn(5000, D, device=cuda_device).bfloat16()
+        x = base.repeat(n // 5000, 1)
+        w, b = params(D, torch.float32, 7, cuda_device)
+        for ck in (None, "e4m3"):
+            outs = []
+            for t in (x, x[-tail:].clone()):
+                t = t.detach().requires_grad_()
+                y = lib.layer_norm(t, w, b, checkpoint=ck)
+                dx, = torch.autograd.grad(y, (t,), t.detach())
+                outs.append((y.detach()[-tail:].clone(), dx[-tail:].clone()))
+                del y, dx, t
+            assert all(torch.equal(p, q) for p, q in zip(*outs))
+        payload, scale = lib.pack_rows_e4m3(x)
+        few, few_scale = lib.pack_rows_e4m3(x[-tail:])
+        assert torch.equal(payload[-tail:].view(torch.uint8), few.view(torch.uint8)) and torch.equal(scale[-tail:], few_scale)
+        assert torch.equal(lib.unpack_rows_e4m3(payload, scale)[-tail:], lib.unpack_rows_e4m3(few, few_scale))
+        del payload, scale
+        ids = torch.randint(n - 300, n, (4096,), device=cuda_device)
+        table = x.requires_grad_()
+        out = lib.embedding(ids, table, 2.0)
+        assert torch.equal(out.detach(), (x.detach()[ids].float() * 2.0).bfloat16())
+        g, = torch.autograd.grad(out, (table,), out.detach())
+        small = x.detach()[n - 300:].clone().requires_grad_()
+        gs, = torch.autograd.grad(lib.embedding(ids - (n - 300), small, 2.0), (small,), out.detach())
+        assert torch.equal(g[n - 300:], gs) and not g[:n - 300].any()
+        del x, table, out, g, small, gs, outs
+        torch.cuda.empty_cache()
 
 
 def test_layer_norm_against_differences(cuda_device):

@@ -33,7 +33,8 @@ def _norm(native, **kw):
 def test_layer_norm_entry_refuses_before_any_launch():
     native = _lib.load()
     bad = [dict(x=None), dict(y=None), dict(rows=-1), dict(dim=0), dict(dim=(1 << 20) + 1), dict(xs=-8), dict(dt=E4M3),
-           dict(pdt=_lib.DTYPE_F16), dict(eps=-1.0), dict(eps=float("nan")), dict(payload=16), dict(scale=16)]
+           dict(pdt=_lib.DTYPE_F16), dict(eps=-1.0), dict(eps=float("nan")), dict(payload=16), dict(scale=16),
+           dict(x=17), dict(y=17), dict(w=18), dict(mean=18)]
     for kw in bad:
         assert _norm(native, **kw) == _lib.ERR_INVALID_ARG, kw
         assert "peer_layer_norm" in _lib.last_error(None)
@@ -55,7 +56,7 @@ def test_layer_norm_backward_entry_refuses_before_any_launch():
     assert need > 0
     bad = [dict(dy=None), dict(x=None), dict(mean=None), dict(rstd=None), dict(rows=-1), dict(dim=0), dict(dt=9), dict(xs=-1),
            dict(dys=-1), dict(payload=16), dict(dw=16), dict(dw=16, ws=16, wb=need - 1), dict(db=16, ws=None, wb=need),
-           dict(pdt=_lib.DTYPE_F16)]
+           dict(pdt=_lib.DTYPE_F16), dict(dy=17), dict(dx=17), dict(add=17), dict(dw=16, ws=24, wb=need)]
     for kw in bad:
         assert _norm_grad(native, **kw) == _lib.ERR_INVALID_ARG, kw
         assert "peer_layer_norm_backward" in _lib.last_error(None)
@@ -66,9 +67,10 @@ def test_packing_entries_refuse_before_any_launch():
     native = _lib.load()
     pack = lambda x=16, xs=8, dt=BF16, rows=4, dim=8, p=16, s=16: native.peer_pack_rows(x, xs, dt, rows, dim, p, s, None)
     unpack = lambda p=16, s=16, dt=BF16, rows=4, dim=8, o=16: native.peer_unpack_rows(p, s, dt, rows, dim, o, None)
-    for kw in (dict(x=None), dict(p=None), dict(s=None), dict(rows=-1), dict(dim=0), dict(dim=1 << 21), dict(dt=E4M3), dict(xs=-1)):
+    for kw in (dict(x=None), dict(p=None), dict(s=None), dict(rows=-1), dict(dim=0), dict(dim=1 << 21), dict(dt=E4M3), dict(xs=-1),
+               dict(x=17), dict(s=18)):
         assert pack(**kw) == _lib.ERR_INVALID_ARG, kw
-    for kw in (dict(o=None), dict(p=None), dict(s=None), dict(rows=-1), dict(dim=0), dict(dim=1 << 21), dict(dt=E4M3)):
+    for kw in (dict(o=None), dict(p=None), dict(s=None), dict(rows=-1), dict(dim=0), dict(dim=1 << 21), dict(dt=E4M3), dict(o=17)):
         assert unpack(**kw) == _lib.ERR_INVALID_ARG, kw
     assert pack(rows=0) == _lib.OK and unpack(rows=0) == _lib.OK
 
@@ -80,7 +82,7 @@ def test_embedding_entries_refuse_before_any_launch():
         return native.peer_embedding(ids, ib, n, w, dt, V, D, 1.0, out, None, None)
 
     for kw in (dict(ids=None), dict(w=None), dict(out=None), dict(ib=2), dict(n=-1), dict(V=0), dict(V=1 << 31), dict(D=0),
-               dict(D=1 << 21), dict(dt=E4M3)):
+               dict(D=1 << 21), dict(dt=E4M3), dict(ids=20), dict(w=17)):
         assert fwd(**kw) == _lib.ERR_INVALID_ARG, kw
         assert "peer_embedding" in _lib.last_error(None)
     assert fwd(n=0) == _lib.OK
@@ -91,7 +93,7 @@ def test_embedding_entries_refuse_before_any_launch():
         return native.peer_embedding_backward(ids, ib, n, g, gs, dt, V, D, 1.0, -1, gw, ws, wb, None)
 
     for kw in (dict(ids=None), dict(g=None), dict(gw=None), dict(ws=None), dict(wb=need - 1), dict(ib=1), dict(n=-1), dict(V=0),
-               dict(D=0), dict(gs=-1), dict(dt=E4M3), dict(n=1 << 31)):
+               dict(D=0), dict(gs=-1), dict(dt=E4M3), dict(n=1 << 31), dict(gw=17), dict(ws=24)):
         assert bwd(**kw) == _lib.ERR_INVALID_ARG, kw
         assert "peer_embedding_backward" in _lib.last_error(None)
 

@@ -106,6 +106,15 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 
+// shared to global memory, asynchronously: addresses and size multiples of 16 bytes.  The wait covers the calling thread's
+// copies and comes before the block ends.
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_s2g_wait() {
+    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 // ---------------------------------------------------------------------------
 // Pieces of a row: what one thread loads at once.  Wide: 16 bytes (rows whose start, stride and width are multiples
 // of 16 bytes); narrow: one value.

@@ -200,42 +200,60 @@ struct ClusterShared {
 // in a bitmap (every block reads all ids, from L2) and writes the unmarked rows.  Launched in front of the sort, which
 // starts as soon as all of these blocks run (programmatic launch; they leave room for it on every SM) and waits for
 // their end only in its last instruction.
-constexpr int ZERO_THREADS = 256, ZERO_WORDS = 1024, ZERO_IDS = 8;      // 32 registers a thread: eight warps fit beside a block of the sort
+// The rows are written by bulk copies from a block of zeros in shared memory: one instruction per 4 KB, so the few warps
+// that fit beside the sort are enough: 262 MB in 44 us.  The ids come through shared memory too, 8,192 at a time, because
+// the registers for that many loads in flight would not fit.
+constexpr int ZERO_THREADS = 256, ZERO_WORDS = 1024;      // 32 registers a thread: eight warps fit beside a block of the sort
+constexpr int ZERO_BYTES = 4096, ZERO_IDS = 8192;
 __global__ void __launch_bounds__(ZERO_THREADS, 8) zero_unnamed_kernel(const RowSortArgs a) {
     __shared__ uint32_t marks[ZERO_WORDS];
+    __shared__ __align__(16) uint4 zeros[ZERO_BYTES / 16];
+    extern __shared__ __align__(16) unsigned char staged[];      // [ZERO_IDS] as they come
     grid_release();
     const int64_t each = (a.vocab + gridDim.x - 1) / gridDim.x;
     const int64_t first = each * blockIdx.x, last = first + each < a.vocab ? first + each : a.vocab;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool vec = a.row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(a.zero_rows) & 15u) == 0;
+    for (int i = threadIdx.x; i < ZERO_BYTES / 16; i += ZERO_THREADS) zeros[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();                                     // the copies read them
     for (int64_t v0 = first; v0 < last; v0 += ZERO_WORDS * 32) {
         const int64_t v1 = v0 + ZERO_WORDS * 32 < last ? v0 + ZERO_WORDS * 32 : last;
         for (int i = threadIdx.x; i < ZERO_WORDS; i += ZERO_THREADS) marks[i] = 0u;
         __syncthreads();
-        for (int64_t i0 = threadIdx.x; i0 < a.n; i0 += ZERO_THREADS * ZERO_IDS) {
-            uint32_t id[ZERO_IDS];                           // loaded together: 16,384 ids are eight rounds of latency
-#pragma unroll
-            for (int k = 0; k < ZERO_IDS; ++k) {
-                const int64_t i = i0 + k * ZERO_THREADS;
-                id[k] = source_key(a, i < a.n ? i : a.n - 1);
+        for (int64_t i0 = 0; i0 < a.n; i0 += ZERO_IDS) {    // a thread reads only what it copied itself
+            const int count = static_cast<int>(a.n - i0 < ZERO_IDS ? a.n - i0 : ZERO_IDS);
+            if (a.id_bytes == 8) {
+                for (int k = threadIdx.x; k < count; k += ZERO_THREADS)
+                    copy_async<8>(smem_u32(staged + k * 8), static_cast<const int64_t*>(a.ids) + i0 + k);
+            } else {
+                for (int k = threadIdx.x; k < count; k += ZERO_THREADS)
+                    copy_async<4>(smem_u32(staged + k * 4), static_cast<const int32_t*>(a.ids) + i0 + k);
             }
-#pragma unroll
-            for (int k = 0; k < ZERO_IDS; ++k)
-                if (id[k] >= v0 && id[k] < v1) atomicOr(&marks[(id[k] - v0) >> 5], 1u << ((id[k] - v0) & 31));
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int k = threadIdx.x; k < count; k += ZERO_THREADS) {
+                const int64_t id = a.id_bytes == 8 ? reinterpret_cast<const int64_t*>(staged)[k] : reinterpret_cast<const int32_t*>(staged)[k];
+                if (id >= v0 && id < v1 && id != a.skip) atomicOr(&marks[(id - v0) >> 5], 1u << ((id - v0) & 31));
+            }
         }
         __syncthreads();
-        for (int64_t v = v0 + warp; v < v1; v += ZERO_THREADS / 32) {
-            if (marks[(v - v0) >> 5] >> ((v - v0) & 31) & 1u) continue;
-            char* row = static_cast<char*>(a.zero_rows) + v * a.row_bytes;
-            if (vec) {
-#pragma unroll 4
-                for (int64_t c = lane; c < a.row_bytes / 16; c += 32) reinterpret_cast<uint4*>(row)[c] = make_uint4(0u, 0u, 0u, 0u);
-            } else {                                     // rows of 2- or 4-byte values
-                for (int64_t c = lane; c < a.row_bytes / 2; c += 32) reinterpret_cast<uint16_t*>(row)[c] = 0;
+        if (vec) {
+            // lane l of warp w: rows v0 + 256 j + 32 w + l, so a word of marks is one warp's
+            for (int64_t v = v0 + threadIdx.x; v < v1; v += ZERO_THREADS) {
+                if (marks[(v - v0) >> 5] >> ((v - v0) & 31) & 1u) continue;
+                char* row = static_cast<char*>(a.zero_rows) + v * a.row_bytes;
+                for (int64_t c = 0; c < a.row_bytes; c += ZERO_BYTES)
+                    bulk_s2g(row + c, smem_u32(zeros), static_cast<uint32_t>(a.row_bytes - c < ZERO_BYTES ? a.row_bytes - c : ZERO_BYTES));
+            }
+        } else {                                             // rows of 2- or 4-byte values at any address
+            for (int64_t v = v0 + warp; v < v1; v += ZERO_THREADS / 32) {
+                if (marks[(v - v0) >> 5] >> ((v - v0) & 31) & 1u) continue;
+                uint16_t* row = reinterpret_cast<uint16_t*>(static_cast<char*>(a.zero_rows) + v * a.row_bytes);
+                for (int64_t c = lane; c < a.row_bytes / 2; c += 32) row[c] = 0;
             }
         }
         __syncthreads();
     }
+    bulk_s2g_wait();
 }
 
 // pairs i of block b, warp w, round k, lane l:  i = ((b * CL_WARPS + w) * IT + k) * 32 + l
@@ -377,7 +395,9 @@ static cudaError_t launch_cluster(RowSortArgs& a, int passes, int per, cudaStrea
     if (e != cudaSuccess) return e;
     if (a.zero_rows && IT <= 2) {                        // four and more pairs a thread: the registers of a whole SM
         const int64_t blocks = a.vocab < GRID_SMS ? a.vocab : GRID_SMS;
-        zero_unnamed_kernel<<<static_cast<unsigned>(blocks), ZERO_THREADS, 0, s>>>(a);
+        const cudaError_t em = cudaFuncSetAttribute(zero_unnamed_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ZERO_IDS * 8);
+        if (em != cudaSuccess) return em;
+        zero_unnamed_kernel<<<static_cast<unsigned>(blocks), ZERO_THREADS, ZERO_IDS * 8, s>>>(a);
         const cudaError_t ez = launch_behind_smem(sort_cluster_kernel<IT>, dim3(CL_BLOCKS), dim3(CL_THREADS), SMEM, s, a, passes, per, a.keys[0], a.pos[0]);
         if (ez != cudaSuccess) return ez;
     } else {

@@ -197,7 +197,7 @@ def _selection_buffers(module, x):
 
 def _kept(module, x):
     """What a node keeps of its input x: (x, None, None), or (None, payload, scale) in 8 bits."""
-    mode = module.activation_checkpoint
+    mode = getattr(module, "activation_checkpoint", None)
     if mode not in (None, "e4m3"):
         raise ValueError(f"activation_checkpoint={mode!r}: None or 'e4m3'")
     return (x, None, None) if mode is None else (None, *pack_rows_e4m3(x))
@@ -309,7 +309,7 @@ def peer_forward_autograd(module, hidden_states: torch.Tensor) -> torch.Tensor:
 def _forward_with_dropout(module, x, w, B, S):
     """Training mode with dropout of the expert activations (experts.py:366): the stages as separate autograd
     nodes, so that the per-slot dropout factor can sit between the softmax and the expert stage."""
-    if module.activation_checkpoint is not None:
+    if getattr(module, "activation_checkpoint", None) is not None:
         raise RuntimeError("activation_checkpoint is not implemented together with dropout: the stages are separate nodes")
     if module.expert_hidden_size != 1:
         raise RuntimeError("dropout with expert_hidden_size > 1 is not implemented (it acts on every neuron)")

@@ -62,6 +62,7 @@ cudaError_t embed_t(const void* ids, int id_bytes, int64_t n, const void* w, int
 
 int report(const char* name, cudaError_t e) {
     if (e == cudaSuccess) return PEER_OK;
+    cudaGetLastError();                                      // reported here, not by the next launch's check
     char buf[256];
     snprintf(buf, sizeof buf, "%s: %s", name, cudaGetErrorString(e));
     set_global_error(buf);

@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
                 }
                 P::store(dst + i * threads * N, P::encode(f));
                 if constexpr (PACK)
-                    *reinterpret_cast<typename P::Packed*>(dst8 + i * threads * N) = pack_piece<T, true>(raw[i], inv, odd);
+                    *reinterpret_cast<typename P::Packed*>(dst8 + i * threads * N) = pack_pairs<T>(x[i], raw[i], inv, odd);
             }
         dst += dst_step;
         if (PACK) dst8 += dst_step;
@@ -926,7 +926,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
                     f[2 * h + 1] = v.y;
                 }
                 store_shared(out + (gt + i * threads) * 16, P::encode(f));
-                if constexpr (PACK) store_shared(out8 + (gt + i * threads) * XB, pack_piece<T, true>(raw[i], inv, odd));
+                if constexpr (PACK) store_shared(out8 + (gt + i * threads) * XB, pack_pairs<T>(x[i], raw[i], inv, odd));
             }
         sync();
         store_row<T>(static_cast<T*>(p.y) + r * p.D, out, bytes, gt, threads);
@@ -1331,6 +1331,7 @@ cudaError_t norm_grad_t(const NormGradParams& p, cudaStream_t s) {
 
 int report(const char* name, cudaError_t e) {
     if (e == cudaSuccess) return PEER_OK;
+    cudaGetLastError();                                      // reported here, not by the next launch's check
     char buf[256];
     snprintf(buf, sizeof buf, "%s: %s", name, cudaGetErrorString(e));
     set_global_error(buf);

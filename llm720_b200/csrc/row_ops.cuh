@@ -269,6 +269,21 @@ __device__ __forceinline__ typename Piece<T, WIDE>::Packed pack_piece(const type
     return Piece<T, WIDE>::encode_packed(f);
 }
 
+// the same from values decoded before; `x` is looked at only when the warp holds infinities or NaN
+template <typename T>
+__device__ __forceinline__ typename Piece<T, true>::Packed pack_pairs(const float2 (&v)[Piece<T, true>::N / 2], const uint4& x, float inv, bool odd) {
+    constexpr int N = Piece<T, true>::N;
+    if (odd) return pack_piece<T, true>(x, inv, true);
+    float f[N];
+#pragma unroll
+    for (int h = 0; h < N / 2; ++h) {
+        const float2 s = __fmul2_rn(v[h], make_float2(inv, inv));
+        f[2 * h] = s.x;
+        f[2 * h + 1] = s.y;
+    }
+    return Piece<T, true>::encode_packed(f);
+}
+
 // Sums of K values (a power of two) over the warp in K - 1 + 5 - log2(K) shuffles: each step halves the values a lane
 // carries.  On return lane k * (32 / K) (and its neighbours up to the next) holds the sum of v[k] as the result.
 template <int K>
@@ -318,7 +333,9 @@ inline cudaError_t launch_behind_smem(void (*kernel)(Params...), dim3 grid, dim3
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+    if (e != cudaSuccess) cudaGetLastError();               // reported here, not by the next launch's check
+    return e;
 }
 template <typename... Params, typename... Args>
 inline cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {

@@ -291,6 +291,7 @@ cudaError_t unpack_t(const uint8_t* payload, const float* scale, int64_t rows, i
 
 int report(const char* name, cudaError_t e) {
     if (e == cudaSuccess) return PEER_OK;
+    cudaGetLastError();                                      // reported here, not by the next launch's check
     char buf[256];
     snprintf(buf, sizeof buf, "%s: %s", name, cudaGetErrorString(e));
     set_global_error(buf);

@@ -270,6 +270,29 @@ def test_rows_behind_two_to_the_31_elements(cuda_device):
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,D", [(5, 31), (40, 256), (1500, 77), (1500, 512), (2100, 515), (1030, 1536), (3, 20001)])
+def test_gradient_of_a_residual_is_added_before_the_rounding(cuda_device, R, D, dtype):
+    """The C entry's ``add``, on every kind of row: dx + add, rounded once."""
+    from llm720_b200 import _lib
+    x, add = stream_rows(R, D, dtype, 1, cuda_device), stream_rows(R, D, dtype, 2, cuda_device)
+    dy = torch.randn(R, D, device=cuda_device).to(dtype)
+    w, _ = params(D, torch.float32, 1, cuda_device)
+    mean = x.double().mean(-1).float()
+    rstd = (1 / torch.sqrt(x.double().var(-1, unbiased=False) + 1e-5)).float()
+    out, dw = torch.empty_like(x), torch.empty(D, device=cuda_device)
+    native = _lib.load()
+    n = native.peer_layer_norm_workspace(R, D)
+    ws = torch.empty(n, dtype=torch.uint8, device=cuda_device)
+    code = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}[dtype]
+    _lib.check(native.peer_layer_norm_backward(
+        dy.data_ptr(), D, x.data_ptr(), D, None, None, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), code, _lib.DTYPE_F32,
+        add.data_ptr(), R, D, out.data_ptr(), dw.data_ptr(), None, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream))
+    ref, err = norm_reference(x, w, None, 1e-5, dy)
+    close(out, ref[1] + add.double(), err[1] + 2 * U * (ref[1].abs() + add.double().abs()), "dx + add")
+    close(dw, ref[2], err[2], "dw")
+
+
 def test_layer_norm_against_differences(cuda_device):
     """dx, dw, db against central differences of sum(y * dy), y from the fp32 kernel, summed in 64 bits.  y carries
     an error of at most ~8 u |y|; through sum|dy| (~200) and h = 2^-6 that is ~2e-2; the third-order term h^2/6 is
@@ -544,7 +567,7 @@ def _all_outputs(x, w, b, table, ids, dy, dye):
     return [t.detach() for t in (y, *g, e, ge, back)]
 
 
-def _inputs(device, seed, n=300, D=264, V=90):
+def _inputs(device, seed, n, D, V):
     g = torch.Generator(device=device).manual_seed(seed)
     r = lambda *s: torch.randn(*s, generator=g, device=device)
     x, table = r(n, D).bfloat16().requires_grad_(), r(V, D).bfloat16().requires_grad_()
@@ -553,8 +576,12 @@ def _inputs(device, seed, n=300, D=264, V=90):
     return x, w, b, table, ids, r(n, D).bfloat16(), r(n, D).bfloat16()
 
 
-def test_two_streams_at_once(cuda_device):
-    sets = [_inputs(cuda_device, s) for s in (1, 2)]
+SIZES = [(300, 264, 90), (70000, 24, 90), (20000, 33, 5000)]       # one launch for the sort, three per digit, odd rows
+
+
+@pytest.mark.parametrize("n,D,V", SIZES)
+def test_two_streams_at_once(cuda_device, n, D, V):
+    sets = [_inputs(cuda_device, s, n, D, V) for s in (1, 2)]
     want = [_all_outputs(*s) for s in sets]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(cuda_device) for _ in sets]
@@ -569,10 +596,11 @@ def test_two_streams_at_once(cuda_device):
             assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
 
 
-def test_captured_and_replayed_with_new_inputs(cuda_device):
+@pytest.mark.parametrize("n,D,V", SIZES)
+def test_captured_and_replayed_with_new_inputs(cuda_device, n, D, V):
     """Forward and backward in two captured graphs, replayed in turn with other inputs."""
-    sets = [_inputs(cuda_device, s) for s in (3, 4)]
-    fresh = [[t.detach().clone() for t in _inputs(cuda_device, s)] for s in (5, 6)]
+    sets = [_inputs(cuda_device, s, n, D, V) for s in (3, 4)]
+    fresh = [[t.detach().clone() for t in _inputs(cuda_device, s, n, D, V)] for s in (5, 6)]
     want = []
     for f in fresh:
         leaves = [t.clone().requires_grad_(i < 4) if t.is_floating_point() else t.clone() for i, t in enumerate(f)]

@@ -135,15 +135,12 @@ __global__ void __launch_bounds__(256) norm_grad_cols_loop_kernel(const NormGrad
 }
 
 // ---------------------------------------------------------------------------
-// Rows of up to 16 values per thread of a 512-thread block: the row stays in registers.
+// Rows in registers.  A group of `warps` warps owns a row; every thread holds the same NV pieces of columns in every row,
+// and one exchange between the group's warps joins their sums.
 //
-// A group of `warps` warps owns a row, every thread the same NV pieces of columns in every row, so the parameters are
-// read once per block and the column sums of the backward pass stay in registers until the end.  A group takes U rows
-// at a time: U rows' loads are in flight together and one exchange between the group's warps serves all of them.
-//
-// Forward statistics: each warp computes the mean of its own columns and the sum of squared deviations from that mean,
-// and the warps' results are merged with  M2 = sum M2_w + n_w (mean_w - mean)^2,  which loses nothing when the mean is
-// large against the deviation and needs one exchange, not two.
+// Forward statistics (here and below): each warp computes the mean of its own columns and the sum of squared deviations
+// from that mean, and the warps' results are merged with  M2 = sum M2_w + n_w (mean_w - mean)^2,  which loses nothing
+// when the mean is large against the deviation and needs one exchange, not two.
 // ---------------------------------------------------------------------------
 constexpr int MAX_WARPS = MAX_ROW_WARPS;
 
@@ -172,8 +169,8 @@ __device__ __forceinline__ void load_param_piece(const void* p, bool f32, int64_
     }
 }
 
-// Forward.  A row per group and at most 64 values per thread: with 2048 bf16 values a warp has its row to itself and
-// there is no exchange; the parameters come from L1.
+// Forward of few rows, of rows too wide for the ring below, and of narrow rows at odd addresses.  A row per group and at
+// most 64 values per thread; the parameters come from L1.
 template <typename T, bool WIDE, int NV, bool MULTI, bool PACK>
 __global__ void __launch_bounds__(512, 2) norm_kernel(const NormParams p, int warps) {
     using P = Piece<T, WIDE>;
@@ -281,111 +278,87 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(const NormParams p, int wa
     }
 }
 
-// KEPT: x comes in its 8-bit form
-template <typename T, bool WIDE, int NV, int U, bool MULTI, bool KEPT>
-__global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, int warps, int ru) {
+// Backward of few rows and of narrow rows at odd addresses: at most 16 values per thread, so the column sums stay in
+// registers until the end.  KEPT: x comes in its 8-bit form.
+template <typename T, bool WIDE, int NV, bool MULTI, bool KEPT>
+__global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, int warps) {
     using P = Piece<T, WIDE>;
     using X = typename std::conditional<KEPT, typename P::Packed, typename P::Raw>::type;
     constexpr int N = P::N, E = NV * N;
-    __shared__ float part[MULTI ? 2 * MAX_WARPS * U * 2 : 1];
+    __shared__ float2 part[MULTI ? 2 * MAX_WARPS : 1];
     extern __shared__ float columns[];                     // [2][threads * E] when the block has several groups
     const int lane = threadIdx.x & 31, threads = warps * 32;
     const int group = MULTI ? threadIdx.x / threads : threadIdx.x >> 5;
     const int gt = threadIdx.x - group * threads, gw = gt >> 5;
     const int groups = blockDim.x / threads;
-    const int64_t pieces = p.D / N;
+    const int pieces = static_cast<int>(p.D / N);
     float w[E], aw[E], ab[E];
     load_params<T, NV, N>(p.w, p.param_f32, p.D, gt, threads, 1.f, w);
 #pragma unroll
     for (int q = 0; q < E; ++q) aw[q] = ab[q] = 0.f;
     const float inv_d = 1.f / static_cast<float>(p.D);
     int parity = 0;
-    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * groups + group) * ru; r0 < p.rows;
-         r0 += static_cast<int64_t>(gridDim.x) * groups * ru) {
-        X x[U][NV];
-        typename P::Raw dy[U][NV];
-        float mean[U], rstd[U], sc[U];
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * groups + group; r < p.rows; r += static_cast<int64_t>(gridDim.x) * groups) {
+        X x[NV];
+        typename P::Raw dy[NV];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t r = r0 + u;
-            const bool row_in = u < ru && r < p.rows;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int64_t c = gt + static_cast<int64_t>(i) * threads;
-                const bool in = row_in && c < pieces;
-                dy[u][i] = in ? P::load(static_cast<const T*>(p.dy) + r * p.dy_stride + c * N) : P::zero();
-                if constexpr (KEPT) x[u][i] = in ? P::load_packed(p.payload + r * p.D + c * N) : X{};
-                else x[u][i] = in ? P::load(static_cast<const T*>(p.x) + r * p.x_stride + c * N) : P::zero();
-            }
-            mean[u] = row_in ? __ldg(p.mean + r) : 0.f;
-            rstd[u] = row_in ? __ldg(p.rstd + r) : 0.f;
-            sc[u] = KEPT && row_in ? __ldg(p.scale + r) : 1.f;
+        for (int i = 0; i < NV; ++i) {
+            const int c = gt + i * threads;
+            const bool in = c < pieces;
+            dy[i] = in ? P::load(static_cast<const T*>(p.dy) + r * p.dy_stride + c * N) : P::zero();
+            if constexpr (KEPT) x[i] = in ? P::load_packed(p.payload + r * p.D + c * N) : X{};
+            else x[i] = in ? P::load(static_cast<const T*>(p.x) + r * p.x_stride + c * N) : P::zero();
         }
-        float s[2 * U];
+        const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r), sc = KEPT ? __ldg(p.scale + r) : 1.f;
+        float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[2 * u] = s[2 * u + 1] = 0.f;
+        for (int i = 0; i < NV; ++i) {
+            float f[N], d[N];
+            if constexpr (KEPT) unpack_piece<T, WIDE>(x[i], sc, f); else P::decode(x[i], f);
+            P::decode(dy[i], d);                            // zero where there is no column
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float f[N], d[N];
-                if constexpr (KEPT) unpack_piece<T, WIDE>(x[u][i], sc[u], f); else P::decode(x[u][i], f);
-                P::decode(dy[u][i], d);                     // zero where there is no column or no row
-#pragma unroll
-                for (int q = 0; q < N; ++q) {
-                    const float n = (f[q] - mean[u]) * rstd[u], g = d[q] * w[i * N + q];
-                    s[2 * u] += g;
-                    s[2 * u + 1] = fmaf(g, n, s[2 * u + 1]);
-                    aw[i * N + q] = fmaf(d[q], n, aw[i * N + q]);
-                    ab[i * N + q] += d[q];
-                }
+            for (int q = 0; q < N; ++q) {
+                const float n = (f[q] - mean) * rstd, g = d[q] * w[i * N + q];
+                s[0] += g;
+                s[1] = fmaf(g, n, s[1]);
+                aw[i * N + q] = fmaf(d[q], n, aw[i * N + q]);
+                ab[i * N + q] += d[q];
             }
         }
         if (!p.dx) continue;
-        const float total = warp_sums<2 * U>(s);
-        float m1[U], m2[U];
+        const float total = warp_sums<2>(s);                // lane 0: the first sum, lane 16: the second
+        float m1 = 0.f, m2 = 0.f;
         if constexpr (!MULTI) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                m1[u] = __shfl_sync(FULL_MASK, total, 2 * u * (16 / U)) * inv_d;
-                m2[u] = __shfl_sync(FULL_MASK, total, (2 * u + 1) * (16 / U)) * inv_d;
-            }
+            m1 = __shfl_sync(FULL_MASK, total, 0);
+            m2 = __shfl_sync(FULL_MASK, total, 16);
         } else {
-            float* slot = part + (parity * MAX_WARPS + group * warps) * U * 2;
-            if (lane % (16 / U) == 0) slot[gw * 2 * U + lane / (16 / U)] = total;
+            float2* slot = part + parity * MAX_WARPS + group * warps;
+            if ((lane & 15) == 0) reinterpret_cast<float*>(slot + gw)[lane >> 4] = total;
             group_sync(group, threads);
-#pragma unroll
-            for (int u = 0; u < U; ++u) m1[u] = m2[u] = 0.f;
-            for (int k = 0; k < warps; ++k)
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float2 v = *reinterpret_cast<const float2*>(slot + (k * U + u) * 2);
-                    m1[u] += v.x;
-                    m2[u] += v.y;
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u) { m1[u] *= inv_d; m2[u] *= inv_d; }
-            parity ^= 1;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t r = r0 + u;
-            if (u >= ru || r >= p.rows) break;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int64_t c = gt + static_cast<int64_t>(i) * threads;
-                if (c >= pieces) break;
-                float f[N], d[N], a[N];
-                if constexpr (KEPT) unpack_piece<T, WIDE>(x[u][i], sc[u], f); else P::decode(x[u][i], f);
-                P::decode(dy[u][i], d);
-                if (p.add) P::decode(P::load(static_cast<const T*>(p.add) + r * p.D + c * N), a);
-#pragma unroll
-                for (int q = 0; q < N; ++q) {
-                    const float n = (f[q] - mean[u]) * rstd[u];
-                    f[q] = rstd[u] * (d[q] * w[i * N + q] - m1[u] - n * m2[u]);
-                    if (p.add) f[q] += a[q];
-                }
-                P::store(static_cast<T*>(p.dx) + r * p.D + c * N, P::encode(f));
+            for (int k = 0; k < warps; ++k) {
+                const float2 v = slot[k];
+                m1 += v.x;
+                m2 += v.y;
             }
+            parity ^= 1;                                    // the next row's exchange leaves these slots alone
+        }
+        m1 *= inv_d;
+        m2 *= inv_d;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = gt + i * threads;
+            if (c >= pieces) break;
+            float f[N], d[N], a[N];
+            if constexpr (KEPT) unpack_piece<T, WIDE>(x[i], sc, f); else P::decode(x[i], f);
+            P::decode(dy[i], d);
+            if (p.add) P::decode(P::load(static_cast<const T*>(p.add) + r * p.D + c * N), a);
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const float n = (f[q] - mean) * rstd;
+                f[q] = rstd * (d[q] * w[i * N + q] - m1 - n * m2);
+                if (p.add) f[q] += a[q];
+            }
+            P::store(static_cast<T*>(p.dx) + r * p.D + c * N, P::encode(f));
         }
     }
     if (!p.dw && !p.db) return;
@@ -1223,19 +1196,14 @@ cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
         if (wide) return norm_ring_launch<T, PACK>(p, s);
         if (p.D > SHIFT_DIM) return norm_shift_launch<T, PACK>(p, s);
     }
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8, 1) : narrow_shape(p.rows, p.D, 8);
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8) : narrow_shape(p.rows, p.D, 8);      // wide: nv is 1 or 8 here
     if (h.warps == 0) {
         norm_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         return cudaGetLastError();
     }
     if (!wide) return h.nv == 4 ? norm_launch<T, false, 4, PACK>(p, h, s)
                     : h.nv == 8 ? norm_launch<T, false, 8, PACK>(p, h, s) : norm_launch<T, false, 16, PACK>(p, h, s);
-    switch (h.nv) {
-        case 1: return norm_launch<T, true, 1, PACK>(p, h, s);
-        case 2: return norm_launch<T, true, 2, PACK>(p, h, s);
-        case 4: return norm_launch<T, true, 4, PACK>(p, h, s);
-        default: return norm_launch<T, true, 8, PACK>(p, h, s);
-    }
+    return h.nv == 1 ? norm_launch<T, true, 1, PACK>(p, h, s) : norm_launch<T, true, 8, PACK>(p, h, s);
 }
 
 template <typename T>
@@ -1243,13 +1211,12 @@ cudaError_t norm_t(const NormParams& p, cudaStream_t s) {
     return p.payload ? norm_pack_t<T, true>(p, s) : norm_pack_t<T, false>(p, s);
 }
 
-template <typename T, bool WIDE, int NV, int U, bool KEPT>
+template <typename T, bool WIDE, int NV, bool KEPT>
 cudaError_t norm_grad_launch(const NormGradParams& p, const RowShape& h, cudaStream_t s) {
-    const unsigned threads = h.warps * h.groups * 32;
+    const unsigned threads = h.warps * h.groups * 32, grid = static_cast<unsigned>(p.splits);
     const size_t smem = h.groups > 1 ? sizeof(float) * 2 * h.warps * 32 * NV * Piece<T, WIDE>::N : 0;
-    const unsigned grid = static_cast<unsigned>(p.splits);
-    if (h.warps > 1) norm_grad_kernel<T, WIDE, NV, U, true, KEPT><<<grid, threads, smem, s>>>(p, h.warps, h.u_rows);
-    else norm_grad_kernel<T, WIDE, NV, U, false, KEPT><<<grid, threads, smem, s>>>(p, h.warps, h.u_rows);
+    if (h.warps > 1) norm_grad_kernel<T, WIDE, NV, true, KEPT><<<grid, threads, smem, s>>>(p, h.warps);
+    else norm_grad_kernel<T, WIDE, NV, false, KEPT><<<grid, threads, smem, s>>>(p, h.warps);
     return cudaGetLastError();
 }
 
@@ -1300,7 +1267,7 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     bool wide = p.D % N == 0 && p.dy_stride % N == 0 && aligned16(p.dy) && (!p.dx || aligned16(p.dx)) && (!p.add || aligned16(p.add)) &&
                 (!p.w || aligned16(p.w));
     wide = wide && (KEPT ? (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0 : p.x_stride % N == 0 && aligned16(p.x));
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16, 1) : narrow_shape(p.rows, p.D, 16);
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16) : narrow_shape(p.rows, p.D, 16);      // wide: nv is 1 or 16 / N
     const bool sums = p.dw || p.db;
     if (p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS && (wide || (!p.add && p.D > SHIFT_DIM && p.rows >= SHIFT_GRAD_ROWS))) {
         const cudaError_t e = wide ? norm_grad_ring_launch<T, KEPT>(p, s) : norm_grad_shift_launch<T, KEPT>(p, s);
@@ -1310,14 +1277,12 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
         if (p.dx) norm_grad_rows_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         if (sums) norm_grad_cols_loop_kernel<T><<<dim3(static_cast<unsigned>((p.D + 31) / 32), static_cast<unsigned>(p.splits)), 256, 0, s>>>(p);
     } else {
-        const int64_t need = (p.rows + static_cast<int64_t>(h.groups) * h.u_rows - 1) / (static_cast<int64_t>(h.groups) * h.u_rows);
+        const int64_t need = (p.rows + h.groups - 1) / h.groups;
         p.splits = static_cast<int>(need < MAX_SPLITS ? need : MAX_SPLITS);
         cudaError_t e;
-        if (!wide) e = h.nv == 4 ? norm_grad_launch<T, false, 4, 1, KEPT>(p, h, s)
-                     : h.nv == 8 ? norm_grad_launch<T, false, 8, 1, KEPT>(p, h, s) : norm_grad_launch<T, false, 16, 1, KEPT>(p, h, s);
-        else if (h.nv == 1) e = norm_grad_launch<T, true, 1, 2, KEPT>(p, h, s);
-        else if (h.nv == 16 / N) e = norm_grad_launch<T, true, 16 / N, 1, KEPT>(p, h, s);
-        else e = norm_grad_launch<T, true, 2, 1, KEPT>(p, h, s);
+        if (!wide) e = h.nv == 4 ? norm_grad_launch<T, false, 4, KEPT>(p, h, s)
+                     : h.nv == 8 ? norm_grad_launch<T, false, 8, KEPT>(p, h, s) : norm_grad_launch<T, false, 16, KEPT>(p, h, s);
+        else e = h.nv == 1 ? norm_grad_launch<T, true, 1, KEPT>(p, h, s) : norm_grad_launch<T, true, 16 / N, KEPT>(p, h, s);
         if (e != cudaSuccess) return e;
     }
     if (sums) return launch_behind(norm_grad_join_kernel<T>, dim3(static_cast<unsigned>((p.D + 31) / 32)), dim3(32 * JOIN_LANES), s, p);

@@ -344,11 +344,11 @@ inline cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 bloc
 
 // ---------------------------------------------------------------------------
 // How a row is spread over threads: `warps` warps per row, `groups` rows' worth of warps per block, nv pieces per
-// thread, u_rows rows at a time per group.  warps == 0: the row is longer than MAX_ROW_WARPS warps take.
+// thread.  warps == 0: the row is longer than MAX_ROW_WARPS warps take.
 // ---------------------------------------------------------------------------
 constexpr int MAX_ROW_WARPS = 16;
 constexpr int GRID_SMS = 148;
-struct RowShape { int warps, groups, nv, u_rows; };
+struct RowShape { int warps, groups, nv; };
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned_to(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == PEER_DTYPE_F32 ? 3u : 1u)) == 0; }
@@ -356,7 +356,7 @@ inline bool aligned_to(const void* p, int dtype) { return (reinterpret_cast<uint
 // Many rows: up to nv_max pieces per thread (doubling from nv_min until one warp takes the row), so that a row needs
 // few warps and few exchanges between them.  Fewer than 1024 rows (under seven per SM): nv_min, a row is then spread
 // wider and finished sooner.
-inline RowShape row_shape(int64_t rows, int64_t pieces, int nv_min, int nv_max, int block_warps, int u_max) {
+inline RowShape row_shape(int64_t rows, int64_t pieces, int nv_min, int nv_max, int block_warps) {
     RowShape s{};
     s.nv = nv_min;
     if (rows >= 1024 || pieces > 32 * MAX_ROW_WARPS * nv_min)
@@ -365,14 +365,12 @@ inline RowShape row_shape(int64_t rows, int64_t pieces, int nv_min, int nv_max, 
     if (warps > MAX_ROW_WARPS) return s;
     s.warps = static_cast<int>(warps);
     s.groups = block_warps / s.warps < 1 ? 1 : block_warps / s.warps;
-    const int64_t ru = (rows + GRID_SMS * s.groups - 1) / (GRID_SMS * s.groups);      // all u_max only when every SM gets some
-    s.u_rows = static_cast<int>(ru < 1 ? 1 : (ru > u_max ? u_max : ru));
     return s;
 }
 
 // rows that are not whole 16-byte pieces: one value at a time, 8 per thread (16 spill) unless the row is wider
 inline RowShape narrow_shape(int64_t rows, int64_t D, int block_warps) {
-    return row_shape(rows, D, 4, D <= 32 * MAX_ROW_WARPS * 8 ? 8 : 16, block_warps, 1);
+    return row_shape(rows, D, 4, D <= 32 * MAX_ROW_WARPS * 8 ? 8 : 16, block_warps);
 }
 
 }  // namespace peer

@@ -246,7 +246,7 @@ cudaError_t pack_t(const void* xv, int64_t x_stride, int64_t rows, int64_t D, ui
         pack_shift_kernel<T, STAGES><<<static_cast<unsigned>(need < cap ? need : cap), groups * warps * 32, smem, s>>>(x, x_stride, rows, D, payload, scale, warps);
         return cudaGetLastError();
     }
-    const RowShape h = wide ? row_shape(rows, D / N, 1, 8, 8, 1) : narrow_shape(rows, D, 8);
+    const RowShape h = wide ? row_shape(rows, D / N, 1, 8, 8) : narrow_shape(rows, D, 8);
     if (h.warps == 0) {
         const unsigned grid = static_cast<unsigned>(rows < GRID_SMS * 64 ? rows : GRID_SMS * 64);
         pack_rows_loop_kernel<T><<<grid, 256, 0, s>>>(x, x_stride, rows, D, payload, scale);

@@ -10,8 +10,8 @@
 //
 // More ids: three launches per digit.  (1) every tile of keys counts its digits, (2) every digit scans its
 // counts over the tiles, (3) every tile scatters its keys; the rank of a key
-// among its tile's equal digits comes from a vote over the warp
-// (match.any) on top of a running count per warp and digit.
+// among its tile's equal digits comes from votes over the warp on top of a
+// running count per warp and digit.
 #include "kernels.h"
 #include "row_ops.cuh"
 

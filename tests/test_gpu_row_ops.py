@@ -349,8 +349,15 @@ def test_layer_norm_refusals(cuda_device):
     with pytest.raises(ValueError, match="dim"):
         lib.layer_norm(torch.zeros(1, (1 << 20) + 1, device=cuda_device))
     y = lib.layer_norm(x.requires_grad_())
-    with pytest.raises(RuntimeError):
-        g, = torch.autograd.grad(y.sum(), (x,), create_graph=True)
+    g, = torch.autograd.grad(y.sum(), (x,), create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    g, = torch.autograd.grad(lib.layer_norm(x.detach(), w.requires_grad_(), w).sum(), (w,), create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    table = torch.randn(5, 4, device=cuda_device, requires_grad=True)
+    g, = torch.autograd.grad(lib.embedding(torch.tensor([1, 2], device=cuda_device), table).sum(), (table,), create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
         g.sum().backward()
 
 

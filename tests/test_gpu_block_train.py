@@ -134,7 +134,8 @@ def test_layer_keeps_its_input_in_8_bits(cuda_device):
 @pytest.mark.parametrize("dtype,D,Dout,H,k,N,T,act", [
     (torch.float32, 32, 48, 2, 4, 64, 7, "gelu"), (torch.float32, 256, 256, 4, 8, 300, 65, "relu"),
     (torch.float32, 1024, 512, 2, 4, 128, 1, "gelu"), (torch.bfloat16, 2048, 2048, 8, 16, 4096, 40, "gelu"),
-    (torch.bfloat16, 512, 1024, 4, 8, 50, 129, "relu"), (torch.bfloat16, 64, 64, 8, 16, 3000, 700, "gelu")])
+    (torch.bfloat16, 512, 1024, 4, 8, 50, 129, "relu"), (torch.bfloat16, 64, 64, 8, 16, 3000, 700, "gelu"),
+    (torch.bfloat16, 136, 72, 3, 15, 200, 33, "gelu"), (torch.float32, 512, 512, 5, 13, 90, 600, "relu")])
 def test_sorted_table_gradients(cuda_device, dtype, D, Dout, H, k, N, T, act):
     """Against the form that adds in fp32 tables (itself checked against autograd), up to 90,000 selections."""
     g = torch.Generator().manual_seed(D + T)
@@ -200,6 +201,42 @@ def test_sorted_table_gradients_skip_and_refuse(cuda_device):
         wop.gather_eval_backward_sorted(z, z, torch.zeros(9, 8, dtype=torch.int32, device=dev), torch.zeros(9, 8, device=dev), t, t)
 
 
+def test_block_train_in_slices_and_with_frozen_parts(cuda_device):
+    """Longer than the handle's scratch: the same gradients; and with nothing below the layer to train."""
+    m, ln, hidden, dy = _bf16_case(cuda_device, (2, 700))
+    y0, g0, names = _grads(m, ln, hidden, dy)
+    n, _, _, _ = _bf16_case(cuda_device, (2, 700))
+    n.max_slice_tokens = 512
+    y1, g1, _ = _grads(n, ln, hidden, dy)
+    assert torch.equal(y0, y1) and torch.equal(m._last_expert_indices, n._last_expert_indices)
+    for name, a, b in zip(names, g0, g1):
+        assert torch.equal(a, b), name
+    for p in ln.parameters():
+        p.requires_grad_(False)
+    y = m.block_train(hidden, ln)                             # hidden itself without a gradient
+    up, = torch.autograd.grad(y, (m.expert_up.weight,), dy)
+    assert torch.equal(up, g0[names.index("expert_up.weight")])
+    for p in m.parameters():
+        p.requires_grad_(False)
+    y = m.block_train(hidden, ln)                             # nothing to train: the inference path
+    assert not y.requires_grad and torch.equal(y, y0)
+    h = hidden.clone().requires_grad_()
+    dh, = torch.autograd.grad(m.block_train(h, ln), (h,), dy)
+    assert torch.equal(dh, g0[0])
+
+
+def test_block_train_with_a_norm_in_the_layers_type(cuda_device):
+    m, ln, hidden, dy = _bf16_case(cuda_device)
+    with torch.no_grad():
+        for p in ln.parameters():
+            p.copy_(p.bfloat16())
+    y0, g0, names = _grads(m, ln, hidden, dy)
+    y1, g1, _ = _grads(m, ln.bfloat16(), hidden, dy)          # the same values, stored in bf16
+    assert torch.equal(y0, y1)
+    for name, a, b in zip(names, g0, g1):
+        assert torch.equal(a.bfloat16(), b), name
+
+
 def test_block_train_refusals(cuda_device):
     m = PEER(64, 64, 256, num_experts_per_tok=4, num_heads=2, query_dim=32, product_key_dim=[16, 16]).to(cuda_device)
     x = torch.randn(1, 4, 64, device=cuda_device)
@@ -221,6 +258,10 @@ def test_block_train_refusals(cuda_device):
     n = PEER(64, 32, 256, num_experts_per_tok=4, num_heads=2, query_dim=32, product_key_dim=[16, 16]).to(cuda_device)
     with pytest.raises(ValueError, match="adds its input back"):
         n.block_train(x, torch.nn.LayerNorm(64).to(cuda_device))
+    f = PEER(64, 64, 256, num_experts_per_tok=4, num_heads=2, query_dim=32, product_key_dim=[16, 16]).to(cuda_device).bfloat16()
+    f.quantize_tables_e4m3()
+    with pytest.raises(RuntimeError, match="inference-only"):
+        f.block_train(x.bfloat16(), torch.nn.LayerNorm(64).to(cuda_device))
     n.table_grad_sums = "other"
     with pytest.raises(ValueError, match="sorted"):
         n(x).sum().backward()

@@ -11,6 +11,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import llm720_b200 as lib
 
@@ -314,6 +315,54 @@ def test_layer_norm_against_differences(cuda_device):
         assert abs(slope - want) <= 2e-2 + 1e-2 * (grads[i].norm() * v.norm()).item(), i
 
 
+def test_layer_norm_of_the_widest_row(cuda_device):
+    D = 1 << 20
+    for dtype, ck in ((torch.bfloat16, None), (torch.float32, "e4m3")):
+        x = stream_rows(2, D, dtype, 12, cuda_device).requires_grad_()
+        w, b = params(D, torch.float32, 12, cuda_device)
+        w.requires_grad_()
+        dy = torch.randn(2, D, device=cuda_device).to(dtype)
+        y = lib.layer_norm(x, w, b, checkpoint=ck)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        ref, err = norm_reference(x.detach(), w.detach(), b, 1e-5, dy, unpacked_reference(x.detach(), dtype) if ck else None)
+        for name, got, r, e in (("y", y.detach(), ref[0], err[0]), ("dx", dx, ref[1], err[1]), ("dw", dw, ref[2], err[2])):
+            close(got, r, e, name)
+        payload, scale = lib.pack_rows_e4m3(x)
+        value, ref_scale = packed_reference(x.detach())
+        assert torch.equal(payload.double() * scale.double().unsqueeze(-1), value) and torch.equal(scale.double(), ref_scale)
+
+
+def test_layer_norm_in_inference_mode_and_recomputed(cuda_device):
+    """Under torch.inference_mode, and inside torch's own recomputation of activations."""
+    x = torch.randn(1200, 264, device=cuda_device, requires_grad=True)
+    w, b = (t.requires_grad_() for t in params(264, torch.float32, 1, cuda_device))
+    y = lib.layer_norm(x, w, b)
+    with torch.inference_mode():
+        assert torch.equal(lib.layer_norm(x, w, b), y)
+        payload, scale = lib.pack_rows_e4m3(x)
+        lib.unpack_rows_e4m3(payload, scale, torch.float32)
+    dy = torch.randn_like(y)
+    want = torch.autograd.grad(y, (x, w, b), dy)
+    again = torch.utils.checkpoint.checkpoint(lib.layer_norm, x, w, b, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(again, (x, w, b), dy), want))
+    # part of the gradients only, and the rest later
+    y = lib.layer_norm(x, w, b)
+    part = torch.autograd.grad(y, (b,), dy, retain_graph=True) + torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(p, q) for p, q in zip(part, (want[2], want[0], want[1])))
+
+
+def test_an_input_changed_in_place_is_noticed(cuda_device):
+    x = torch.randn(8, 16, device=cuda_device)
+    w = torch.ones(16, device=cuda_device, requires_grad=True)
+    y = lib.layer_norm(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = lib.layer_norm(x, w, checkpoint="e4m3")               # keeps its own copy of x
+    x.add_(1)
+    y.sum().backward()
+
+
 def test_layer_norm_of_nothing(cuda_device):
     for shape in ((0, 64), (3, 0, 64)):
         x = torch.randn(shape, device=cuda_device, requires_grad=True)
@@ -456,6 +505,8 @@ def ids_of(kind, n, V, device, seed=0):
         return (torch.exp(u * math.log(V)) - 1).long().clamp(0, V - 1)
     if kind == "descending":
         return (V - 1 - torch.arange(n, device=device) % V)
+    if kind == "none":
+        return torch.full((n,), -1, device=device)
     ids = torch.randint(-3, V + 3, (n,), generator=g, device=device)               # "outside": some ids beyond the table
     ids[::3] = -1
     return ids
@@ -477,7 +528,7 @@ def embedding_reference(ids, weight, scale, dy, padding_idx):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("kind", ["uniform", "one", "zipf", "descending", "outside"])
+@pytest.mark.parametrize("kind", ["uniform", "one", "zipf", "descending", "outside", "none"])
 @pytest.mark.parametrize("n,V,D", [(1, 1, 1), (1, 5, 8), (7, 3, 33), (16, 16, 64), (17, 100, 7), (1000, 2, 40), (333, 5000, 136),
                                    (2049, 257, 24), (5000, 70000, 16), (12001, 500, 12),
                                    (20000, 33, 264), (33000, 300, 48), (70001, 1000, 8), (66000, 70000, 4)])

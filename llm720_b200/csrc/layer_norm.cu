@@ -401,15 +401,16 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
 }
 
 // ---------------------------------------------------------------------------
-// ---------------------------------------------------------------------------
 // Many rows of whole 16-byte pieces.  A group of warps owns a row, 16 columns per thread, the same columns in every row,
 // so parameters and column sums stay in registers.  Every thread copies its own pieces of the group's next rows into
 // shared memory (cp.async) while it works on the current one; nobody else reads them, so the ring needs no barrier and
 // no registers, and what is left in a row's chain is one exchange between the group's warps.
 // With the loads covered the instruction count decides: values are decoded once, kept as fp32 pairs across the exchange
-// and go through the packed fp32 instructions, two columns each.  W > 0: the row is exactly W full warps (512 W
-// columns), which turns the addresses of a thread's pieces and the exchange into constants; W == 0 takes any other
-// width.
+// and go through the packed fp32 instructions, two columns each.  The forward pass takes two rows at a time of the 16-bit
+// types, whose exchanges cover one another; the backward pass has no registers for two.  16384 x 2048 bf16: forward 24.8 us
+// (5.4 TB/s), dx 34.8 us (5.8 TB/s), all gradients 39.0 us; 4096 x 8192: 26.6, 37.0 and 45.2 us.
+// W > 0: the row is exactly W full warps (512 W columns), which turns the addresses of a thread's pieces and the exchange
+// into constants; W == 0 takes any other width.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float2 splat(float a) { return make_float2(a, a); }
 // 1/sqrt(v): the hardware estimate and one Newton step (relative error below 2^-23); 0, infinite and NaN pass through
@@ -432,14 +433,25 @@ __device__ __forceinline__ void load_param_pairs(const void* p, bool f32, const 
     }
 }
 
-template <typename T, int W, bool PACK, int STAGES>
+// Exchange of a group that takes two rows at a time: every warp leaves its part of both rows in 32 slots, and after the
+// group's barrier lane 16 u + k of every warp picks up warp k's part of row u, so a few shuffles over half a warp replace
+// 2 x warps reads by every thread.
+template <int K>
+__device__ __forceinline__ void half_warp_sums(float (&v)[K]) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < K; ++i) v[i] += __shfl_xor_sync(FULL_MASK, v[i], o);
+}
+
+template <typename T, int W, int U, bool PACK, int STAGES>
 __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormParams p, int row_warps) {
     using P = Piece<T, true>;
     constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2;
-    constexpr int STAGE = NV * RING_THREADS * 16;           // bytes: [piece][thread]
+    constexpr int ROW = NV * RING_THREADS * 16, STAGE = U * ROW;      // bytes: [row][piece][thread]
     extern __shared__ __align__(16) unsigned char ring_smem[];
-    __shared__ float2 part[2 * MAX_WARPS];
-    __shared__ uint32_t part_top[2 * MAX_WARPS];
+    __shared__ float2 part[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];      // U == 2: [parity][group][row][warp]
+    __shared__ uint32_t part_top[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];
     __shared__ float held[MAX_WARPS];                       // columns of each of the group's warps
     const int warps = W ? W : row_warps;
     const int lane = threadIdx.x & 31, threads = warps * 32;
@@ -463,13 +475,16 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
     const uint32_t slot0 = smem_u32(ring_smem) + threadIdx.x * 16, slot_end = slot0 + STAGES * STAGE;
     uint32_t slot = slot0, fetch_slot = slot0;
     auto fetch = [&]() {
-        if (to_fetch > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (in[i]) copy_async<16>(fetch_slot + i * RING_THREADS * 16, src + i * threads * N);
+        for (int u = 0; u < U; ++u) {
+            if (to_fetch > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (in[i]) copy_async<16>(fetch_slot + u * ROW + i * RING_THREADS * 16, src + i * threads * N);
+            }
+            src += src_step;
+            --to_fetch;
         }
-        src += src_step;
-        --to_fetch;
         fetch_slot += STAGE;
         if (fetch_slot == slot_end) fetch_slot = slot0;
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -485,84 +500,136 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
     uint8_t* dst8 = p.payload + first * p.D + gt * N;
     const int64_t dst_step = step * p.D;
     int64_t r = first;
-    int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
-    for (; rows > 0; --rows) {
+    // this row's slots; the next row's leave them alone
+    int exchange = U == 2 ? group * 32 : group * warps, other = U == 2 ? 8 * 32 : MAX_WARPS;
+    for (; rows > 0; rows -= U) {
         fetch();
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        typename P::Raw raw[NV];
-        float2 x[NV][H], s2 = splat(0.f);
+        typename P::Raw raw[U][NV];
+        float2 x[U][NV][H];
+        float mean[U], m2[U];
+        uint32_t top[U];
+        bool odd[U];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            raw[i] = in[i] ? shared_at<uint4>(slot + i * RING_THREADS * 16) : P::zero();
-            float f[N];
-            P::decode(raw[i], f);
+        for (int u = 0; u < U; ++u) {
+            float2 s2 = splat(0.f);
 #pragma unroll
-            for (int h = 0; h < H; ++h) { x[i][h] = make_float2(f[2 * h], f[2 * h + 1]); s2 = __fadd2_rn(s2, x[i][h]); }
+            for (int i = 0; i < NV; ++i) {
+                raw[u][i] = in[i] && u < rows ? shared_at<uint4>(slot + u * ROW + i * RING_THREADS * 16) : P::zero();
+                float f[N];
+                P::decode(raw[u][i], f);
+#pragma unroll
+                for (int h = 0; h < H; ++h) { x[u][i][h] = make_float2(f[2 * h], f[2 * h + 1]); s2 = __fadd2_rn(s2, x[u][i][h]); }
+            }
+            mean[u] = s2.x + s2.y;
+            odd[u] = false;
+            top[u] = 0u;
+            if (PACK) top[u] = warp_top<T, true, NV>(raw[u], odd[u]);
         }
         slot += STAGE;
         if (slot == slot_end) slot = slot0;
-        bool odd = false;
-        uint32_t top = 0u;
-        if (PACK) top = warp_top<T, true, NV>(raw, odd);
-        float mean = warp_sum(s2.x + s2.y) * inv_mine;
-        const float2 neg = splat(-mean);
-        s2 = splat(0.f);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (in[i]) {
+        for (int u = 0; u < U; ++u) mean[u] = warp_sum(mean[u]) * inv_mine;
 #pragma unroll
-                for (int h = 0; h < H; ++h) { const float2 d = __fadd2_rn(x[i][h], neg); s2 = __ffma2_rn(d, d, s2); }
-            }
-        float m2 = warp_sum(s2.x + s2.y);
-        if (warps > 1) {
+        for (int u = 0; u < U; ++u) {
+            const float2 neg = splat(-mean[u]);
+            float2 s2 = splat(0.f);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (in[i]) {
+#pragma unroll
+                    for (int h = 0; h < H; ++h) { const float2 d = __fadd2_rn(x[u][i][h], neg); s2 = __ffma2_rn(d, d, s2); }
+                }
+            m2[u] = s2.x + s2.y;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) m2[u] = warp_sum(m2[u]);
+        if (warps == 1) {
+        } else if constexpr (U == 2) {
             if (lane == 0) {
-                part[exchange + gw] = make_float2(mean, m2);
-                if (PACK) part_top[exchange + gw] = top;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    part[exchange + u * 16 + gw] = make_float2(mean[u], m2[u]);
+                    if (PACK) part_top[exchange + u * 16 + gw] = top[u];
+                }
             }
             group_sync(group, threads);
-            mean = 0.f;
+            const bool has = (lane & 15) < warps;
+            const float2 v = has ? part[exchange + lane] : splat(0.f);
+            const float n = has ? (W ? 32.f * RING_COLUMNS : held[lane & 15]) : 0.f;
+            float m[1] = {n * v.x};
+            half_warp_sums<1>(m);
+            m[0] *= inv_d;
+            const float d = v.x - m[0];
+            float q[1] = {fmaf(n * d, d, v.y)};
+            half_warp_sums<1>(q);
+            uint32_t t = PACK && has ? part_top[exchange + lane] : 0u;
+            if (PACK) {
 #pragma unroll
-            for (int k = 0; k < (W ? W : warps); ++k) {
-                mean = fmaf(W ? 1.f : held[k], part[exchange + k].x, mean);
-                if (PACK) top = max(top, part_top[exchange + k]);
+                for (int o = 8; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(FULL_MASK, t, o));
             }
-            mean *= W ? 1.f / (W ? W : 1) : inv_d;
-            m2 = 0.f;
 #pragma unroll
-            for (int k = 0; k < (W ? W : warps); ++k) {
-                const float2 v = part[exchange + k];
-                const float d = v.x - mean;
-                m2 += fmaf((W ? 32.f * RING_COLUMNS : held[k]) * d, d, v.y);
+            for (int u = 0; u < U; ++u) {
+                mean[u] = __shfl_sync(FULL_MASK, m[0], u * 16);
+                m2[u] = __shfl_sync(FULL_MASK, q[0], u * 16);
+                if (PACK) top[u] = __shfl_sync(FULL_MASK, t, u * 16);
             }
             exchange += other;
             other = -other;
-        }
-        const float rstd = inverse_sqrt(m2 * inv_d + p.eps);
-        const float2 r2 = splat(rstd), m2p = splat(-mean);
-        const int e = PACK ? e4m3_scale_exponent(top) : 0;
-        const float inv = exp2_int(-e);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (in[i]) {
-                float f[N];
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const float2 v = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[i][h], m2p), r2), w[i][h], b[i][h]);
-                    f[2 * h] = v.x;
-                    f[2 * h + 1] = v.y;
-                }
-                P::store(dst + i * threads * N, P::encode(f));
-                if constexpr (PACK)
-                    *reinterpret_cast<typename P::Packed*>(dst8 + i * threads * N) = pack_pairs<T>(x[i], raw[i], inv, odd);
+        } else {
+            if (lane == 0) {
+                part[exchange + gw] = make_float2(mean[0], m2[0]);
+                if (PACK) part_top[exchange + gw] = top[0];
             }
-        dst += dst_step;
-        if (PACK) dst8 += dst_step;
-        if (gt == 0) {
-            if (p.mean) p.mean[r] = mean;
-            if (p.rstd) p.rstd[r] = rstd;
-            if (PACK) p.scale[r] = exp2_int(e);
+            group_sync(group, threads);
+            float m = 0.f, q = 0.f;
+#pragma unroll
+            for (int k = 0; k < (W ? W : warps); ++k) {
+                m = fmaf(W ? 1.f : held[k], part[exchange + k].x, m);
+                if (PACK) top[0] = max(top[0], part_top[exchange + k]);
+            }
+            m *= W ? 1.f / (W ? W : 1) : inv_d;
+#pragma unroll
+            for (int k = 0; k < (W ? W : warps); ++k) {
+                const float2 v = part[exchange + k];
+                const float d = v.x - m;
+                q += fmaf((W ? 32.f * RING_COLUMNS : held[k]) * d, d, v.y);
+            }
+            mean[0] = m;
+            m2[0] = q;
+            exchange += other;
+            other = -other;
         }
-        r += step;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= rows) break;
+            const float rstd = inverse_sqrt(m2[u] * inv_d + p.eps);
+            const float2 r2 = splat(rstd), minus = splat(-mean[u]);
+            const int e = PACK ? e4m3_scale_exponent(top[u]) : 0;
+            const float inv = exp2_int(-e);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (in[i]) {
+                    float f[N];
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const float2 v = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[u][i][h], minus), r2), w[i][h], b[i][h]);
+                        f[2 * h] = v.x;
+                        f[2 * h + 1] = v.y;
+                    }
+                    P::store(dst + i * threads * N, P::encode(f));
+                    if constexpr (PACK)
+                        *reinterpret_cast<typename P::Packed*>(dst8 + i * threads * N) = pack_pairs<T>(x[u][i], raw[u][i], inv, odd[u]);
+                }
+            dst += dst_step;
+            if (PACK) dst8 += dst_step;
+            if (gt == 0) {
+                if (p.mean) p.mean[r] = mean[u];
+                if (p.rstd) p.rstd[r] = rstd;
+                if (PACK) p.scale[r] = exp2_int(e);
+            }
+            r += step;
+        }
     }
 }
 
@@ -682,11 +749,19 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const N
             } else {
                 if ((lane & 15) == 0) reinterpret_cast<float*>(part + exchange + gw)[lane >> 4] = total;
                 group_sync(group, threads);
+                if (W == 16 || (W == 0 && warps >= 8)) {    // a warp's part per lane, joined by shuffles
+                    const float2 v = (lane & 15) < warps ? part[exchange + (lane & 15)] : splat(0.f);
+                    float both[2] = {v.x, v.y};
+                    half_warp_sums<2>(both);
+                    m1 = both[0];
+                    m2 = both[1];
+                } else {
 #pragma unroll
-                for (int k = 0; k < (W ? W : warps); ++k) {
-                    const float2 v = part[exchange + k];
-                    m1 += v.x;
-                    m2 += v.y;
+                    for (int k = 0; k < (W ? W : warps); ++k) {
+                        const float2 v = part[exchange + k];
+                        m1 += v.x;
+                        m2 += v.y;
+                    }
                 }
                 exchange += other;
                 other = -other;
@@ -761,8 +836,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const N
 // ---------------------------------------------------------------------------
 // The same for rows that are not whole 16-byte pieces at 16-byte addresses (an odd width, an odd stride, a view that
 // begins anywhere), brought and stored as the granules that cover them (row_shift.cuh).  A granule is another thread's,
-// so a row has a barrier behind its arrival and one before its results leave.  16384 x 2001 bf16: forward 56 us, all
-// gradients 67 us, against 172 and 187 us one value at a time.
+// so a row has a barrier behind its arrival and one before its results leave.  16384 x 2001 bf16: forward 46 us, all
+// gradients 64 us, against 172 and 187 us one value at a time.
 // ---------------------------------------------------------------------------
 // parameters of this thread's columns, `absent` beyond the row's end
 template <typename T, int NV, int N>
@@ -780,21 +855,21 @@ __device__ __forceinline__ void load_param_values(const void* p, bool f32, int D
     }
 }
 
-template <typename T, bool PACK, int STAGES>
+template <typename T, int U, bool PACK, int STAGES>
 __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormParams p, int warps) {
     using P = Piece<T, true>;
     constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2, XB = static_cast<int>(sizeof(typename P::Packed));
     extern __shared__ __align__(16) unsigned char ring_smem[];
-    __shared__ float2 part[2 * MAX_WARPS];
-    __shared__ uint32_t part_top[2 * MAX_WARPS];
+    __shared__ float2 part[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];      // U == 2: [parity][group][row][warp]
+    __shared__ uint32_t part_top[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];
     __shared__ float held[MAX_WARPS];                       // columns of each of the group's warps
     const int lane = threadIdx.x & 31, threads = warps * 32;
     const int group = threadIdx.x / threads, gt = threadIdx.x - group * threads, gw = gt >> 5;
     const int groups = blockDim.x / threads, D = static_cast<int>(p.D), bytes = D * static_cast<int>(sizeof(T));
-    // a group's memory: STAGES rows of x, 16 bytes, a row of y, 16 bytes, a row of payload
+    // a group's memory: STAGES times U rows of x, then U times {16 bytes, a row of y}, U times {16 bytes, a row of payload}
     const int room = row_room(threads * RING_COLUMNS, sizeof(T)), room8 = row_room(threads * RING_COLUMNS, 1);
-    const uint32_t slot0 = smem_u32(ring_smem) + group * ((STAGES + 1) * room + room8 + 32), slot_end = slot0 + STAGES * room;
-    const uint32_t out = slot_end + 16, out8 = out + room + 16;
+    const uint32_t slot0 = smem_u32(ring_smem) + group * U * ((STAGES + 1) * room + room8 + 32), slot_end = slot0 + STAGES * U * room;
+    const uint32_t out = slot_end + 16, out8 = slot_end + U * (room + 16) + 16;
     auto sync = [&]() { if (warps > 1) group_sync(group, threads); else __syncwarp(); };
     int valid[NV], mine = 0;
 #pragma unroll
@@ -810,10 +885,13 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
     const int64_t src_step = step * p.x_stride;
     uint32_t slot = slot0, fetch_slot = slot0;
     auto fetch = [&]() {
-        if (to_fetch > 0) fetch_row(fetch_slot, src, bytes, gt, threads);
-        src += src_step;
-        --to_fetch;
-        fetch_slot += room;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (to_fetch > 0) fetch_row(fetch_slot, src, bytes, gt, threads);
+            src += src_step;
+            --to_fetch;
+            fetch_slot += room;
+        }
         if (fetch_slot == slot_end) fetch_slot = slot0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -825,91 +903,148 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
     __syncthreads();
     const float inv_mine = mine > 0 ? 1.f / static_cast<float>(mine) : 0.f, inv_d = 1.f / static_cast<float>(D);
     int64_t r = first;
-    int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
-    for (; rows > 0; --rows) {
+    // this row's slots; the next row's leave them alone
+    int exchange = U == 2 ? group * 32 : group * warps, other = U == 2 ? 8 * 32 : MAX_WARPS;
+    for (; rows > 0; rows -= U) {
         fetch();
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         sync();                                             // the other threads' granules
-        const uint32_t shift = offset16(cur);
-        cur += src_step;
-        typename P::Raw raw[NV];
-        float2 x[NV][H], s2 = splat(0.f);
+        typename P::Raw raw[U][NV];
+        float2 x[U][NV][H];
+        float mean[U], m2[U];
+        uint32_t top[U];
+        bool odd[U];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            raw[i] = valid[i] ? shared_shifted(slot + (gt + i * threads) * 16, shift) : P::zero();      // zeros behind the row
-            float f[N];
-            P::decode(raw[i], f);
+        for (int u = 0; u < U; ++u) {
+            const uint32_t shift = offset16(cur);
+            cur += src_step;
+            float2 s2 = splat(0.f);
 #pragma unroll
-            for (int h = 0; h < H; ++h) { x[i][h] = make_float2(f[2 * h], f[2 * h + 1]); s2 = __fadd2_rn(s2, x[i][h]); }
-        }
-        slot += room;
-        if (slot == slot_end) slot = slot0;
-        bool odd = false;
-        uint32_t top = 0u;
-        if (PACK) top = warp_top<T, true, NV>(raw, odd);
-        float mean = warp_sum(s2.x + s2.y) * inv_mine;
-        const float2 neg = splat(-mean);
-        s2 = splat(0.f);
+            for (int i = 0; i < NV; ++i) {
+                raw[u][i] = valid[i] && u < rows ? shared_shifted(slot + (gt + i * threads) * 16, shift) : P::zero();      // zeros behind the row
+                float f[N];
+                P::decode(raw[u][i], f);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                float2 d = __fadd2_rn(x[i][h], neg);
-                if (valid[i] < N) {                         // the row's last piece, and those behind it
-                    if (2 * h >= valid[i]) d.x = 0.f;
-                    if (2 * h + 1 >= valid[i]) d.y = 0.f;
-                }
-                s2 = __ffma2_rn(d, d, s2);
+                for (int h = 0; h < H; ++h) { x[u][i][h] = make_float2(f[2 * h], f[2 * h + 1]); s2 = __fadd2_rn(s2, x[u][i][h]); }
             }
+            slot += room;
+            mean[u] = s2.x + s2.y;
+            odd[u] = false;
+            top[u] = 0u;
+            if (PACK) top[u] = warp_top<T, true, NV>(raw[u], odd[u]);
         }
-        float m2 = warp_sum(s2.x + s2.y);
-        if (warps > 1) {
+        if (slot == slot_end) slot = slot0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mean[u] = warp_sum(mean[u]) * inv_mine;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float2 neg = splat(-mean[u]);
+            float2 s2 = splat(0.f);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    float2 d = __fadd2_rn(x[u][i][h], neg);
+                    if (valid[i] < N) {                     // the row's last piece, and those behind it
+                        if (2 * h >= valid[i]) d.x = 0.f;
+                        if (2 * h + 1 >= valid[i]) d.y = 0.f;
+                    }
+                    s2 = __ffma2_rn(d, d, s2);
+                }
+            }
+            m2[u] = s2.x + s2.y;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) m2[u] = warp_sum(m2[u]);
+        if (warps == 1) {
+        } else if constexpr (U == 2) {
             if (lane == 0) {
-                part[exchange + gw] = make_float2(mean, m2);
-                if (PACK) part_top[exchange + gw] = top;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    part[exchange + u * 16 + gw] = make_float2(mean[u], m2[u]);
+                    if (PACK) part_top[exchange + u * 16 + gw] = top[u];
+                }
             }
             group_sync(group, threads);
-            mean = 0.f;
-            for (int k = 0; k < warps; ++k) {
-                mean = fmaf(held[k], part[exchange + k].x, mean);
-                if (PACK) top = max(top, part_top[exchange + k]);
+            const bool has = (lane & 15) < warps;
+            const float2 v = has ? part[exchange + lane] : splat(0.f);
+            const float n = has ? held[lane & 15] : 0.f;
+            float m[1] = {n * v.x};
+            half_warp_sums<1>(m);
+            m[0] *= inv_d;
+            const float d = v.x - m[0];
+            float q[1] = {fmaf(n * d, d, v.y)};
+            half_warp_sums<1>(q);
+            uint32_t t = PACK && has ? part_top[exchange + lane] : 0u;
+            if (PACK) {
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(FULL_MASK, t, o));
             }
-            mean *= inv_d;
-            m2 = 0.f;
-            for (int k = 0; k < warps; ++k) {
-                const float2 v = part[exchange + k];
-                const float d = v.x - mean;
-                m2 += fmaf(held[k] * d, d, v.y);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                mean[u] = __shfl_sync(FULL_MASK, m[0], u * 16);
+                m2[u] = __shfl_sync(FULL_MASK, q[0], u * 16);
+                if (PACK) top[u] = __shfl_sync(FULL_MASK, t, u * 16);
             }
             exchange += other;
             other = -other;
-        }
-        const float rstd = inverse_sqrt(m2 * inv_d + p.eps);
-        const float2 r2 = splat(rstd), m2p = splat(-mean);
-        const int e = PACK ? e4m3_scale_exponent(top) : 0;
-        const float inv = exp2_int(-e);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (valid[i]) {
-                float f[N];
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const float2 v = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[i][h], m2p), r2), w[i][h], b[i][h]);
-                    f[2 * h] = v.x;
-                    f[2 * h + 1] = v.y;
-                }
-                store_shared(out + (gt + i * threads) * 16, P::encode(f));
-                if constexpr (PACK) store_shared(out8 + (gt + i * threads) * XB, pack_pairs<T>(x[i], raw[i], inv, odd));
+        } else {
+            if (lane == 0) {
+                part[exchange + gw] = make_float2(mean[0], m2[0]);
+                if (PACK) part_top[exchange + gw] = top[0];
             }
-        sync();
-        store_row<T>(static_cast<T*>(p.y) + r * p.D, out, bytes, gt, threads);
-        if (PACK) store_row<uint8_t>(p.payload + r * p.D, out8, D, gt, threads);
-        if (gt == 0) {
-            if (p.mean) p.mean[r] = mean;
-            if (p.rstd) p.rstd[r] = rstd;
-            if (PACK) p.scale[r] = exp2_int(e);
+            group_sync(group, threads);
+            float m = 0.f, q = 0.f;
+            for (int k = 0; k < warps; ++k) {
+                m = fmaf(held[k], part[exchange + k].x, m);
+                if (PACK) top[0] = max(top[0], part_top[exchange + k]);
+            }
+            m *= inv_d;
+            for (int k = 0; k < warps; ++k) {
+                const float2 v = part[exchange + k];
+                const float d = v.x - m;
+                q += fmaf(held[k] * d, d, v.y);
+            }
+            mean[0] = m;
+            m2[0] = q;
+            exchange += other;
+            other = -other;
         }
-        r += step;
+        float rstd[U];
+        int e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            rstd[u] = inverse_sqrt(m2[u] * inv_d + p.eps);
+            e[u] = PACK ? e4m3_scale_exponent(top[u]) : 0;
+            const float2 r2 = splat(rstd[u]), minus = splat(-mean[u]);
+            const float inv = exp2_int(-e[u]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (valid[i]) {
+                    float f[N];
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const float2 v = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[u][i][h], minus), r2), w[i][h], b[i][h]);
+                        f[2 * h] = v.x;
+                        f[2 * h + 1] = v.y;
+                    }
+                    store_shared(out + u * (room + 16) + (gt + i * threads) * 16, P::encode(f));
+                    if constexpr (PACK) store_shared(out8 + u * (room8 + 16) + (gt + i * threads) * XB, pack_pairs<T>(x[u][i], raw[u][i], inv, odd[u]));
+                }
+        }
+        sync();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= rows) break;
+            store_row<T>(static_cast<T*>(p.y) + r * p.D, out + u * (room + 16), bytes, gt, threads);
+            if (PACK) store_row<uint8_t>(p.payload + r * p.D, out8 + u * (room8 + 16), D, gt, threads);
+            if (gt == 0) {
+                if (p.mean) p.mean[r] = mean[u];
+                if (p.rstd) p.rstd[r] = rstd[u];
+                if (PACK) p.scale[r] = exp2_int(e[u]);
+            }
+            r += step;
+        }
     }
 }
 
@@ -1018,11 +1153,11 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const 
             } else {
                 if ((lane & 15) == 0) reinterpret_cast<float*>(part + exchange + gw)[lane >> 4] = total;
                 group_sync(group, threads);
-                for (int k = 0; k < warps; ++k) {
-                    const float2 v = part[exchange + k];
-                    m1 += v.x;
-                    m2 += v.y;
-                }
+                const float2 v = (lane & 15) < warps ? part[exchange + (lane & 15)] : splat(0.f);
+                float both[2] = {v.x, v.y};                 // a warp's part per lane, joined by shuffles
+                half_warp_sums<2>(both);
+                m1 = both[0];
+                m2 = both[1];
                 exchange += other;
                 other = -other;
             }
@@ -1130,7 +1265,7 @@ unsigned row_blocks(int64_t rows) { return static_cast<unsigned>(rows < 148 * 64
 
 constexpr int64_t RING_ROWS = 1024;   // below, a block sees too few rows for a ring to run ahead
 // rows at any address: a warp's 512 columns are too many for narrower ones (32768 x 129 bf16: 23 us forward, 21 us one
-// value at a time; 16384 x 2001: 56 and 172); the backward pass needs more rows (1500 x 1001 fp32: 14 us, 12 one value
+// value at a time; 16384 x 2001: 46 and 172); the backward pass needs more rows (1500 x 1001 fp32: 14 us, 12 one value
 // at a time; 5003 x 1537 fp16: 27 and 41)
 constexpr int64_t SHIFT_DIM = 256, SHIFT_GRAD_ROWS = 2048;
 
@@ -1143,10 +1278,12 @@ inline int ring_width(int64_t D) {
 
 template <typename T, int W, bool PACK>
 cudaError_t norm_ring_width(const NormParams& p, cudaStream_t s) {
-    constexpr int STAGES = sizeof(T) == 4 ? 4 : 6;           // 128 KB, 96 KB
-    constexpr int SMEM = STAGES * RING_THREADS * RING_COLUMNS * static_cast<int>(sizeof(T));
-    auto* kernel = norm_ring_kernel<T, W, PACK, STAGES>;
+    // rows a group takes at a time: two cover one another's exchange (16384 x 2048 bf16 24.8 us instead of 26.8, x 1536 22.7
+    // instead of 30, 4096 x 8192 26.8 instead of 37); fp32 rows are bound by memory with one
+    constexpr int U = sizeof(T) == 4 ? 1 : 2, ROWS = sizeof(T) == 4 ? 4 : 6;      // rows in the ring: 128 KB, 96 KB
+    constexpr int SMEM = ROWS * RING_THREADS * RING_COLUMNS * static_cast<int>(sizeof(T));
     const int warps = ring_warps(p.D), groups = MAX_WARPS / warps;
+    auto* kernel = norm_ring_kernel<T, W, U, PACK, ROWS / U>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     const int64_t need = (p.rows + groups - 1) / groups;
@@ -1167,10 +1304,10 @@ cudaError_t norm_ring_launch(const NormParams& p, cudaStream_t s) {
 
 template <typename T, bool PACK>
 cudaError_t norm_shift_launch(const NormParams& p, cudaStream_t s) {
-    constexpr int STAGES = sizeof(T) == 4 ? 3 : 5;           // with the results' rows at most 160 KB
-    auto* kernel = norm_shift_kernel<T, PACK, STAGES>;
+    constexpr int U = sizeof(T) == 4 ? 1 : 2, STAGES = sizeof(T) == 4 ? 3 : 2;      // with the results' rows at most 150 KB
+    auto* kernel = norm_shift_kernel<T, U, PACK, STAGES>;
     const int warps = ring_warps(p.D), groups = MAX_WARPS / warps, columns = warps * 32 * RING_COLUMNS;
-    const int smem = groups * ((STAGES + 1) * row_room(columns, sizeof(T)) + row_room(columns, 1) + 32);
+    const int smem = groups * U * ((STAGES + 1) * row_room(columns, sizeof(T)) + row_room(columns, 1) + 32);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const int64_t need = (p.rows + groups - 1) / groups;

@@ -67,10 +67,12 @@ void need_rows(const Tensor& t, const char* name) {
 }
 
 // t [..., D] as [rows, D] with consecutive values in a row: a view wherever one exists (row strides of any size, zero
-// included, are the kernels' business), else a contiguous copy
+// included, are the kernels' business), else a contiguous copy.  A negated view (the imaginary part of a conjugate) has
+// the wrong signs in memory and is resolved first; where a table or parameters are one, the call is refused.
 Tensor as_rows(const Tensor& t) {
     const int64_t D = t.size(-1);
     Tensor rows = t.dim() == 2 ? t : t.reshape({t.numel() / D, D});
+    rows = rows.resolve_neg();
     return D == 1 || rows.stride(1) == 1 ? rows : rows.contiguous();
 }
 
@@ -107,7 +109,7 @@ NormCodes check_norm(const Tensor& x, const Tensor& w, const Tensor& b, double e
         if (p.device() != x.device()) throw std::runtime_error(text(name, " is on ", p.device(), ", x on ", x.device()));
         if (p.scalar_type() != at::kFloat && p.scalar_type() != x.scalar_type())
             throw py::type_error(text(name, " is ", dtype_name(p.scalar_type()), ": parameters are float32 or of x's dtype, ", dtype_name(x.scalar_type())));
-        if (!p.is_contiguous()) throw py::value_error(text(name, " must be contiguous"));
+        if (!p.is_contiguous() || p.is_neg()) throw py::value_error(text(name, " must be contiguous"));
         c.param = code_of(p.scalar_type(), name);
     };
     one(w, "weight");
@@ -231,7 +233,7 @@ Tensor unpack_rows(const Tensor& payload_in, const Tensor& scale_in, at::ScalarT
         throw std::runtime_error(text("scale is on ", scale_in.device(), ", payload on ", payload_in.device()));
     const at::AutoGradMode off(false);
     const c10::cuda::CUDAGuard guard(payload_in.device());
-    const Tensor payload = payload_in.contiguous(), scale = scale_in.contiguous();
+    const Tensor payload = payload_in.contiguous(), scale = scale_in.contiguous().resolve_neg();
     Tensor out = at::empty(payload.sizes(), payload.options().dtype(dtype));
     const int64_t D = payload.size(-1);
     check(peer_unpack_rows(payload.data_ptr(), scale.data_ptr<float>(), code, payload.numel() / D, D, out.data_ptr(), stream_of(payload)));
@@ -286,7 +288,7 @@ Tensor embedding(const Tensor& ids_in, const Tensor& weight, double scale, std::
     code_of(weight.scalar_type(), "weight");
     if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
         throw py::value_error(text("weight must be a [rows, width] table, got ", weight.sizes()));
-    if (!weight.is_contiguous()) throw py::value_error("weight must be contiguous");
+    if (!weight.is_contiguous() || weight.is_neg()) throw py::value_error("weight must be contiguous");
     if (ids_in.scalar_type() != at::kInt && ids_in.scalar_type() != at::kLong)
         throw py::type_error(text("ids is ", dtype_name(ids_in.scalar_type()), ", expected int32 or int64"));
     if (ids_in.device() != weight.device())

@@ -225,6 +225,35 @@ def test_block_train_in_slices_and_with_frozen_parts(cuda_device):
     assert torch.equal(dh, g0[0])
 
 
+@pytest.mark.parametrize("ck", [None, "e4m3"])
+def test_block_train_captured_and_replayed(cuda_device, ck):
+    m, ln, hidden, dy = _bf16_case(cuda_device)
+    m.activation_checkpoint = ck
+    h = hidden.clone().requires_grad_()
+    leaves = [h, ln.weight, ln.bias] + [p for n, p in m.named_parameters() if "sub_keys" not in n]
+
+    def step():
+        y = m.block_train(h, ln)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2):
+        g = torch.Generator(device=cuda_device).manual_seed(seed)
+        with torch.no_grad():
+            h.copy_(torch.randn(h.shape, generator=g, device=cuda_device).to(h.dtype))
+        graph.replay()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
 def test_block_train_with_a_norm_in_the_layers_type(cuda_device):
     m, ln, hidden, dy = _bf16_case(cuda_device)
     with torch.no_grad():

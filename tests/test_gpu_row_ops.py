@@ -363,6 +363,31 @@ def test_an_input_changed_in_place_is_noticed(cuda_device):
     y.sum().backward()
 
 
+def test_negated_views_are_read_with_their_signs(cuda_device):
+    """The imaginary part of a conjugate is a view whose signs are in a flag, not in memory."""
+    for D in (1, 40):
+        z = torch.randn(6, D, dtype=torch.complex64, device=cuda_device)
+        neg = z.conj().imag
+        assert neg.is_neg()
+        plain = -z.imag
+        b = torch.randn(D, device=cuda_device, requires_grad=True)
+        x = torch.randn(6, D, device=cuda_device, requires_grad=True)
+        assert torch.equal(lib.layer_norm(neg, None, b), lib.layer_norm(plain, None, b))
+        for got, want in zip(torch.autograd.grad(lib.layer_norm(x, None, b), (x, b), neg),
+                             torch.autograd.grad(lib.layer_norm(x, None, b), (x, b), plain)):
+            assert torch.equal(got, want)
+        for got, want in zip(lib.pack_rows_e4m3(neg), lib.pack_rows_e4m3(plain)):
+            assert torch.equal(got.float(), want.float())
+        ids = torch.tensor([1, 0, 2, 2, 1, 5], device=cuda_device)
+        grads = [torch.autograd.grad(lib.embedding(ids, x), (x,), dy)[0] for dy in (neg, plain)]
+        assert torch.equal(*grads)
+    one = torch.randn(1, dtype=torch.complex64, device=cuda_device).conj().imag
+    with pytest.raises(ValueError, match="contiguous"):
+        lib.layer_norm(torch.randn(3, 1, device=cuda_device), one)
+    with pytest.raises(ValueError, match="contiguous"):
+        lib.embedding(torch.tensor([0], device=cuda_device), one.view(1, 1))
+
+
 def test_layer_norm_of_nothing(cuda_device):
     for shape in ((0, 64), (3, 0, 64)):
         x = torch.randn(shape, device=cuda_device, requires_grad=True)

@@ -43,9 +43,8 @@ __device__ __forceinline__ void store_shared(uint32_t at, uint32_t v) {
 __device__ __forceinline__ void copy_async_filled(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// 16 bytes at offset `shift` (0 to 15) of the 32 at `at`
-__device__ __forceinline__ uint4 shared_shifted(uint32_t at, uint32_t shift) {
-    const uint4 a = shared_at<uint4>(at), b = shared_at<uint4>(at + 16);
+// 16 bytes at offset `shift` (0 to 15) of two granules
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, uint32_t shift) {
     uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     if (shift & 8u) {
 #pragma unroll
@@ -58,6 +57,10 @@ __device__ __forceinline__ uint4 shared_shifted(uint32_t at, uint32_t shift) {
     const uint32_t bits = (shift & 3u) * 8u;
     return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
                       __funnelshift_r(w[3], w[4], bits));
+}
+// 16 bytes at offset `shift` of the 32 at `at`
+__device__ __forceinline__ uint4 shared_shifted(uint32_t at, uint32_t shift) {
+    return shifted(shared_at<uint4>(at), shared_at<uint4>(at + 16), shift);
 }
 // 8 or 4 bytes at any shared address
 template <typename V> __device__ __forceinline__ V shared_unaligned(uint32_t at);
@@ -100,6 +103,37 @@ __device__ __forceinline__ void store_row(void* row, uint32_t src, int bytes, in
                 if (at >= 0 && at < bytes) *reinterpret_cast<U*>(static_cast<char*>(row) + at) = e[q];
             }
         }
+    }
+}
+
+// The same without shared memory, for a thread that takes 16 / sizeof(T) values of a row of D from value `at` on, where `at`
+// may lie up to that many in front of the row or behind it: the one or two granules that hold them, zeros for one that holds
+// none of the row's values, and the values' offset in them.
+struct Granules { uint4 lo, hi; uint32_t shift; };
+template <typename T>
+__device__ __forceinline__ Granules load_granules(const T* row, int64_t at, int64_t D) {
+    constexpr int N = 16 / sizeof(T);
+    const char* a = reinterpret_cast<const char*>(row + at);
+    Granules g;
+    g.shift = offset16(a);
+    const uint4* first = reinterpret_cast<const uint4*>(a - g.shift);
+    const int lead = static_cast<int>(g.shift / sizeof(T));              // values in front of the thread's in the first granule
+    const bool some = at < D;
+    g.lo = some && at + N - lead > 0 ? __ldg(first) : make_uint4(0u, 0u, 0u, 0u);
+    g.hi = some && lead > 0 && at + N - lead < D ? __ldg(first + 1) : make_uint4(0u, 0u, 0u, 0u);
+    return g;
+}
+// values [at, at + 16 / sizeof(T)) to a row, the address of value `at` being a granule's
+template <typename T>
+__device__ __forceinline__ void store_granule(T* row, int64_t at, int64_t D, const uint4& v) {
+    constexpr int N = 16 / sizeof(T);
+    if (at >= 0 && at + N <= D) {
+        *reinterpret_cast<uint4*>(row + at) = v;
+    } else {
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (at + q >= 0 && at + q < D) row[at + q] = e[q];
     }
 }
 

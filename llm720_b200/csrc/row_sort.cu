@@ -14,6 +14,7 @@
 // running count per warp and digit.
 #include "kernels.h"
 #include "row_ops.cuh"
+#include "row_shift.cuh"
 
 namespace peer {
 
@@ -248,7 +249,8 @@ __global__ void __launch_bounds__(ZERO_THREADS, 8) zero_unnamed_kernel(const Row
             for (int64_t v = v0 + warp; v < v1; v += ZERO_THREADS / 32) {
                 if (marks[(v - v0) >> 5] >> ((v - v0) & 31) & 1u) continue;
                 uint16_t* row = reinterpret_cast<uint16_t*>(static_cast<char*>(a.zero_rows) + v * a.row_bytes);
-                for (int64_t c = lane; c < a.row_bytes / 2; c += 32) row[c] = 0;
+                for (int64_t c = lane * 8 - static_cast<int>(offset16(row) / 2); c < a.row_bytes / 2; c += 256)
+                    store_granule(row, c, a.row_bytes / 2, make_uint4(0u, 0u, 0u, 0u));
             }
         }
         __syncthreads();

@@ -594,6 +594,47 @@ def test_embedding_sums_in_the_order_of_the_positions(cuda_device):
         assert torch.equal(gw[v], acc)
 
 
+@pytest.mark.parametrize("D", [1, 7, 40, 67])
+@pytest.mark.parametrize("more", [0, 40000])
+def test_embedding_of_ids_that_begin_and_end_anywhere_in_a_tile(cuda_device, more, D):
+    """Ids with one position fewer, as many and one more than a tile of 16 or 64 (the latter behind 32,768 ids), from every
+    offset in one; frequent ids next to one another."""
+    repeats = [1, 15, 1, 16, 2, 17, 31, 32, 33, 3, 63, 64, 65, 5, 127, 128, 129, 16, 16, 64, 64, 17, 65, 7, 1500, 900] * 3
+    for lead in (0, 1, 7, 15, 40):
+        each = torch.tensor([lead] + repeats + [more], device=cuda_device)
+        V = each.numel() + 2                                   # the last two without a position
+        g = torch.Generator(device=cuda_device).manual_seed(lead)
+        ids = torch.repeat_interleave(torch.arange(each.numel(), device=cuda_device), each)
+        ids = ids[torch.randperm(ids.numel(), generator=g, device=cuda_device)]
+        w = torch.randn(V, D, generator=g, device=cuda_device).bfloat16().requires_grad_()
+        dy = torch.randn(ids.numel(), D, generator=g, device=cuda_device).bfloat16()
+        gw, = torch.autograd.grad(lib.embedding(ids, w, 0.5), (w,), dy)
+        ref, ref_grad, err = embedding_reference(ids, w.detach(), 0.5, dy, None)
+        close(gw, ref_grad, err, "grad")
+        assert not gw[-2:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [1, 2, 3, 7, 9, 15, 31, 129, 514, 2051])
+def test_embedding_rows_at_any_address(cuda_device, D, dtype):
+    """Tables and gradients that begin at every value of 16 bytes, rows of odd widths; what lies around the rows is left
+    alone and never enters them."""
+    V, n = 37, 300
+    g = torch.Generator(device=cuda_device).manual_seed(D)
+    ids = torch.randint(-2, V, (n,), generator=g, device=cuda_device)
+    nan = float("nan")
+    for off in (0, 1, 3, 6):
+        big = torch.full((V * D + 16,), nan, device=cuda_device, dtype=dtype)
+        w = big[off:off + V * D].view(V, D).copy_(torch.randn(V, D, generator=g, device=cuda_device)).requires_grad_()
+        wide = torch.full((n, D + 2 * off + 1), nan, device=cuda_device, dtype=dtype)
+        dy = wide[:, off:off + D].copy_(torch.randn(n, D, generator=g, device=cuda_device))
+        out = lib.embedding(ids, w, 3.0)
+        gw, = torch.autograd.grad(out, (w,), dy)
+        ref, ref_grad, err = embedding_reference(ids, w.detach(), 3.0, dy, None)
+        close(out.detach(), ref, 0 * ref, "out")
+        close(gw, ref_grad, err, "grad")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_embedding_views_shapes_and_empty_batches(cuda_device, dtype):
     V, D = 50, 24

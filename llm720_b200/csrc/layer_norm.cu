@@ -80,60 +80,6 @@ __global__ void __launch_bounds__(256) norm_loop_kernel(const NormParams p) {
     }
 }
 
-// x[r, c] of the backward pass, from either form
-template <typename T>
-__device__ __forceinline__ float kept_x(const NormGradParams& p, int64_t r, int64_t c, float s) {
-    return p.payload ? unpacked<T>(e4m3_value(p.payload[r * p.D + c]), s) : to_f32<T>(static_cast<const T*>(p.x)[r * p.x_stride + c]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) norm_grad_rows_loop_kernel(const NormGradParams p) {
-    __shared__ float buf[33];
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const T* dyr = static_cast<const T*>(p.dy) + r * p.dy_stride;
-        const float mean = p.mean[r], rstd = p.rstd[r], sc = p.payload ? p.scale[r] : 1.f;
-        float s1 = 0.f, s2 = 0.f;
-        for (int64_t c = threadIdx.x; c < p.D; c += blockDim.x) {
-            const float g = to_f32<T>(dyr[c]) * (p.w ? param_at<T>(p.w, p.param_f32, c) : 1.f);
-            s1 += g;
-            s2 = fmaf(g, (kept_x<T>(p, r, c, sc) - mean) * rstd, s2);
-        }
-        s1 = block_sum(s1, buf) / static_cast<float>(p.D);
-        s2 = block_sum(s2, buf) / static_cast<float>(p.D);
-        for (int64_t c = threadIdx.x; c < p.D; c += blockDim.x) {
-            const float g = to_f32<T>(dyr[c]) * (p.w ? param_at<T>(p.w, p.param_f32, c) : 1.f);
-            float v = rstd * (g - s1 - (kept_x<T>(p, r, c, sc) - mean) * rstd * s2);
-            if (p.add) v += to_f32<T>(static_cast<const T*>(p.add)[r * p.D + c]);
-            static_cast<T*>(p.dx)[r * p.D + c] = from_f32<T>(v);
-        }
-    }
-}
-
-// column sums of one split of the rows: 32 columns by 8 row lanes per block
-template <typename T>
-__global__ void __launch_bounds__(256) norm_grad_cols_loop_kernel(const NormGradParams p) {
-    __shared__ float sw[8][33], sb[8][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
-    const int64_t per = (p.rows + p.splits - 1) / p.splits;
-    const int64_t r0 = per * blockIdx.y, r1 = r0 + per < p.rows ? r0 + per : p.rows;
-    float aw = 0.f, ab = 0.f;
-    if (c < p.D)
-        for (int64_t r = r0 + ty; r < r1; r += 8) {
-            const float d = to_f32<T>(static_cast<const T*>(p.dy)[r * p.dy_stride + c]);
-            aw = fmaf(d, (kept_x<T>(p, r, c, p.payload ? p.scale[r] : 1.f) - p.mean[r]) * p.rstd[r], aw);
-            ab += d;
-        }
-    sw[ty][tx] = aw;
-    sb[ty][tx] = ab;
-    __syncthreads();
-    if (ty == 0 && c < p.D) {
-        for (int i = 1; i < 8; ++i) { aw += sw[i][tx]; ab += sb[i][tx]; }
-        p.partial[(static_cast<int64_t>(blockIdx.y) * 2 + 0) * p.D + c] = aw;
-        p.partial[(static_cast<int64_t>(blockIdx.y) * 2 + 1) * p.D + c] = ab;
-    }
-}
-
 // ---------------------------------------------------------------------------
 // Rows in registers.  A group of `warps` warps owns a row; every thread holds the same NV pieces of columns in every row,
 // and one exchange between the group's warps joins their sums.
@@ -1222,6 +1168,98 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const 
     }
 }
 
+// Backward of rows beyond 8,192 values (and of wide ones at odd addresses when there are few): dx by a block per row, which
+// reads it twice, the second time from L1; the column sums by a pass of their own.  4096 x 12288 bf16: dx 84 us, all gradients
+// 138 us (floor 46 us; 238 and 350 us value by value): no ring as below, whose 16 columns per thread end at 8,192.
+template <typename T, bool WIDE, bool KEPT>
+__device__ __forceinline__ void x_piece(const NormGradParams& p, int64_t r, int64_t c, float scale, float (&f)[Piece<T, WIDE>::N]) {
+    using P = Piece<T, WIDE>;
+    if constexpr (KEPT) unpack_piece<T, WIDE>(P::load_packed(p.payload + r * p.D + c), scale, f);
+    else P::decode(P::load(static_cast<const T*>(p.x) + r * p.x_stride + c), f);
+}
+
+template <typename T, bool WIDE, bool KEPT>
+__global__ void __launch_bounds__(256) norm_grad_rows_loop_kernel(const NormGradParams p) {
+    using P = Piece<T, WIDE>;
+    constexpr int N = P::N;
+    __shared__ float buf[33];
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const T* dyr = static_cast<const T*>(p.dy) + r * p.dy_stride;
+        const float mean = p.mean[r], rstd = p.rstd[r], sc = KEPT ? p.scale[r] : 1.f;
+        float s1 = 0.f, s2 = 0.f;
+        auto piece = [&](int64_t c, float (&g)[N], float (&n)[N]) {      // g = dy w, n = (x - mean) rstd
+            P::decode(P::load(dyr + c), g);
+            x_piece<T, WIDE, KEPT>(p, r, c, sc, n);
+            float w[N];
+            if (p.w) {
+                load_param_piece<T, N>(p.w, p.param_f32, c, w);
+#pragma unroll
+                for (int q = 0; q < N; ++q) g[q] *= w[q];
+            }
+#pragma unroll
+            for (int q = 0; q < N; ++q) n[q] = (n[q] - mean) * rstd;
+        };
+#pragma unroll 4
+        for (int64_t c = threadIdx.x * N; c < p.D; c += blockDim.x * N) {
+            float g[N], n[N];
+            piece(c, g, n);
+#pragma unroll
+            for (int q = 0; q < N; ++q) { s1 += g[q]; s2 = fmaf(g[q], n[q], s2); }
+        }
+        s1 = block_sum(s1, buf) / static_cast<float>(p.D);
+        s2 = block_sum(s2, buf) / static_cast<float>(p.D);
+#pragma unroll 2
+        for (int64_t c = threadIdx.x * N; c < p.D; c += blockDim.x * N) {
+            float g[N], n[N], a[N];
+            piece(c, g, n);
+            if (p.add) P::decode(P::load(static_cast<const T*>(p.add) + r * p.D + c), a);
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                g[q] = rstd * (g[q] - s1 - n[q] * s2);
+                if (p.add) g[q] += a[q];
+            }
+            P::store(static_cast<T*>(p.dx) + r * p.D + c, P::encode(g));
+        }
+    }
+}
+
+// column sums of one split of the rows: 32 pieces of columns by 8 row lanes per block
+template <typename T, bool WIDE, bool KEPT>
+__global__ void __launch_bounds__(256) norm_grad_cols_loop_kernel(const NormGradParams p) {
+    using P = Piece<T, WIDE>;
+    constexpr int N = P::N;
+    __shared__ float sums[8][2][N][32];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + tx) * N;
+    const int64_t per = (p.rows + p.splits - 1) / p.splits;
+    const int64_t r0 = per * blockIdx.y, r1 = r0 + per < p.rows ? r0 + per : p.rows;
+    float aw[N], ab[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) aw[q] = ab[q] = 0.f;
+    if (c < p.D) {
+#pragma unroll 4
+        for (int64_t r = r0 + ty; r < r1; r += 8) {
+            const float mean = p.mean[r], rstd = p.rstd[r];
+            float d[N], x[N];
+            P::decode(P::load(static_cast<const T*>(p.dy) + r * p.dy_stride + c), d);
+            x_piece<T, WIDE, KEPT>(p, r, c, KEPT ? p.scale[r] : 1.f, x);
+#pragma unroll
+            for (int q = 0; q < N; ++q) { aw[q] = fmaf(d[q], (x[q] - mean) * rstd, aw[q]); ab[q] += d[q]; }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) { sums[ty][0][q][tx] = aw[q]; sums[ty][1][q][tx] = ab[q]; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * N * 32; i += 256) {
+        const int which = i / (N * 32), k = i % (N * 32);
+        const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 * N + k;
+        float t = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) t += sums[y][which][k % N][k / N];
+        if (col < p.D) p.partial[(static_cast<int64_t>(blockIdx.y) * 2 + which) * p.D + col] = t;
+    }
+}
+
 // `splits` partial rows to the gradients: 32 columns by 32 lanes of partials per block, so that a lane's few loads are
 // all in flight at once
 constexpr int JOIN_LANES = 32;
@@ -1411,8 +1449,16 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     } else if (h.warps == 0 || p.rows == 0) {
         p.splits = splits_for(p.rows);
-        if (p.dx) norm_grad_rows_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
-        if (sums) norm_grad_cols_loop_kernel<T><<<dim3(static_cast<unsigned>((p.D + 31) / 32), static_cast<unsigned>(p.splits)), 256, 0, s>>>(p);
+        const int64_t columns = wide ? 32 * N : 32;
+        const dim3 grid(static_cast<unsigned>((p.D + columns - 1) / columns), static_cast<unsigned>(p.splits));
+        if (p.dx) {
+            if (wide) norm_grad_rows_loop_kernel<T, true, KEPT><<<row_blocks(p.rows), 256, 0, s>>>(p);
+            else norm_grad_rows_loop_kernel<T, false, KEPT><<<row_blocks(p.rows), 256, 0, s>>>(p);
+        }
+        if (sums) {
+            if (wide) norm_grad_cols_loop_kernel<T, true, KEPT><<<grid, 256, 0, s>>>(p);
+            else norm_grad_cols_loop_kernel<T, false, KEPT><<<grid, 256, 0, s>>>(p);
+        }
     } else {
         const int64_t need = (p.rows + h.groups - 1) / h.groups;
         p.splits = static_cast<int>(need < MAX_SPLITS ? need : MAX_SPLITS);

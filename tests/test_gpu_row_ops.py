@@ -315,6 +315,14 @@ def test_layer_norm_against_differences(cuda_device):
         assert abs(slope - want) <= 2e-2 + 1e-2 * (grads[i].norm() * v.norm()).item(), i
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,D", [(300, 8208), (200, 8201), (1100, 9216)])
+def test_layer_norm_of_many_rows_beyond_8192_values(cuda_device, R, D, dtype):
+    for ck in (None, "e4m3"):
+        test_layer_norm_and_its_gradients(cuda_device, R, D, dtype, ck)
+    test_gradient_of_a_residual_is_added_before_the_rounding(cuda_device, R, D, dtype)
+
+
 def test_layer_norm_of_the_widest_row(cuda_device):
     D = 1 << 20
     for dtype, ck in ((torch.bfloat16, None), (torch.float32, "e4m3")):

@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
 }
 
 // ---------------------------------------------------------------------------
-// Many rows of whole 16-byte pieces.  A group of warps owns a row, 16 columns per thread, the same columns in every row,
+// Many or wide rows of whole 16-byte pieces.  A group of warps owns a row, 16 columns per thread, the same columns in every row,
 // so parameters and column sums stay in registers.  Every thread copies its own pieces of the group's next rows into
 // shared memory (cp.async) while it works on the current one; nobody else reads them, so the ring needs no barrier and
 // no registers, and what is left in a row's chain is one exchange between the group's warps.
@@ -1301,11 +1301,20 @@ int splits_for(int64_t rows) {
 
 unsigned row_blocks(int64_t rows) { return static_cast<unsigned>(rows < 148 * 64 ? rows : 148 * 64); }
 
-constexpr int64_t RING_ROWS = 1024;   // below, a block sees too few rows for a ring to run ahead
-// rows at any address: a warp's 512 columns are too many for narrower ones (32768 x 129 bf16: 23 us forward, 21 us one
-// value at a time; 16384 x 2001: 46 and 172); the backward pass needs more rows (1500 x 1001 fp32: 14 us, 12 one value
-// at a time; 5003 x 1537 fp16: 27 and 41)
-constexpr int64_t SHIFT_DIM = 256, SHIFT_GRAD_ROWS = 2048;
+// Ring kernels take many rows, many values, or rows so wide that the others' exchange between sixteen warps costs more than
+// the start of a ring.  Measured, rings / others: forward 1000 x 1024 bf16 5.2 / 6.1 us, 512 x 1024 4.7 / 4.2, 128 x 8192
+// 5.2 / 10.3, 64 x 8191 7.9 / 18.6; all gradients 256 x 2048 bf16 8.3 / 10.3 us, 256 x 1024 fp32 8.3 / 6.7, 64 x 8192 12.4 / 16.5.
+constexpr int64_t RING_ROWS = 1024, RING_DIM = 4096;
+constexpr int64_t RING_VALUES = 1000000, RING_GRAD_VALUES = 1 << 19;
+bool ring_pays(int64_t rows, int64_t D, int64_t values) { return rows >= RING_ROWS || rows * D >= values || D > RING_DIM; }
+
+// Rows at any address: a warp's 512 columns are too many for narrower ones (32768 x 129 bf16: 23 us forward, 21 us one
+// value at a time; 16384 x 2001: 46 and 172); the backward pass needs more rows (1500 x 1001 bf16: 13.4 us, 12.4 one value at a
+// time; 1500 x 4099: 29 and 33; 512 x 8191: 27 and 21; 5003 x 1537 fp16: 27 and 41)
+constexpr int64_t SHIFT_DIM = 256, SHIFT_GRAD_ROWS = 2048, SHIFT_GRAD_DIM = 2000;
+bool shift_grad_pays(int64_t rows, int64_t D) {
+    return D > SHIFT_DIM && (rows >= SHIFT_GRAD_ROWS || (rows >= RING_ROWS && D >= SHIFT_GRAD_DIM));
+}
 
 // the width a ring kernel is built for: W full warps when the row is exactly that, else 0
 inline int ring_width(int64_t D) {
@@ -1367,7 +1376,7 @@ cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
     const bool wide = p.D % N == 0 && p.x_stride % N == 0 && aligned16(p.x) && aligned16(p.y) && (!p.w || aligned16(p.w)) &&
                       (!p.b || aligned16(p.b)) && (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0;
-    if (p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS) {
+    if (ring_pays(p.rows, p.D, RING_VALUES) && ring_warps(p.D) <= MAX_WARPS) {
         if (wide) return norm_ring_launch<T, PACK>(p, s);
         if (p.D > SHIFT_DIM) return norm_shift_launch<T, PACK>(p, s);
     }
@@ -1376,8 +1385,7 @@ cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
         norm_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         return cudaGetLastError();
     }
-    if (!wide) return h.nv == 4 ? norm_launch<T, false, 4, PACK>(p, h, s)
-                    : h.nv == 8 ? norm_launch<T, false, 8, PACK>(p, h, s) : norm_launch<T, false, 16, PACK>(p, h, s);
+    if (!wide) return h.nv == 4 ? norm_launch<T, false, 4, PACK>(p, h, s) : norm_launch<T, false, 8, PACK>(p, h, s);      // up to RING_DIM here
     return h.nv == 1 ? norm_launch<T, true, 1, PACK>(p, h, s) : norm_launch<T, true, 8, PACK>(p, h, s);
 }
 
@@ -1442,9 +1450,9 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     bool wide = p.D % N == 0 && p.dy_stride % N == 0 && aligned16(p.dy) && (!p.dx || aligned16(p.dx)) && (!p.add || aligned16(p.add)) &&
                 (!p.w || aligned16(p.w));
     wide = wide && (KEPT ? (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0 : p.x_stride % N == 0 && aligned16(p.x));
-    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16) : narrow_shape(p.rows, p.D, 16);      // wide: nv is 1 or 16 / N
+    const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16) : narrow_shape(p.rows, p.D, 16);      // wide: nv is 1, or 4 of fp32 here
     const bool sums = p.dw || p.db;
-    if (p.rows >= RING_ROWS && ring_warps(p.D) <= MAX_WARPS && (wide || (!p.add && p.D > SHIFT_DIM && p.rows >= SHIFT_GRAD_ROWS))) {
+    if (p.rows > 0 && ring_warps(p.D) <= MAX_WARPS && (wide ? ring_pays(p.rows, p.D, RING_GRAD_VALUES) : !p.add && shift_grad_pays(p.rows, p.D))) {
         const cudaError_t e = wide ? norm_grad_ring_launch<T, KEPT>(p, s) : norm_grad_shift_launch<T, KEPT>(p, s);
         if (e != cudaSuccess) return e;
     } else if (h.warps == 0 || p.rows == 0) {
@@ -1465,7 +1473,8 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
         cudaError_t e;
         if (!wide) e = h.nv == 4 ? norm_grad_launch<T, false, 4, KEPT>(p, h, s)
                      : h.nv == 8 ? norm_grad_launch<T, false, 8, KEPT>(p, h, s) : norm_grad_launch<T, false, 16, KEPT>(p, h, s);
-        else e = h.nv == 1 ? norm_grad_launch<T, true, 1, KEPT>(p, h, s) : norm_grad_launch<T, true, 16 / N, KEPT>(p, h, s);
+        else if constexpr (N == 8) e = norm_grad_launch<T, true, 1, KEPT>(p, h, s);      // up to RING_DIM here
+        else e = h.nv == 1 ? norm_grad_launch<T, true, 1, KEPT>(p, h, s) : norm_grad_launch<T, true, 4, KEPT>(p, h, s);
         if (e != cudaSuccess) return e;
     }
     if (sums) return launch_behind(norm_grad_join_kernel<T>, dim3(static_cast<unsigned>((p.D + 31) / 32)), dim3(32 * JOIN_LANES), s, p);

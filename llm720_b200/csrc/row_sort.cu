@@ -176,6 +176,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of a barrier that orders no memory on its way in: behind the wait every block of the cluster has started,
+// and its shared memory may be accessed.
+__device__ __forceinline__ void cluster_started_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_started_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // address of this block's shared memory location in another block of the cluster
 __device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
     uint32_t r;
@@ -263,6 +267,7 @@ template <int IT>
 __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 1) sort_cluster_kernel(const RowSortArgs a, int passes,
                                                                                                        int per, uint32_t* keys_out,
                                                                                                        uint32_t* order_out) {
+    cluster_started_arrive();                            // waited for in front of the first store to another block
     extern __shared__ __align__(16) unsigned char cluster_smem[];
     ClusterShared& sh = *reinterpret_cast<ClusterShared*>(cluster_smem);
     uint2* pairs = reinterpret_cast<uint2*>(cluster_smem + sizeof(ClusterShared));      // [CL_THREADS * IT]
@@ -309,6 +314,7 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(CL_THREADS, 
         sh.quarter[q][d] = run;
         __syncthreads();
         const uint32_t t0 = sh.quarter[0][d], t1 = sh.quarter[1][d], t2 = sh.quarter[2][d], t3 = sh.quarter[3][d];
+        if (p == 0) cluster_started_wait();             // shared memory of a block that has not started is not there
         {                                               // this block's count of digit d to all eight blocks
             const uint32_t at = smem_u32(&sh.totals[rank][d]);
 #pragma unroll

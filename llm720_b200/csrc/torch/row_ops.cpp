@@ -9,6 +9,7 @@
 // take at 16384 x 2048 (67 us); as here the whole pass costs 71 us.
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -50,6 +51,15 @@ void check(int rc) {
 void need_cuda(const Tensor& t, const char* name) {
     if (!t.is_cuda())
         throw std::runtime_error(text(name, " is on ", t.device(), ": peer_b200 runs on CUDA devices only (sm_100a); there is no CPU path"));
+}
+
+// A tangent would be dropped: the kernels see the values only, and the result would look like a constant.
+bool has_tangent(const Tensor& t) {
+    return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+void refuse_tangent(const Tensor& t, const char* name) {
+    if (has_tangent(t))
+        throw std::runtime_error(text(name, " carries a tangent: peer_b200 differentiates backward only, not in forward-mode"));
 }
 
 int code_of(at::ScalarType t, const char* name) {
@@ -98,6 +108,9 @@ variable_list once(variable_list grads) {
 struct NormCodes { int x, param; };
 
 NormCodes check_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+    refuse_tangent(x, "x");
+    refuse_tangent(w, "weight");
+    refuse_tangent(b, "bias");
     need_cuda(x, "x");
     NormCodes c{code_of(x.scalar_type(), "x"), PEER_DTYPE_F32};
     need_rows(x, "x");
@@ -208,6 +221,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 // ---- 8-bit rows -------------------------------------------------------------------------------------------------------
 
 std::pair<Tensor, Tensor> pack_rows(const Tensor& x_in) {
+    refuse_tangent(x_in, "x");
     need_cuda(x_in, "x");
     const int code = code_of(x_in.scalar_type(), "x");
     need_rows(x_in, "x");
@@ -222,6 +236,7 @@ std::pair<Tensor, Tensor> pack_rows(const Tensor& x_in) {
 }
 
 Tensor unpack_rows(const Tensor& payload_in, const Tensor& scale_in, at::ScalarType dtype) {
+    refuse_tangent(scale_in, "scale");
     need_cuda(payload_in, "payload");
     if (payload_in.scalar_type() != at::kFloat8_e4m3fn || scale_in.scalar_type() != at::kFloat)
         throw py::type_error(text("payload is ", dtype_name(payload_in.scalar_type()), " and scale ", dtype_name(scale_in.scalar_type()),
@@ -284,6 +299,7 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
 };
 
 Tensor embedding(const Tensor& ids_in, const Tensor& weight, double scale, std::optional<int64_t> padding_idx, const OptTensor& dropped) {
+    refuse_tangent(weight, "weight");
     need_cuda(weight, "weight");
     code_of(weight.scalar_type(), "weight");
     if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
@@ -327,6 +343,13 @@ void check_norm_arguments(const Tensor& x, const OptTensor& weight, const OptTen
     check_norm(x, weight.value_or(Tensor()), bias.value_or(Tensor()), eps);
 }
 
+// for peer.py: whether any of the layer's tensors carries one
+bool any_tangent(const std::vector<OptTensor>& tensors) {
+    for (const auto& t : tensors)
+        if (t && has_tangent(*t)) return true;
+    return false;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -338,4 +361,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("block_norm", &block_norm);
     m.def("block_norm_grad", &block_norm_grad);
     m.def("check_norm_arguments", &check_norm_arguments);
+    m.def("any_tangent", &any_tangent);
 }

@@ -15,8 +15,9 @@ from typing import List, Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
-from . import _lib
+from . import _ext, _lib
 
 _DT = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
        torch.float8_e4m3fn: _lib.DTYPE_E4M3, torch.float16: _lib.DTYPE_F16}
@@ -424,6 +425,12 @@ class PeerOp:
         return int(self.lib.peer_launch_count(self.handle))
 
 
+def _refuse_tangents(*tensors):
+    """The kernels see values only: a tangent that a tensor carries would be dropped without a word."""
+    if forward_ad._current_level >= 0 and _ext.load().any_tangent(list(tensors)):
+        raise RuntimeError("a tensor carries a tangent: peer_b200 differentiates backward only, not in forward-mode")
+
+
 class PEER(nn.Module):
     """Parameter Efficient Expert Retrieval layer on the B200 kernels.
 
@@ -654,6 +661,7 @@ class PEER(nn.Module):
         dt = self.query_proj.weight.dtype
         if hidden_states.dtype != dt:
             raise TypeError(f"hidden_states is {hidden_states.dtype} but the module's parameters are {dt}")
+        _refuse_tangents(hidden_states, *w.values())
         return w, dt
 
     # -- forward --------------------------------------------------------------
@@ -693,6 +701,7 @@ class PEER(nn.Module):
         if self.training and self.dropout.p > 0:
             raise RuntimeError("block_forward is an inference path: call eval() first (dropout is set)")
         w, dt = self._prepare(hidden_states)
+        _refuse_tangents(ln_2.weight, ln_2.bias)
         if hidden_states.device.type != "cuda":
             raise RuntimeError("peer_b200 runs on CUDA devices only (sm_100a); there is no CPU path")
         B, S, _ = hidden_states.shape
@@ -715,6 +724,7 @@ class PEER(nn.Module):
         "e4m3"``) and the selection; the norm's output and statistics are formed anew in the backward pass.
         ``ln_2``'s parameters are fp32 or of the layer's dtype."""
         w, dt = self._prepare(hidden_states)
+        _refuse_tangents(getattr(ln_2, "weight", None), getattr(ln_2, "bias", None))
         if self.input_dim != self.output_dim:
             raise ValueError(f"a block adds its input back: input_dim {self.input_dim} must equal output_dim {self.output_dim}")
         if not (self._needs_grad(hidden_states) or

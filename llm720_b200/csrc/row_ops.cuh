@@ -54,9 +54,10 @@ template <typename T> __device__ __forceinline__ float unpacked(float payload_va
     const float v = payload_value * scale;
     return fabsf(v) > max_finite<T>() ? copysignf(max_finite<T>(), v) : v;     // NaN stays NaN
 }
-// a row with such a scale may hold values that need the clamp: 448 * scale does not fit the type
+// A row with such a scale may hold values that need the clamp, 448 * |scale| being above the type's largest.  The limit, 2^7 or
+// 2^119, is the largest power of two below that; a caller's own scale may be any number, negative or NaN.
 template <typename T> __device__ __forceinline__ bool may_clamp(float scale) {
-    return scale >= (max_finite<T>() < 1e5f ? 256.f : 1.329227996e36f);         // 2^8, 2^120
+    return !(fabsf(scale) <= (max_finite<T>() < 1e5f ? 128.f : 6.646139979e35f));
 }
 
 __device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(FULL_MASK, v); }

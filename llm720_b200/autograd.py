@@ -270,8 +270,6 @@ def block_train_autograd(module, hidden_states: torch.Tensor, norm) -> torch.Ten
     w = module._weights()
     if w["down_scale"] is not None:
         raise RuntimeError("quantised (FP8) expert tables are inference-only: no backward pass")
-    if tuple(norm.normalized_shape) != (module.input_dim,):
-        raise ValueError(f"ln_2 normalises {tuple(norm.normalized_shape)}, the layer's input is ({module.input_dim},)")
     B, S, _ = hidden_states.shape
     hidden = hidden_states.contiguous().view(B * S, module.input_dim)
     _ext.load().check_norm_arguments(hidden, norm.weight, norm.bias, norm.eps)

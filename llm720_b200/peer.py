@@ -153,6 +153,9 @@ class PeerOp:
         """out = hidden + layer(LayerNorm(hidden)); hidden, out [T, D] on the device; ln_w, ln_b fp32 [D] or None."""
         self._dev(ln_w, "ln_w", torch.float32)
         self._dev(ln_b, "ln_b", torch.float32)
+        for name, p in (("ln_w", ln_w), ("ln_b", ln_b)):
+            if p is not None and p.numel() != self.cfg.input_dim:
+                raise ValueError(f"{name} has {p.numel()} values, expected {self.cfg.input_dim}")
         if out.data_ptr() == hidden.data_ptr():
             raise ValueError("out may not alias hidden")
         self._dev(product_ids_out, "product_ids_out", torch.int32)
@@ -702,6 +705,10 @@ class PEER(nn.Module):
             raise RuntimeError("block_forward is an inference path: call eval() first (dropout is set)")
         w, dt = self._prepare(hidden_states)
         _refuse_tangents(ln_2.weight, ln_2.bias)
+        for name in ("weight", "bias"):
+            p = getattr(ln_2, name)
+            if p is not None and p.numel() != self.input_dim:
+                raise ValueError(f"ln_2.{name} has {p.numel()} values, the layer's input {self.input_dim}")
         if hidden_states.device.type != "cuda":
             raise RuntimeError("peer_b200 runs on CUDA devices only (sm_100a); there is no CPU path")
         B, S, _ = hidden_states.shape
@@ -727,6 +734,8 @@ class PEER(nn.Module):
         _refuse_tangents(getattr(ln_2, "weight", None), getattr(ln_2, "bias", None))
         if self.input_dim != self.output_dim:
             raise ValueError(f"a block adds its input back: input_dim {self.input_dim} must equal output_dim {self.output_dim}")
+        if tuple(ln_2.normalized_shape) != (self.input_dim,):
+            raise ValueError(f"ln_2 normalises {tuple(ln_2.normalized_shape)}, the layer's input is ({self.input_dim},)")
         if not (self._needs_grad(hidden_states) or
                 (torch.is_grad_enabled() and any(p.requires_grad for p in ln_2.parameters()))):
             return self.block_forward(hidden_states, ln_2)

@@ -388,8 +388,20 @@ class PeerOp:
         self._dev(weights, "weights", torch.float32)
         self._dev(down, "expert_down", self.table_dtype)
         self._dev(up, "expert_up", self.table_dtype)
-        T = x.shape[0]
+        T, c = x.shape[0], self.cfg
         n_rows = down.shape[0] if grad_rows is None else int(grad_rows)
+        if not 1 <= n_rows <= c.num_experts:
+            raise ValueError(f"grad_rows={n_rows} of {c.num_experts} experts")
+        for t, name, shape in ((x, "x", (T, c.input_dim)), (grad_out, "grad_out", (T, c.output_dim))):
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} is {tuple(t.shape)}, expected {shape}")
+        neurons = max(c.expert_hidden_size, 1)              # more than one is refused by the library
+        for t, name, width in ((down, "expert_down", c.input_dim * neurons), (up, "expert_up", c.output_dim * neurons)):
+            if t.dim() != 2 or t.shape[0] < n_rows or t.shape[1] != width:
+                raise ValueError(f"{name} is {tuple(t.shape)}, expected at least {n_rows} rows of {width}")
+        for t, name in ((ids32, "ids"), (weights, "weights")):
+            if t.numel() != T * c.num_heads * c.top_k:
+                raise ValueError(f"{name} has {t.numel()} entries, expected {T} x {c.num_heads * c.top_k}")
         gx = torch.empty(T, self.cfg.input_dim, dtype=torch.float32, device=self.device)
         gw = torch.empty(T, self.cfg.num_heads * self.cfg.top_k, dtype=torch.float32, device=self.device)
         gd = torch.empty(n_rows, down.shape[1], dtype=self.table_dtype, device=self.device)

@@ -446,6 +446,12 @@ def _refuse_tangents(*tensors):
         raise RuntimeError("a tensor carries a tangent: peer_b200 differentiates backward only, not in forward-mode")
 
 
+def _is_plain_layer_norm(ln) -> bool:
+    """A call of ln is the formula over its weight, bias and eps: no forward of its own, no hooks."""
+    return (isinstance(ln, nn.LayerNorm) and type(ln).forward is nn.LayerNorm.forward and "forward" not in vars(ln) and
+            not (ln._forward_pre_hooks or ln._forward_hooks or ln._backward_pre_hooks or ln._backward_hooks))
+
+
 class PEER(nn.Module):
     """Parameter Efficient Expert Retrieval layer on the B200 kernels.
 
@@ -741,11 +747,15 @@ class PEER(nn.Module):
         """``hidden_states + self(ln_2(hidden_states))`` with a gradient: the training form of ``block_forward``,
         same values.  One autograd node that keeps ``hidden_states`` (in 8 bits with ``activation_checkpoint =
         "e4m3"``) and the selection; the norm's output and statistics are formed anew in the backward pass.
-        ``ln_2``'s parameters are fp32 or of the layer's dtype."""
+        ``ln_2``'s parameters are fp32 or of the layer's dtype.  The norm is computed from them; where ``ln_2`` does
+        more (a subclass's forward, hooks, another kind of norm) it is called as a module and the expression is
+        evaluated as written, in several nodes.  As with any method, hooks of the layer itself do not run."""
         w, dt = self._prepare(hidden_states)
         _refuse_tangents(getattr(ln_2, "weight", None), getattr(ln_2, "bias", None))
         if self.input_dim != self.output_dim:
             raise ValueError(f"a block adds its input back: input_dim {self.input_dim} must equal output_dim {self.output_dim}")
+        if not _is_plain_layer_norm(ln_2):
+            return hidden_states + self(ln_2(hidden_states))
         if tuple(ln_2.normalized_shape) != (self.input_dim,):
             raise ValueError(f"ln_2 normalises {tuple(ln_2.normalized_shape)}, the layer's input is ({self.input_dim},)")
         if not (self._needs_grad(hidden_states) or

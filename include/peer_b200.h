@@ -366,6 +366,11 @@ int peer_layer_norm_backward(const void* grad_y, int64_t grad_stride, const void
                              int32_t param_dtype, const void* add, int64_t rows, int64_t dim, void* grad_x,
                              void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The norm inside peer_block_forward, bit for bit: its output (contiguous rows) and statistics formed again for a backward
+ * pass, which hands mean and rstd [rows] (both or none) to peer_layer_norm_backward.  weight, bias fp32 or NULL. */
+int peer_block_norm(const void* x, int32_t dtype, const float* weight, const float* bias, float eps, int64_t rows,
+                    int64_t dim, void* out, float* mean, float* rstd, void* stream);
+
 /* Activation checkpoints: rows as e4m3 bytes with one fp32 scale each, the smallest power of two that brings
  * the row's largest finite magnitude to at most 448 (1 for a row of zeros, at least 2^-126).  Rounded to
  * nearest even; infinite and NaN values become NaN. */

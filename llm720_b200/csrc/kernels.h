@@ -204,9 +204,9 @@ cudaError_t launch_select_grad(const SelectGradArgs& a, cudaStream_t s);
 cudaError_t launch_route_tuples(const int32_t* ids, const float* weights, int64_t n_tokens, int entries_per_token,
                                 int64_t rows_per_rank, int world, int32_t* send, cudaStream_t s);
 
-// LayerNorm over the model dimension, fp32 parameters (block_ln.cu)
+// LayerNorm over the model dimension, fp32 parameters (block_ln.cu); mean, rstd: optional, the rows' statistics
 cudaError_t launch_block_ln(const void* x, int act_dtype, int64_t rows, int D, const float* w, const float* b, float eps,
-                            void* out, cudaStream_t s);
+                            void* out, float* mean, float* rstd, cudaStream_t s);
 // Positions of ids in the order of the ids (row_sort.cu).  `row_sort_layout` cuts a workspace of `row_sort_bytes(n)`
 // bytes; after the launch `sorted_keys` / `order` point at the sorted ids (vocab for the skipped ones, at the end) and
 // their positions.

@@ -607,7 +607,7 @@ extern "C" int peer_block_forward(peer_handle_t h, const peer_tensors_t* t, cons
     for (int64_t t0 = 0; t0 < n_tokens; t0 += c.max_tokens) {
         const int64_t n = n_tokens - t0 < c.max_tokens ? n_tokens - t0 : c.max_tokens;
         const char* xs = static_cast<const char*>(t->x) + t0 * c.input_dim * ab;
-        CU_TRY(h, launch_block_ln(xs, c.act_dtype, n, c.input_dim, ln_w, ln_b, ln_eps, h->x_ln, s));
+        CU_TRY(h, launch_block_ln(xs, c.act_dtype, n, c.input_dim, ln_w, ln_b, ln_eps, h->x_ln, nullptr, nullptr, s));
         h->launches += 1;
         rc = forward_slice(h, t, h->x_ln, static_cast<char*>(t->out) + t0 * c.output_dim * ab,
                            t->ids_out ? t->ids_out + t0 * HK : nullptr, t->scores_out ? t->scores_out + t0 * HK : nullptr,

@@ -323,10 +323,19 @@ Tensor embedding(const Tensor& ids_in, const Tensor& weight, double scale, std::
 
 // ---- for autograd.py: the norm inside the block's node ------------------------------------------------------------------
 
+// The forward pass's values again (peer_block_norm), and the statistics [2, rows].
 std::pair<Tensor, Tensor> block_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-    NormOut o = norm_forward(x, w, b, eps, check_norm(x, w, b, eps), true, false);
-    return {o.y, o.stats};
+    const NormCodes c = check_norm(x, w, b, eps);
+    const at::AutoGradMode off(false);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor rows = as_rows(x).contiguous(), w32 = w.defined() ? w.to(at::kFloat) : w, b32 = b.defined() ? b.to(at::kFloat) : b;
+    const int64_t R = rows.size(0), D = rows.size(1);
+    Tensor y = at::empty(x.sizes(), x.options()), stats = at::empty({2, R}, x.options().dtype(at::kFloat));
+    float* mean = stats.data_ptr<float>();
+    check(peer_block_norm(rows.data_ptr(), c.x, static_cast<const float*>(ptr(w32)), static_cast<const float*>(ptr(b32)),
+                          static_cast<float>(eps), R, D, y.data_ptr(), mean, mean + R, stream_of(x)));
+    return {y, stats};
 }
 
 std::tuple<OptTensor, OptTensor, OptTensor> block_norm_grad(const Tensor& grad, const Tensor& x, const Tensor& stats, const OptTensor& weight,

@@ -48,3 +48,18 @@ def test_the_operator_refuses_them_too():
     for w, b in ((torch.ones(32), None), (None, torch.ones(65))):
         with pytest.raises(ValueError, match="64"):
             op.block_forward(h, {}, w, b, 1e-5, out)
+
+
+def test_the_block_norms_entry_refuses_before_any_launch():
+    from llm720_b200 import _lib
+    native = _lib.load()
+
+    def call(x=16, dt=_lib.DTYPE_BF16, w=None, b=None, eps=1e-5, rows=4, dim=8, out=16, mean=16, rstd=16):
+        return native.peer_block_norm(x, dt, w, b, eps, rows, dim, out, mean, rstd, None)
+
+    for kw in (dict(x=None), dict(out=None), dict(rows=-1), dict(dim=0), dict(dim=(1 << 20) + 1), dict(dt=_lib.DTYPE_E4M3),
+               dict(eps=-1.0), dict(eps=float("nan")), dict(mean=None), dict(rstd=None), dict(x=17), dict(out=17), dict(w=18),
+               dict(b=18), dict(mean=18)):
+        assert call(**kw) == _lib.ERR_INVALID_ARG, kw
+        assert "peer_block_norm" in _lib.last_error(None)
+    assert call(rows=0, x=None, out=None) == _lib.OK

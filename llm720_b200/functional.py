@@ -10,6 +10,7 @@ import torch
 from .peer import PeerOp
 
 _OPS = {}
+_CAPTURED = []              # handles whose scratch a captured graph holds addresses of: never closed
 
 
 def peer_forward(x: torch.Tensor, query_weight: torch.Tensor, query_bias: Optional[torch.Tensor],
@@ -60,7 +61,7 @@ def peer_forward(x: torch.Tensor, query_weight: torch.Tensor, query_bias: Option
     T = B * S
     op = _OPS.get(key)
     if op is None or op.cfg.max_tokens < min(T, 16384):
-        if op is not None:
+        if op is not None and not any(op is kept for kept in _CAPTURED):
             op.close()
         op = PeerOp(input_dim=D, output_dim=out_dim, num_heads=num_heads, query_dim=query_dim,
                     product_key_dim=(n0, n1), top_k=top_k, act_dtype=x.dtype, table_dtype=u.dtype,
@@ -68,6 +69,8 @@ def peer_forward(x: torch.Tensor, query_weight: torch.Tensor, query_bias: Option
                     index_mode=index_mode, max_tokens=min(max(T, 1), 16384),
                     expert_hidden_size=expert_hidden_size, device=x.device)
         _OPS[key] = op
+    if torch.cuda.is_current_stream_capturing() and not any(op is kept for kept in _CAPTURED):
+        _CAPTURED.append(op)
     w = dict(query_w=qw, query_b=None if query_bias is None else query_bias.reshape(-1),
              ln_w=None if ln_weight is None else ln_weight.reshape(-1)[:query_dim],
              ln_b=None if ln_bias is None else ln_bias.reshape(-1)[:query_dim],

@@ -540,6 +540,7 @@ class PEER(nn.Module):
         self._op_key = None
         self._sel_op: Optional[PeerOp] = None
         self._sel_op_key = None
+        self._captured_ops: List[PeerOp] = []
         self._tier = None           # (row_map, cache_down, cache_up) while the tables live in host memory
 
     # -- FP8 tables ---------------------------------------------------------
@@ -648,7 +649,14 @@ class PEER(nn.Module):
             self._op_key = key
             if self._tier is not None:
                 self._op.set_row_tier(*self._tier)
-        return self._op
+        return self._kept_for_graphs(self._op)
+
+    def _kept_for_graphs(self, op: PeerOp) -> PeerOp:
+        """A graph that is being captured holds addresses of the handle's scratch: the handle then lives as long as
+        the module, whatever takes its place."""
+        if torch.cuda.is_current_stream_capturing() and not any(op is kept for kept in self._captured_ops):
+            self._captured_ops.append(op)
+        return op
 
     def _product_operator(self, device, act_dtype, n_tokens: int) -> PeerOp:
         """A second handle whose selection returns i0 * n1 + i1 whatever ``index_mode`` is: the
@@ -666,7 +674,7 @@ class PEER(nn.Module):
                                   index_mode="product", max_tokens=cap,
                                   expert_hidden_size=self.expert_hidden_size, device=device)
             self._sel_op_key = key
-        return self._sel_op
+        return self._kept_for_graphs(self._sel_op)
 
     def _needs_grad(self, hidden_states: torch.Tensor) -> bool:
         need = torch.is_grad_enabled() and (hidden_states.requires_grad or

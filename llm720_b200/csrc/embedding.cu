@@ -24,7 +24,8 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int id_bytes, int64_t 
 
 // `group` threads (a warp, or the block when there are few tokens) per token, 16-byte pieces.  Not WIDE: the pieces are the
 // granules of the row that is written, read as two granules and shifted (20,000 x 2500 bf16: 37 us, 57 value by value); the
-// values in front of the first whole granule and behind the last one are copied by a thread each.
+// values in front of the first whole granule and behind the last one are copied by a thread each, and so are those of a piece
+// whose granules reach beyond the table.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) embed_kernel(const void* __restrict__ ids, int id_bytes, int64_t n, const T* __restrict__ w,
                                                     int64_t vocab, int64_t D, float scale, T* __restrict__ out,
@@ -38,18 +39,20 @@ __global__ void __launch_bounds__(256) embed_kernel(const void* __restrict__ ids
         if (!inside && dropped && gt == 0) atomicAdd(dropped, 1ULL);
         const T* row = w + (inside ? id : 0) * D;          // row 0 is read in place of none: no test between the loads
         T* dst = out + t * D;
-        int64_t begin = 0, end = D;
+        int begin = 0, end = static_cast<int>(D);
         uint32_t shift = 0;
         if constexpr (!WIDE) {
-            begin = (16u - offset16(dst)) % 16u / sizeof(T);
-            begin = begin < D ? begin : D;
-            end = D - (D - begin) % N;
-            const int64_t c = gt < N ? gt : end + gt - N;
-            if (gt < N ? gt < begin : c < D) dst[c] = from_f32<T>(inside ? to_f32<T>(row[c]) * scale : 0.f);
-            shift = offset16(row + begin);
+            const PieceRange range = piece_range(reinterpret_cast<uintptr_t>(row), reinterpret_cast<uintptr_t>(dst), static_cast<int>(D),
+                                                 sizeof(T), reinterpret_cast<uintptr_t>(w), reinterpret_cast<uintptr_t>(w + vocab * D));
+            begin = range.begin;
+            end = range.end;
+            shift = range.shift;
+            // fewer than 2 N values at either end: lanes 0 to 15 in front, 16 to 31 behind
+            const int c = gt < 16 ? gt : end + gt - 16;
+            if (gt < 16 ? gt < begin : c < D && gt < 32) dst[c] = from_f32<T>(inside ? to_f32<T>(row[c]) * scale : 0.f);
         }
 #pragma unroll 4
-        for (int64_t c = begin + static_cast<int64_t>(gt) * N; c < end; c += group * N) {
+        for (int c = begin + gt * N; c < end; c += group * N) {
             float f[N];
             if constexpr (WIDE) {
                 P::decode(P::load(row + c), f);

@@ -830,10 +830,10 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
     const T* cur = src;
     const int64_t src_step = step * p.x_stride;
     uint32_t slot = slot0, fetch_slot = slot0;
-    auto fetch = [&]() {
+    auto fetch = [&](auto head) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (to_fetch > 0) fetch_row(fetch_slot, src, bytes, gt, threads);
+            if (to_fetch > 0) fetch_row<decltype(head)::value>(fetch_slot, src, bytes, gt, threads, p.x);
             src += src_step;
             --to_fetch;
             fetch_slot += room;
@@ -841,7 +841,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
         if (fetch_slot == slot_end) fetch_slot = slot0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    fetch(std::true_type());
+    for (int k = 1; k < STAGES - 1; ++k) fetch(std::false_type());
     float2 w[NV][H], b[NV][H];
     load_param_values<T, NV, N>(p.w, p.param_f32, D, gt, threads, 1.f, w);
     load_param_values<T, NV, N>(p.b, p.param_f32, D, gt, threads, 0.f, b);
@@ -852,7 +853,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
     // this row's slots; the next row's leave them alone
     int exchange = U == 2 ? group * 32 : group * warps, other = U == 2 ? 8 * 32 : MAX_WARPS;
     for (; rows > 0; rows -= U) {
-        fetch();
+        fetch(std::false_type());
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         sync();                                             // the other threads' granules
         typename P::Raw raw[U][NV];
@@ -1027,11 +1028,11 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const 
     const char* cur_x = src_x;
     const int64_t dy_step = step * p.dy_stride, x_step = step * (KEPT ? p.D : p.x_stride * static_cast<int64_t>(sizeof(T)));
     uint32_t slot = slot0, fetch_slot = slot0;
-    auto fetch = [&]() {
+    auto fetch = [&](auto head) {
         if (to_fetch > 0) {
             if (brings) copy_async<4>(fetch_slot + room + room_x + gt * 4, src_stat);
-            fetch_row(fetch_slot, src_dy, bytes, gt, threads);
-            fetch_row(fetch_slot + room, src_x, x_bytes, gt, threads);
+            fetch_row<decltype(head)::value>(fetch_slot, src_dy, bytes, gt, threads, p.dy);
+            fetch_row<decltype(head)::value>(fetch_slot + room, src_x, x_bytes, gt, threads, KEPT ? static_cast<const void*>(p.payload) : p.x);
         }
         src_dy += dy_step;
         src_x += x_step;
@@ -1041,7 +1042,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const 
         if (fetch_slot == slot_end) fetch_slot = slot0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    fetch(std::true_type());
+    for (int k = 1; k < STAGES - 1; ++k) fetch(std::false_type());
     float2 w[NV][H], aw[NV][H], ab[NV][H];
     load_param_values<T, NV, N>(p.w, p.param_f32, D, gt, threads, 1.f, w);
 #pragma unroll
@@ -1051,7 +1053,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const 
     int64_t r = first;
     int exchange = group * warps, other = MAX_WARPS;        // this row's slots; the next row's leave them alone
     for (; rows > 0; --rows) {
-        fetch();
+        fetch(std::false_type());
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         sync();                                             // the other threads' granules
         const uint4 st = shared_at<uint4>(slot + room + room_x);
@@ -1378,10 +1380,10 @@ cudaError_t norm_pack_t(const NormParams& p, cudaStream_t s) {
                       (!p.b || aligned16(p.b)) && (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0;
     if (ring_pays(p.rows, p.D, RING_VALUES) && ring_warps(p.D) <= MAX_WARPS) {
         if (wide) return norm_ring_launch<T, PACK>(p, s);
-        if (p.D > SHIFT_DIM) return norm_shift_launch<T, PACK>(p, s);
+        if (p.D > SHIFT_DIM && first_row_alone(p.x, p.x_stride * static_cast<int64_t>(sizeof(T)), p.rows)) return norm_shift_launch<T, PACK>(p, s);
     }
     const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 8, 8) : narrow_shape(p.rows, p.D, 8);      // wide: nv is 1 or 8 here
-    if (h.warps == 0) {
+    if (h.warps == 0 || (!wide && p.D > RING_DIM)) {      // the latter: expanded or overlapping rows at an odd address
         norm_loop_kernel<T><<<row_blocks(p.rows), 256, 0, s>>>(p);
         return cudaGetLastError();
     }
@@ -1452,7 +1454,9 @@ cudaError_t norm_grad_kept_t(NormGradParams p, cudaStream_t s) {
     wide = wide && (KEPT ? (reinterpret_cast<uintptr_t>(p.payload) & (N - 1)) == 0 : p.x_stride % N == 0 && aligned16(p.x));
     const RowShape h = wide ? row_shape(p.rows, p.D / N, 1, 16 / N, 16) : narrow_shape(p.rows, p.D, 16);      // wide: nv is 1, or 4 of fp32 here
     const bool sums = p.dw || p.db;
-    if (p.rows > 0 && ring_warps(p.D) <= MAX_WARPS && (wide ? ring_pays(p.rows, p.D, RING_GRAD_VALUES) : !p.add && shift_grad_pays(p.rows, p.D))) {
+    const bool alone = wide || (first_row_alone(p.dy, p.dy_stride * static_cast<int64_t>(sizeof(T)), p.rows) &&
+                                (KEPT || first_row_alone(p.x, p.x_stride * static_cast<int64_t>(sizeof(T)), p.rows)));
+    if (p.rows > 0 && ring_warps(p.D) <= MAX_WARPS && (wide ? ring_pays(p.rows, p.D, RING_GRAD_VALUES) : alone && !p.add && shift_grad_pays(p.rows, p.D))) {
         const cudaError_t e = wide ? norm_grad_ring_launch<T, KEPT>(p, s) : norm_grad_shift_launch<T, KEPT>(p, s);
         if (e != cudaSuccess) return e;
     } else if (h.warps == 0 || p.rows == 0) {

@@ -2,6 +2,7 @@
 // (the format is defined in row_ops.cuh).  Packing reads 2 (4) bytes and writes
 // 1 per value, unpacking the reverse: both are bound by HBM.
 #include <cstdio>
+#include <type_traits>
 
 #include "kernels.h"
 #include "row_ops.cuh"
@@ -129,18 +130,19 @@ __global__ void __launch_bounds__(RING_THREADS, 2) pack_shift_kernel(const T* __
     const T* src = x + first * x_stride;
     const T* cur = src;
     uint32_t slot = slot0, fetch_slot = slot0;
-    auto fetch = [&]() {
-        if (to_fetch > 0) fetch_row(fetch_slot, src, bytes, gt, threads);
+    auto fetch = [&](auto head) {
+        if (to_fetch > 0) fetch_row<decltype(head)::value>(fetch_slot, src, bytes, gt, threads, x);
         src += step * x_stride;
         --to_fetch;
         fetch_slot += room;
         if (fetch_slot == slot_end) fetch_slot = slot0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    fetch(std::true_type());
+    for (int k = 1; k < STAGES - 1; ++k) fetch(std::false_type());
     int parity = 0;
     for (int64_t r = first; left > 0; --left, r += step) {
-        fetch();
+        fetch(std::false_type());
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         sync();                                             // the other threads' granules
         const uint32_t shift = offset16(cur);
@@ -189,17 +191,18 @@ __global__ void __launch_bounds__(RING_THREADS, 2) unpack_shift_kernel(const uin
     int left = first < rows ? static_cast<int>((rows - first + step - 1) / step) : 0;
     int64_t fetch_row_no = first;
     uint32_t slot = slot0, fetch_slot = slot0;
-    auto fetch = [&]() {
-        if (fetch_row_no < rows) fetch_row(fetch_slot, payload + fetch_row_no * D, D, gt, threads);
+    auto fetch = [&](auto head) {
+        if (fetch_row_no < rows) fetch_row<decltype(head)::value>(fetch_slot, payload + fetch_row_no * D, D, gt, threads, payload);
         fetch_row_no += step;
         fetch_slot += room8;
         if (fetch_slot == slot_end) fetch_slot = slot0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int k = 0; k < STAGES - 1; ++k) fetch();
+    fetch(std::true_type());
+    for (int k = 1; k < STAGES - 1; ++k) fetch(std::false_type());
     for (int64_t r = first; left > 0; --left, r += step) {
         const float s = __ldg(scale + r);
-        fetch();
+        fetch(std::false_type());
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         sync();                                             // the other threads' granules; the last row's results have left
         const uint32_t shift = offset16(payload + r * D);
@@ -236,7 +239,8 @@ cudaError_t pack_t(const void* xv, int64_t x_stride, int64_t rows, int64_t D, ui
     constexpr int N = 16 / sizeof(T);
     const T* x = static_cast<const T*>(xv);
     const bool wide = D % N == 0 && x_stride % N == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(payload) & (N - 1)) == 0;
-    if (!wide && rows >= SHIFT_ROWS && D >= 512 && ring_warps(D) <= MAX_ROW_WARPS) {      // 32768 x 65: 19 us against 10
+    if (!wide && rows >= SHIFT_ROWS && D >= 512 && ring_warps(D) <= MAX_ROW_WARPS &&
+        first_row_alone(x, x_stride * static_cast<int64_t>(sizeof(T)), rows)) {      // 32768 x 65: 19 us against 10
         constexpr int STAGES = 4;
         const int warps = ring_warps(D), groups = MAX_ROW_WARPS / warps, columns = warps * 32 * RING_COLUMNS;
         const int smem = groups * (STAGES * row_room(columns, sizeof(T)) + 16 + row_room(columns, 1));
@@ -273,7 +277,7 @@ cudaError_t unpack_t(const uint8_t* payload, const float* scale, int64_t rows, i
         unpack_rows_kernel<T><<<grid, 256, 0, s>>>(payload, scale, rows, D, segments, static_cast<T*>(out));
         return cudaGetLastError();
     }
-    if (rows >= SHIFT_ROWS && ring_warps(D) <= MAX_ROW_WARPS) {
+    if (rows >= SHIFT_ROWS && ring_warps(D) <= MAX_ROW_WARPS && first_row_alone(payload, D, rows)) {
         constexpr int STAGES = 4;
         const int warps = ring_warps(D), groups = MAX_ROW_WARPS / warps, columns = warps * 32 * RING_COLUMNS;
         const int smem = groups * (STAGES * row_room(columns, 1) + 16 + row_room(columns, sizeof(T)));

@@ -1,10 +1,12 @@
 // Rows at any address.  A row is brought into shared memory as the aligned 16-byte granules that cover it; thread c's
 // 16 bytes lie at the same offset, 0 to 15, in granules c and c + 1 for every thread, and come out with a few selects and
 // a funnel shift.  Results are laid down in shared memory in the row's own order and leave as aligned granules the same
-// way, the first and last by value.  A copy never reads past the row's end (the rest of the granule is filled with
-// zeros); it may read up to 15 bytes before the row's start, inside the 16 bytes that hold its first value.
+// way, the first and last by value.  A granule at a row's end may hold values of its neighbours, which are not used; one
+// that reaches beyond the buffer's first or last value is read value by value (granule.h), so nothing outside the buffer
+// (from its first row's first value to its last row's last one) is read.
 #pragma once
 
+#include "granule.h"
 #include "row_ops.cuh"
 
 namespace peer {
@@ -77,13 +79,38 @@ template <> __device__ __forceinline__ uint32_t shared_unaligned<uint32_t>(uint3
 __device__ __forceinline__ int granules(uint32_t shift, int bytes) { return (static_cast<int>(shift) + bytes + 15) >> 4; }
 __device__ __forceinline__ uint32_t offset16(const void* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u; }
 
-// a group's threads bring the granules of one row, and zeros in the one behind them (a thread's 16 bytes may reach there)
-__device__ __forceinline__ void fetch_row(uint32_t dst, const void* row, int bytes, int gt, int threads) {
+// A granule that reaches beyond its buffer [begin, end), value by value, zeros in place of what lies outside.  Rare (the first
+// and last rows of a buffer at an odd address), so it is kept out of line: beside the loads of whole granules its branches
+// would keep them from being in flight together.
+template <typename T>
+__device__ __noinline__ uint4 partial_granule(const void* g, const void* begin, const void* end) {
+    const GranulePart part = granule_part(reinterpret_cast<uintptr_t>(g), reinterpret_cast<uintptr_t>(begin), reinterpret_cast<uintptr_t>(end));
+    alignas(16) T v[16 / sizeof(T)];
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(16 / sizeof(T)); ++q) {
+        const int byte = q * static_cast<int>(sizeof(T));
+        v[q] = byte >= part.first && byte < part.last ? __ldg(static_cast<const T*>(g) + q) : T{};
+    }
+    return *reinterpret_cast<const uint4*>(v);
+}
+
+// a group's threads bring the granules of one row, and zeros in the one behind them (a thread's 16 bytes may reach there).
+// Behind the row's own end nothing is read.  HEAD: the row may be the buffer's first, and its first granule reach out in front.
+template <bool HEAD>
+__device__ __forceinline__ void fetch_row(uint32_t dst, const void* row, int bytes, int gt, int threads, const void* begin) {
     const uint32_t shift = offset16(row);
     const char* first = static_cast<const char*>(row) - shift;
     const int n = granules(shift, bytes), end = static_cast<int>(shift) + bytes;
-    for (int c = gt; c <= n; c += threads) copy_async_filled(dst + c * 16, c < n ? first + c * 16 : first, max(min(16, end - c * 16), 0));
+    int c = gt;
+    if (HEAD && gt == 0 && first < static_cast<const char*>(begin)) {
+        store_shared(dst, partial_granule<uint8_t>(first, begin, static_cast<const char*>(row) + bytes));
+        c += threads;
+    }
+    for (; c <= n; c += threads) copy_async_filled(dst + c * 16, c < n ? first + c * 16 : first, max(min(16, end - c * 16), 0));
 }
+// Only the first row's granules reach out in front of the buffer, so only a ring's first fetch asks: rows closer together than
+// a granule (`stride` bytes) at an odd address go by value.
+inline bool first_row_alone(const void* begin, int64_t stride, int64_t rows) { return rows <= 1 || stride >= 16 || aligned16(begin); }
 // a row laid down at `src` (16 bytes in front of it are the group's too) to its place in memory; U: a value
 template <typename U>
 __device__ __forceinline__ void store_row(void* row, uint32_t src, int bytes, int gt, int threads) {
@@ -108,21 +135,31 @@ __device__ __forceinline__ void store_row(void* row, uint32_t src, int bytes, in
 
 // The same without shared memory, for a thread that takes 16 / sizeof(T) values of a row of D from value `at` on, where `at`
 // may lie up to that many in front of the row or behind it: the one or two granules that hold them, zeros for one that holds
-// none of the row's values, and the values' offset in them.
+// none of the row's values, and the values' offset in them.  `load_granules` is for rows 16 bytes and more away from the ends of
+// their buffer; its loads have no branch between them.  `load_edge_granules` takes any row.
 struct Granules { uint4 lo, hi; uint32_t shift; };
 template <typename T>
 __device__ __forceinline__ Granules load_granules(const T* row, int64_t at, int64_t D) {
-    constexpr int N = 16 / sizeof(T);
-    const char* a = reinterpret_cast<const char*>(row + at);
+    const GranuleWants w = granule_wants(reinterpret_cast<uintptr_t>(row), at, D, sizeof(T));
+    const uint4* first = reinterpret_cast<const uint4*>(w.first);
     Granules g;
-    g.shift = offset16(a);
-    const uint4* first = reinterpret_cast<const uint4*>(a - g.shift);
-    const int lead = static_cast<int>(g.shift / sizeof(T));              // values in front of the thread's in the first granule
-    const bool some = at < D;
-    g.lo = some && at + N - lead > 0 ? __ldg(first) : make_uint4(0u, 0u, 0u, 0u);
-    g.hi = some && lead > 0 && at + N - lead < D ? __ldg(first + 1) : make_uint4(0u, 0u, 0u, 0u);
+    g.shift = w.shift;
+    g.lo = w.lo ? __ldg(first) : make_uint4(0u, 0u, 0u, 0u);
+    g.hi = w.hi ? __ldg(first + 1) : make_uint4(0u, 0u, 0u, 0u);
     return g;
 }
+template <typename T>
+__device__ __forceinline__ Granules load_edge_granules(const T* row, int64_t at, int64_t D, const void* begin, const void* end) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(begin), e = reinterpret_cast<uintptr_t>(end);
+    const GranuleWants w = granule_wants(reinterpret_cast<uintptr_t>(row), at, D, sizeof(T));
+    const uint4* first = reinterpret_cast<const uint4*>(w.first);
+    Granules g{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u), w.shift};
+    if (w.lo) g.lo = granule_inside(w.first, b, e) ? __ldg(first) : partial_granule<T>(first, begin, end);
+    if (w.hi) g.hi = granule_inside(w.first + 16, b, e) ? __ldg(first + 1) : partial_granule<T>(first + 1, begin, end);
+    return g;
+}
+// rows at either end of a buffer of n rows that lie within 16 bytes of it, for rows `stride` bytes apart
+inline int64_t edge_rows(int64_t n, int64_t stride) { return stride >= 16 ? 1 : stride > 0 ? (16 + stride - 1) / stride : n; }
 // values [at, at + 16 / sizeof(T)) to a row, the address of value `at` being a granule's
 template <typename T>
 __device__ __forceinline__ void store_granule(T* row, int64_t at, int64_t D, const uint4& v) {

@@ -22,6 +22,8 @@ struct SumParams {
     const uint32_t* keys; const uint32_t* order;   // sorted ids (vocab = none) and their positions
     int64_t n; uint32_t vocab;
     const void* src; int64_t src_stride;           // rows that are added
+    const void* src_end;                           // behind the last one's last value (not WIDE)
+    uint32_t edge, inner;                          // rows [edge, edge + inner) are 16 bytes away from the ends of src (not WIDE)
     const float* coef; uint32_t per_row;           // position j adds coef[j] * row j / per_row
     float scale;
     void* out; int64_t D;
@@ -107,7 +109,7 @@ __device__ __forceinline__ int first_index(int lo, int hi, const F& below) {
 // block when rows are short).  Eight rows' pieces are in flight per thread, four where rows are not whole 16-byte pieces; the
 // additions keep the order of positions.  Not WIDE: a thread's columns begin at a granule of the row that it writes, so they
 // depend on the id, and are read as two granules and shifted (20,000 ids of 8,000 x 2500 bf16: the gradient takes
-// 63 us, 109 value by value).
+// 66 us, 109 value by value).
 template <typename T, bool WIDE, int PER, bool COEF>
 __global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p) {
     using P = Piece<T, true>;
@@ -124,6 +126,7 @@ __global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p)
     }
     const int subs = SUM_THREADS / p.row_threads, sub = threadIdx.x / p.row_threads;
     const int64_t job = blockIdx.x - p.zero_blocks, slab = job % p.slabs, tile0 = job / p.slabs * subs;
+    bool edge = false;                                     // rows within 16 bytes of the ends of src among them
     for (int i = threadIdx.x; i < (subs + 2) * PER; i += SUM_THREADS) {
         const int64_t j = (tile0 - 1) * PER + i;
         s_key[i] = j >= 0 && j < p.n ? p.keys[j] : p.vocab;
@@ -131,8 +134,9 @@ __global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p)
         const uint32_t at = j < p.n ? p.order[j] : 0u;
         s_pos[i - PER] = COEF ? at / p.per_row : at;
         if constexpr (COEF) s_coef[i - PER] = j < p.n ? p.coef[at] : 0.f;
+        if constexpr (!WIDE) edge |= j < p.n && at - p.edge >= p.inner;
     }
-    __syncthreads();
+    const bool edges = __syncthreads_or(edge) != 0;        // one block or two of the grid
     const int64_t tile = tile0 + sub, t0 = tile * PER;
     const int64_t c = (slab * p.row_threads + (threadIdx.x - sub * p.row_threads)) * N;
     if (t0 >= p.n || c >= p.D + (WIDE ? 0 : N - 1)) return;
@@ -192,10 +196,18 @@ __global__ void __launch_bounds__(SUM_THREADS) row_sum_kernel(const SumParams p)
     };
     for (; j < end; j += U) {
         std::conditional_t<WIDE, uint4, Granules> raw[U];
+        if constexpr (WIDE) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if constexpr (WIDE) raw[u] = j + u < end ? P::load(src + static_cast<int64_t>(pos[j + u]) * p.src_stride + c) : P::zero();
-            else if (j + u < end) raw[u] = load_granules(src + static_cast<int64_t>(pos[j + u]) * p.src_stride, column(key[j + u]), p.D);
+            for (int u = 0; u < U; ++u) raw[u] = j + u < end ? P::load(src + static_cast<int64_t>(pos[j + u]) * p.src_stride + c) : P::zero();
+        } else if (!edges) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j + u < end) raw[u] = load_granules(src + static_cast<int64_t>(pos[j + u]) * p.src_stride, column(key[j + u]), p.D);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j + u < end)
+                    raw[u] = load_edge_granules(src + static_cast<int64_t>(pos[j + u]) * p.src_stride, column(key[j + u]), p.D, src, p.src_end);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -310,10 +322,14 @@ cudaError_t sums_launch(SumParams p, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t sums_t(const SumParams& p, cudaStream_t s) {
+cudaError_t sums_t(SumParams p, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
     const bool wide = p.D % N == 0 && p.src_stride % N == 0 && aligned16(p.src) && aligned16(p.out);
     const bool small = per_tile_for(p.n) == 16;
+    p.src_end = static_cast<const T*>(p.src) + (p.n - 1) * p.src_stride + p.D;      // one row per position
+    const int64_t edge = edge_rows(p.n, p.src_stride * static_cast<int64_t>(sizeof(T)));
+    p.edge = static_cast<uint32_t>(edge);
+    p.inner = static_cast<uint32_t>(p.n > 2 * edge ? p.n - 2 * edge : 0);
     if (p.coef) {                                           // the expert tables: always whole 16-byte pieces
         if (!wide) return cudaErrorInvalidValue;
         return small ? sums_launch<T, true, 16, true>(p, s) : sums_launch<T, true, 64, true>(p, s);

@@ -42,6 +42,36 @@ struct NormGradParams {
     int splits;
 };
 
+// ---------------------------------------------------------------------------
+// Rows in registers.  A group of `warps` warps owns a row; every thread holds the same NV pieces of columns in every row,
+// and one exchange between the group's warps joins their sums.
+//
+// Forward statistics (here and below): each warp takes the mean of its own columns, rounded, as a center c and sums the
+// deviations from it, s = sum(x - c), and their squares, q.  About any one center c0 a warp's n columns then have
+//   sum(x - c0) = s + n e =: t,   sum(x - c0)^2 = q + e (s + t),   e = c - c0,
+// so one exchange of (c, q, s) gives the row's  mean = c0 + T / D  and  M2 = Q - T^2 / D  with T, Q summed over the warps.  The
+// centers cancel: without s the roundings of the warps' means (2^-24 of the mean) would enter M2 times the distance between the
+// warps' means (530 fp32 values of 1000 +- 0.5: a deviation off by 250 * 2^-24 and more; the mean, too, is only as good).  c0 is
+// the first warp's center, which lies within four deviations of the mean (it holds 1/16 of the columns at least), mostly far less.
+// For the 16-bit types s costs no pass: where the mean is large against the deviation the values share their leading bits, a
+// warp's sum S of at most 2,048 of them is exact in fp32, and s = S - n c is one fma (zero where n is a power of two, as in rows of
+// 512 W columns); elsewhere its rounding is one of the values' magnitude, as everywhere.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void add_part(float c0, float c, float q, float s, float n, float& t_all, float& q_all) {
+    const float e = c - c0, t = fmaf(n, e, s);
+    t_all += t;
+    q_all += fmaf(e, s + t, q);
+}
+// T, Q about c0 to the mean and M2, which rounding can take below zero and overflow to inf - inf; rows with an infinity or NaN
+// have a mean of NaN
+__device__ __forceinline__ void finish_stats(float c0, float t, float q, float inv_d, float& mean, float& m2) {
+    const float off = t * inv_d, inf = __uint_as_float(F32_INF_BITS);
+    mean = c0 + off;
+    m2 = fmaf(-t, off, q);
+    if (!(m2 >= 0.f)) m2 = fabsf(mean) < inf ? (fabsf(q) < inf ? 0.f : inf) : q;
+}
+constexpr int MAX_WARPS = MAX_ROW_WARPS;
+
 // any width, any alignment: one block per row
 template <typename T>
 __global__ void __launch_bounds__(256) norm_loop_kernel(const NormParams p) {
@@ -55,10 +85,19 @@ __global__ void __launch_bounds__(256) norm_loop_kernel(const NormParams p) {
             s += v;
             top = max(top, finite_abs_bits(v));
         }
-        const float mean = block_sum(s, buf) / static_cast<float>(p.D);
-        float ss = 0.f;
-        for (int64_t c = threadIdx.x; c < p.D; c += blockDim.x) { const float d = to_f32<T>(xr[c]) - mean; ss = fmaf(d, d, ss); }
-        const float rstd = 1.0f / sqrtf(block_sum(ss, buf) / static_cast<float>(p.D) + p.eps);
+        const float inv_d = 1.f / static_cast<float>(p.D), center = block_sum(s, buf) * inv_d;
+        float q = 0.f;
+        s = 0.f;
+        for (int64_t c = threadIdx.x; c < p.D; c += blockDim.x) {
+            const float d = to_f32<T>(xr[c]) - center;
+            s += d;
+            q = fmaf(d, d, q);
+        }
+        s = block_sum(s, buf);
+        q = block_sum(q, buf);
+        float mean, m2;
+        finish_stats(center, s, q, inv_d, mean, m2);
+        const float rstd = 1.0f / sqrtf(m2 * inv_d + p.eps);
         T* yr = static_cast<T*>(p.y) + r * p.D;
         for (int64_t c = threadIdx.x; c < p.D; c += blockDim.x) {
             float v = (to_f32<T>(xr[c]) - mean) * rstd;
@@ -79,16 +118,6 @@ __global__ void __launch_bounds__(256) norm_loop_kernel(const NormParams p) {
         }
     }
 }
-
-// ---------------------------------------------------------------------------
-// Rows in registers.  A group of `warps` warps owns a row; every thread holds the same NV pieces of columns in every row,
-// and one exchange between the group's warps joins their sums.
-//
-// Forward statistics (here and below): each warp computes the mean of its own columns and the sum of squared deviations
-// from that mean, and the warps' results are merged with  M2 = sum M2_w + n_w (mean_w - mean)^2,  which loses nothing
-// when the mean is large against the deviation and needs one exchange, not two.
-// ---------------------------------------------------------------------------
-constexpr int MAX_WARPS = MAX_ROW_WARPS;
 
 template <typename T, int NV, int N>
 __device__ __forceinline__ void load_params(const void* p, bool f32, int64_t D, int first, int step, float absent, float (&f)[NV * N]) {
@@ -121,7 +150,8 @@ template <typename T, bool WIDE, int NV, bool MULTI, bool PACK>
 __global__ void __launch_bounds__(512, 2) norm_kernel(const NormParams p, int warps) {
     using P = Piece<T, WIDE>;
     constexpr int N = P::N;
-    __shared__ float2 part[MULTI ? 2 * MAX_WARPS : 1];
+    __shared__ float2 part[MULTI ? 2 * MAX_WARPS : 1];     // center and squares of a warp
+    __shared__ float part_sum[MULTI ? 2 * MAX_WARPS : 1];
     __shared__ uint32_t part_top[MULTI && PACK ? 2 * MAX_WARPS : 1];
     const int lane = threadIdx.x & 31, threads = warps * 32;
     const int group = MULTI ? threadIdx.x / threads : threadIdx.x >> 5;
@@ -156,37 +186,42 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(const NormParams p, int wa
         bool odd = false;                                   // the warp holds an infinity or NaN of this row
         uint32_t top = 0u;
         if (PACK) top = warp_top<T, WIDE, NV>(x, odd);
-        float mean = warp_sum(s) * inv_mine, m2 = 0.f;      // of the warp's columns
+        s = warp_sum(s);
+        float mean = s * inv_mine, m2 = 0.f;                // the warp's center, deviations from it and their squares
+        s = sizeof(T) == 2 ? fmaf(-mine, mean, s) : 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (gt + i * threads < pieces) {
                 float f[N];
                 P::decode(x[i], f);
 #pragma unroll
-                for (int q = 0; q < N; ++q) { const float d = f[q] - mean; m2 = fmaf(d, d, m2); }
+                for (int q = 0; q < N; ++q) {
+                    const float d = f[q] - mean;
+                    if (sizeof(T) == 4) s += d;
+                    m2 = fmaf(d, d, m2);
+                }
             }
         }
+        if constexpr (sizeof(T) == 4) s = warp_sum(s);
         m2 = warp_sum(m2);
-        if constexpr (MULTI) {
-            float2* slot = part + parity * MAX_WARPS + group * warps;
-            uint32_t* slot_top = part_top + (PACK ? parity * MAX_WARPS + group * warps : 0);
+        if constexpr (!MULTI) {
+            finish_stats(mean, s, m2, inv_d, mean, m2);
+        } else {
+            const int at = parity * MAX_WARPS + group * warps;
             if (lane == 0) {
-                slot[gw] = make_float2(mean, m2);
-                if (PACK) slot_top[gw] = top;
+                part[at + gw] = make_float2(mean, m2);
+                part_sum[at + gw] = s;
+                if (PACK) part_top[at + gw] = top;
             }
             group_sync(group, threads);
-            mean = 0.f;
+            const float c0 = part[at].x;
+            float t = 0.f, q = 0.f;
             for (int k = 0; k < warps; ++k) {
-                mean = fmaf(columns_of(k), slot[k].x, mean);
-                if (PACK) top = max(top, slot_top[k]);
+                const float2 v = part[at + k];
+                add_part(c0, v.x, v.y, part_sum[at + k], columns_of(k), t, q);
+                if (PACK) top = max(top, part_top[at + k]);
             }
-            mean *= inv_d;
-            m2 = 0.f;
-            for (int k = 0; k < warps; ++k) {
-                const float2 v = slot[k];
-                const float d = v.x - mean;
-                m2 += fmaf(columns_of(k) * d, d, v.y);
-            }
+            finish_stats(c0, t, q, inv_d, mean, m2);
             parity ^= 1;                                    // the next row's exchange leaves these slots alone
         }
         const float rstd = 1.f / sqrtf(m2 * inv_d + p.eps);
@@ -396,7 +431,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
     constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2;
     constexpr int ROW = NV * RING_THREADS * 16, STAGE = U * ROW;      // bytes: [row][piece][thread]
     extern __shared__ __align__(16) unsigned char ring_smem[];
-    __shared__ float2 part[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];      // U == 2: [parity][group][row][warp]
+    __shared__ float2 part[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];      // center and squares; U == 2: [parity][group][row][warp]
+    __shared__ float part_sum[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];
     __shared__ uint32_t part_top[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];
     __shared__ float held[MAX_WARPS];                       // columns of each of the group's warps
     const int warps = W ? W : row_warps;
@@ -453,7 +489,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         typename P::Raw raw[U][NV];
         float2 x[U][NV][H];
-        float mean[U], m2[U];
+        float mean[U], m2[U], dev[U];                       // first the warp's center, squares and sum of the deviations from it
         uint32_t top[U];
         bool odd[U];
 #pragma unroll
@@ -475,40 +511,55 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
         slot += STAGE;
         if (slot == slot_end) slot = slot0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) mean[u] = warp_sum(mean[u]) * inv_mine;
+        for (int u = 0; u < U; ++u) {
+            const float sum = warp_sum(mean[u]);
+            mean[u] = sum * inv_mine;
+            dev[u] = U == 2 && !W ? fmaf(-static_cast<float>(mine), mean[u], sum) : 0.f;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float2 neg = splat(-mean[u]);
-            float2 s2 = splat(0.f);
+            float2 s1 = splat(0.f), s2 = splat(0.f);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (in[i]) {
 #pragma unroll
-                    for (int h = 0; h < H; ++h) { const float2 d = __fadd2_rn(x[u][i][h], neg); s2 = __ffma2_rn(d, d, s2); }
+                    for (int h = 0; h < H; ++h) {
+                        const float2 d = __fadd2_rn(x[u][i][h], neg);
+                        if (U == 1) s1 = __fadd2_rn(s1, d);
+                        s2 = __ffma2_rn(d, d, s2);
+                    }
                 }
             m2[u] = s2.x + s2.y;
+            if (U == 1) dev[u] = s1.x + s1.y;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) m2[u] = warp_sum(m2[u]);
+        for (int u = 0; u < U; ++u) {
+            m2[u] = warp_sum(m2[u]);
+            if (U == 1) dev[u] = warp_sum(dev[u]);
+        }
         if (warps == 1) {
-        } else if constexpr (U == 2) {
-            if (lane == 0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u) finish_stats(mean[u], dev[u], m2[u], inv_d, mean[u], m2[u]);
+        } else if constexpr (U == 2) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (lane == 0) {
                     part[exchange + u * 16 + gw] = make_float2(mean[u], m2[u]);
+                    if (!W) part_sum[exchange + u * 16 + gw] = dev[u];
                     if (PACK) part_top[exchange + u * 16 + gw] = top[u];
                 }
             }
             group_sync(group, threads);
             const bool has = (lane & 15) < warps;
-            const float2 v = has ? part[exchange + lane] : splat(0.f);
-            const float n = has ? (W ? 32.f * RING_COLUMNS : held[lane & 15]) : 0.f;
-            float m[1] = {n * v.x};
-            half_warp_sums<1>(m);
-            m[0] *= inv_d;
-            const float d = v.x - m[0];
-            float q[1] = {fmaf(n * d, d, v.y)};
-            half_warp_sums<1>(q);
+            const float c0 = part[exchange + (lane & 16)].x;
+            float both[2] = {0.f, 0.f}, row_mean, row_m2;
+            if (has) {
+                const float2 v = part[exchange + lane];
+                add_part(c0, v.x, v.y, W ? 0.f : part_sum[exchange + lane], (W ? 32.f * RING_COLUMNS : held[lane & 15]), both[0], both[1]);
+            }
+            half_warp_sums<2>(both);
+            finish_stats(c0, both[0], both[1], inv_d, row_mean, row_m2);
             uint32_t t = PACK && has ? part_top[exchange + lane] : 0u;
             if (PACK) {
 #pragma unroll
@@ -516,8 +567,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                mean[u] = __shfl_sync(FULL_MASK, m[0], u * 16);
-                m2[u] = __shfl_sync(FULL_MASK, q[0], u * 16);
+                mean[u] = __shfl_sync(FULL_MASK, row_mean, u * 16);
+                m2[u] = __shfl_sync(FULL_MASK, row_m2, u * 16);
                 if (PACK) top[u] = __shfl_sync(FULL_MASK, t, u * 16);
             }
             exchange += other;
@@ -525,24 +576,19 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_ring_kernel(const NormPa
         } else {
             if (lane == 0) {
                 part[exchange + gw] = make_float2(mean[0], m2[0]);
+                part_sum[exchange + gw] = dev[0];
                 if (PACK) part_top[exchange + gw] = top[0];
             }
             group_sync(group, threads);
-            float m = 0.f, q = 0.f;
-#pragma unroll
-            for (int k = 0; k < (W ? W : warps); ++k) {
-                m = fmaf(W ? 1.f : held[k], part[exchange + k].x, m);
-                if (PACK) top[0] = max(top[0], part_top[exchange + k]);
-            }
-            m *= W ? 1.f / (W ? W : 1) : inv_d;
+            const float c0 = part[exchange].x;
+            float t = 0.f, q = 0.f;
 #pragma unroll
             for (int k = 0; k < (W ? W : warps); ++k) {
                 const float2 v = part[exchange + k];
-                const float d = v.x - m;
-                q += fmaf((W ? 32.f * RING_COLUMNS : held[k]) * d, d, v.y);
+                add_part(c0, v.x, v.y, part_sum[exchange + k], W ? 32.f * RING_COLUMNS : held[k], t, q);
+                if (PACK) top[0] = max(top[0], part_top[exchange + k]);
             }
-            mean[0] = m;
-            m2[0] = q;
+            finish_stats(c0, t, q, inv_d, mean[0], m2[0]);
             exchange += other;
             other = -other;
         }
@@ -806,7 +852,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
     using P = Piece<T, true>;
     constexpr int N = P::N, NV = RING_COLUMNS / N, H = N / 2, XB = static_cast<int>(sizeof(typename P::Packed));
     extern __shared__ __align__(16) unsigned char ring_smem[];
-    __shared__ float2 part[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];      // U == 2: [parity][group][row][warp]
+    __shared__ float2 part[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];      // center and squares; U == 2: [parity][group][row][warp]
+    __shared__ float part_sum[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];
     __shared__ uint32_t part_top[U == 2 ? 2 * 8 * 32 : 2 * MAX_WARPS];
     __shared__ float held[MAX_WARPS];                       // columns of each of the group's warps
     const int lane = threadIdx.x & 31, threads = warps * 32;
@@ -858,7 +905,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
         sync();                                             // the other threads' granules
         typename P::Raw raw[U][NV];
         float2 x[U][NV][H];
-        float mean[U], m2[U];
+        float mean[U], m2[U], dev[U];                       // first the warp's center, squares and sum of the deviations from it
         uint32_t top[U];
         bool odd[U];
 #pragma unroll
@@ -882,11 +929,15 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
         }
         if (slot == slot_end) slot = slot0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) mean[u] = warp_sum(mean[u]) * inv_mine;
+        for (int u = 0; u < U; ++u) {
+            const float sum = warp_sum(mean[u]);
+            mean[u] = sum * inv_mine;
+            dev[u] = U == 2 ? fmaf(-static_cast<float>(mine), mean[u], sum) : 0.f;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float2 neg = splat(-mean[u]);
-            float2 s2 = splat(0.f);
+            float2 s1 = splat(0.f), s2 = splat(0.f);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -896,32 +947,40 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
                         if (2 * h >= valid[i]) d.x = 0.f;
                         if (2 * h + 1 >= valid[i]) d.y = 0.f;
                     }
+                    if (U == 1) s1 = __fadd2_rn(s1, d);
                     s2 = __ffma2_rn(d, d, s2);
                 }
             }
             m2[u] = s2.x + s2.y;
+            if (U == 1) dev[u] = s1.x + s1.y;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) m2[u] = warp_sum(m2[u]);
+        for (int u = 0; u < U; ++u) {
+            m2[u] = warp_sum(m2[u]);
+            if (U == 1) dev[u] = warp_sum(dev[u]);
+        }
         if (warps == 1) {
-        } else if constexpr (U == 2) {
-            if (lane == 0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u) finish_stats(mean[u], dev[u], m2[u], inv_d, mean[u], m2[u]);
+        } else if constexpr (U == 2) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (lane == 0) {
                     part[exchange + u * 16 + gw] = make_float2(mean[u], m2[u]);
+                    part_sum[exchange + u * 16 + gw] = dev[u];
                     if (PACK) part_top[exchange + u * 16 + gw] = top[u];
                 }
             }
             group_sync(group, threads);
             const bool has = (lane & 15) < warps;
-            const float2 v = has ? part[exchange + lane] : splat(0.f);
-            const float n = has ? held[lane & 15] : 0.f;
-            float m[1] = {n * v.x};
-            half_warp_sums<1>(m);
-            m[0] *= inv_d;
-            const float d = v.x - m[0];
-            float q[1] = {fmaf(n * d, d, v.y)};
-            half_warp_sums<1>(q);
+            const float c0 = part[exchange + (lane & 16)].x;
+            float both[2] = {0.f, 0.f}, row_mean, row_m2;
+            if (has) {
+                const float2 v = part[exchange + lane];
+                add_part(c0, v.x, v.y, part_sum[exchange + lane], held[lane & 15], both[0], both[1]);
+            }
+            half_warp_sums<2>(both);
+            finish_stats(c0, both[0], both[1], inv_d, row_mean, row_m2);
             uint32_t t = PACK && has ? part_top[exchange + lane] : 0u;
             if (PACK) {
 #pragma unroll
@@ -929,8 +988,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                mean[u] = __shfl_sync(FULL_MASK, m[0], u * 16);
-                m2[u] = __shfl_sync(FULL_MASK, q[0], u * 16);
+                mean[u] = __shfl_sync(FULL_MASK, row_mean, u * 16);
+                m2[u] = __shfl_sync(FULL_MASK, row_m2, u * 16);
                 if (PACK) top[u] = __shfl_sync(FULL_MASK, t, u * 16);
             }
             exchange += other;
@@ -938,22 +997,18 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_shift_kernel(const NormP
         } else {
             if (lane == 0) {
                 part[exchange + gw] = make_float2(mean[0], m2[0]);
+                part_sum[exchange + gw] = dev[0];
                 if (PACK) part_top[exchange + gw] = top[0];
             }
             group_sync(group, threads);
-            float m = 0.f, q = 0.f;
-            for (int k = 0; k < warps; ++k) {
-                m = fmaf(held[k], part[exchange + k].x, m);
-                if (PACK) top[0] = max(top[0], part_top[exchange + k]);
-            }
-            m *= inv_d;
+            const float c0 = part[exchange].x;
+            float t = 0.f, q = 0.f;
             for (int k = 0; k < warps; ++k) {
                 const float2 v = part[exchange + k];
-                const float d = v.x - m;
-                q += fmaf(held[k] * d, d, v.y);
+                add_part(c0, v.x, v.y, part_sum[exchange + k], held[k], t, q);
+                if (PACK) top[0] = max(top[0], part_top[exchange + k]);
             }
-            mean[0] = m;
-            m2[0] = q;
+            finish_stats(c0, t, q, inv_d, mean[0], m2[0]);
             exchange += other;
             other = -other;
         }

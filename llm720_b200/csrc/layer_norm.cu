@@ -1423,8 +1423,13 @@ template <typename T, bool WIDE, int NV, bool PACK>
 cudaError_t norm_launch(const NormParams& p, const RowShape& h, cudaStream_t s) {
     const int64_t need = (p.rows + h.groups - 1) / h.groups;
     const unsigned grid = static_cast<unsigned>(need < GRID_SMS * 16 ? need : GRID_SMS * 16), threads = h.warps * h.groups * 32;
-    if (h.warps > 1) norm_kernel<T, WIDE, NV, true, PACK><<<grid, threads, 0, s>>>(p, h.warps);
-    else norm_kernel<T, WIDE, NV, false, PACK><<<grid, threads, 0, s>>>(p, h.warps);
+    if constexpr (!WIDE || NV == 1) {                        // eight pieces a thread: rows of three warps and more
+        if (h.warps == 1) {
+            norm_kernel<T, WIDE, NV, false, PACK><<<grid, threads, 0, s>>>(p, h.warps);
+            return cudaGetLastError();
+        }
+    }
+    norm_kernel<T, WIDE, NV, true, PACK><<<grid, threads, 0, s>>>(p, h.warps);
     return cudaGetLastError();
 }
 
@@ -1455,8 +1460,13 @@ template <typename T, bool WIDE, int NV, bool KEPT>
 cudaError_t norm_grad_launch(const NormGradParams& p, const RowShape& h, cudaStream_t s) {
     const unsigned threads = h.warps * h.groups * 32, grid = static_cast<unsigned>(p.splits);
     const size_t smem = h.groups > 1 ? sizeof(float) * 2 * h.warps * 32 * NV * Piece<T, WIDE>::N : 0;
-    if (h.warps > 1) norm_grad_kernel<T, WIDE, NV, true, KEPT><<<grid, threads, smem, s>>>(p, h.warps);
-    else norm_grad_kernel<T, WIDE, NV, false, KEPT><<<grid, threads, smem, s>>>(p, h.warps);
+    if constexpr (WIDE ? NV == 1 : NV < 16) {                // sixteen values a thread: rows of five warps and more
+        if (h.warps == 1) {
+            norm_grad_kernel<T, WIDE, NV, false, KEPT><<<grid, threads, smem, s>>>(p, h.warps);
+            return cudaGetLastError();
+        }
+    }
+    norm_grad_kernel<T, WIDE, NV, true, KEPT><<<grid, threads, smem, s>>>(p, h.warps);
     return cudaGetLastError();
 }
 

@@ -227,9 +227,17 @@ cudaError_t pack_launch(const T* x, int64_t x_stride, int64_t rows, int64_t D, u
                         cudaStream_t s) {
     const int64_t need = (rows + h.groups - 1) / h.groups;
     const unsigned grid = static_cast<unsigned>(need < GRID_SMS * 16 ? need : GRID_SMS * 16), threads = h.warps * h.groups * 32;
-    if (h.warps > 1) pack_rows_kernel<T, WIDE, NV, true><<<grid, threads, 0, s>>>(x, x_stride, rows, D, payload, scale, h.warps);
-    else pack_rows_kernel<T, WIDE, NV, false><<<grid, threads, 0, s>>>(x, x_stride, rows, D, payload, scale, h.warps);
-    return cudaGetLastError();
+    if constexpr (NV < 16) {                                 // sixteen values a thread: rows of nine warps and more
+        if (h.warps == 1) {
+            pack_rows_kernel<T, WIDE, NV, false><<<grid, threads, 0, s>>>(x, x_stride, rows, D, payload, scale, h.warps);
+            return cudaGetLastError();
+        }
+    }
+    if constexpr (!WIDE || NV == 1 || NV == 8) {             // two and four pieces: what brings a row down to one warp
+        pack_rows_kernel<T, WIDE, NV, true><<<grid, threads, 0, s>>>(x, x_stride, rows, D, payload, scale, h.warps);
+        return cudaGetLastError();
+    }
+    return cudaErrorInvalidValue;
 }
 
 constexpr int64_t SHIFT_ROWS = 1024;      // fewer rows: latency, not the loads' width, decides

@@ -156,7 +156,7 @@ class PeerOp:
         for name, p in (("ln_w", ln_w), ("ln_b", ln_b)):
             if p is not None and p.numel() != self.cfg.input_dim:
                 raise ValueError(f"{name} has {p.numel()} values, expected {self.cfg.input_dim}")
-        if out.data_ptr() == hidden.data_ptr():
+        if hidden.numel() and out.data_ptr() == hidden.data_ptr():
             raise ValueError("out may not alias hidden")
         self._dev(product_ids_out, "product_ids_out", torch.int32)
         t = self._tensors(hidden, w, out, ids_out, scores_out, product_ids_out=product_ids_out)

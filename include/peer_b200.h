@@ -22,6 +22,8 @@
 extern "C" {
 #endif
 
+/* Changes when a struct or function that was there changes; added functions leave it (a library without them fails at link or
+ * load time). */
 #define PEER_B200_ABI_VERSION 2
 
 /* Return codes.  Nothing in this library falls back to another code path:
@@ -342,7 +344,8 @@ int peer_usage_histogram(const int64_t* ids, int64_t n_ids, int64_t* counts, int
  * Rows are `dim` consecutive values (1 <= dim <= PEER_ROW_DIM_MAX); inputs may have a row stride (in
  * elements) of their own, outputs are contiguous and overlap no input; pointers are aligned to their type.
  * dtype: F32, BF16 or F16; sums and statistics are fp32.
- * Results do not vary from run to run (no accumulation in memory). */
+ * Nothing outside the buffers is read, whatever their addresses: a buffer of rows reaches from its first row's first value to its
+ * last row's last one.  Results do not vary from run to run (no accumulation in memory). */
 #define PEER_ROW_DIM_MAX (1 << 20)
 
 /* Layer norm, the block's ln_2 (llm/models/foundation.py:118, 196-199) as an operator with a gradient:
@@ -377,7 +380,7 @@ int peer_block_norm(const void* x, int32_t dtype, const float* weight, const flo
 int peer_pack_rows(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t dim, void* payload,
                    float* scale, void* stream);
 
-/* The values packed rows stand for: payload * scale, clamped to dtype's finite range. */
+/* The values packed rows stand for: payload * scale (any scale, a caller's own too), clamped to dtype's finite range. */
 int peer_unpack_rows(const void* payload, const float* scale, int32_t dtype, int64_t rows, int64_t dim, void* out,
                      void* stream);
 

@@ -27,6 +27,6 @@ def pack_rows_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def unpack_rows_e4m3(payload: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that ``pack_rows_e4m3``'s result stands for, clamped to the finite range of ``dtype``.  Not
-    differentiable."""
+    """The values that ``pack_rows_e4m3``'s result stands for, clamped to the finite range of ``dtype``
+    (scale may be any fp32 numbers).  Not differentiable."""
     return _ext.load().unpack_rows(payload, scale, dtype)

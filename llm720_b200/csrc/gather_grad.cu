@@ -232,7 +232,7 @@ cudaError_t launch_ch(const GradParams& p, int sm_count, cudaStream_t s) {
 // themselves, so as in the forward pass they are kept on their way: every lane copies its own chunks of the next entries'
 // rows into shared memory (cp.async, nobody else reads them, so no barrier), FACTOR_DEPTH - 1 entries ahead; u is read from
 // there once and stays in registers for dx.  Ids, weights and results are held by the lanes, 32 entries at a time.
-// 16,384 tokens x 128 pairs of 4 KB rows: 2.5 ms = 6.9 TB/s; reading rows where they are used 7.5 ms.
+// 16,384 tokens x 128 pairs of 4 KB rows: 2.7 ms = 6.4 TB/s; reading rows where they are used 7.5 ms.
 constexpr int FACTOR_WARPS = 8, FACTOR_DEPTH = 3;
 
 template <typename XT, int CH>

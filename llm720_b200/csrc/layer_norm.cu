@@ -388,8 +388,9 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, 
 // no registers, and what is left in a row's chain is one exchange between the group's warps.
 // With the loads covered the instruction count decides: values are decoded once, kept as fp32 pairs across the exchange
 // and go through the packed fp32 instructions, two columns each.  The forward pass takes two rows at a time of the 16-bit
-// types, whose exchanges cover one another; the backward pass has no registers for two.  16384 x 2048 bf16: forward 24.8 us
-// (5.4 TB/s), dx 34.8 us (5.8 TB/s), all gradients 39.0 us; 4096 x 8192: 26.6, 37.0 and 45.2 us.
+// types, whose exchanges cover one another; the backward pass has no registers for two.  One block per SM, whose registers and
+// shared memory it takes.  16384 x 2048 bf16: forward 25.4 us (5.3 TB/s), dx 34.3 us (5.9 TB/s), all gradients 38.9 us;
+// 4096 x 8192: 26.8, 37.3 and 45.2 us.
 // W > 0: the row is exactly W full warps (512 W columns), which turns the addresses of a thread's pieces and the exchange
 // into constants; W == 0 takes any other width.
 // ---------------------------------------------------------------------------
@@ -828,7 +829,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_ring_kernel(const N
 // ---------------------------------------------------------------------------
 // The same for rows that are not whole 16-byte pieces at 16-byte addresses (an odd width, an odd stride, a view that
 // begins anywhere), brought and stored as the granules that cover them (row_shift.cuh).  A granule is another thread's,
-// so a row has a barrier behind its arrival and one before its results leave.  16384 x 2001 bf16: forward 46 us, all
+// so a row has a barrier behind its arrival and one before its results leave.  16384 x 2001 bf16: forward 47 us, all
 // gradients 64 us, against 172 and 187 us one value at a time.
 // ---------------------------------------------------------------------------
 // parameters of this thread's columns, `absent` beyond the row's end
@@ -1225,8 +1226,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) norm_grad_shift_kernel(const 
     }
 }
 
-// Backward of rows beyond 8,192 values (and of wide ones at odd addresses when there are few): dx by a block per row, which
-// reads it twice, the second time from L1; the column sums by a pass of their own.  4096 x 12288 bf16: dx 84 us, all gradients
+// Backward of rows beyond 8,192 values, and of an empty batch (column sums of zero): dx by a block per row, which reads it
+// twice, the second time from L1; the column sums by a pass of their own.  4096 x 12288 bf16: dx 84 us, all gradients
 // 138 us (floor 46 us; 238 and 350 us value by value): no ring as below, whose 16 columns per thread end at 8,192.
 template <typename T, bool WIDE, bool KEPT>
 __device__ __forceinline__ void x_piece(const NormGradParams& p, int64_t r, int64_t c, float scale, float (&f)[Piece<T, WIDE>::N]) {
@@ -1366,7 +1367,7 @@ constexpr int64_t RING_VALUES = 1000000, RING_GRAD_VALUES = 1 << 19;
 bool ring_pays(int64_t rows, int64_t D, int64_t values) { return rows >= RING_ROWS || rows * D >= values || D > RING_DIM; }
 
 // Rows at any address: a warp's 512 columns are too many for narrower ones (32768 x 129 bf16: 23 us forward, 21 us one
-// value at a time; 16384 x 2001: 46 and 172); the backward pass needs more rows (1500 x 1001 bf16: 13.4 us, 12.4 one value at a
+// value at a time; 16384 x 2001: 47 and 172); the backward pass needs more rows (1500 x 1001 bf16: 13.4 us, 12.4 one value at a
 // time; 1500 x 4099: 29 and 33; 512 x 8191: 27 and 21; 5003 x 1537 fp16: 27 and 41)
 constexpr int64_t SHIFT_DIM = 256, SHIFT_GRAD_ROWS = 2048, SHIFT_GRAD_DIM = 2000;
 bool shift_grad_pays(int64_t rows, int64_t D) {
@@ -1382,8 +1383,8 @@ inline int ring_width(int64_t D) {
 
 template <typename T, int W, bool PACK>
 cudaError_t norm_ring_width(const NormParams& p, cudaStream_t s) {
-    // rows a group takes at a time: two cover one another's exchange (16384 x 2048 bf16 24.8 us instead of 26.8, x 1536 22.7
-    // instead of 30, 4096 x 8192 26.8 instead of 37); fp32 rows are bound by memory with one
+    // rows a group takes at a time: two cover one another's exchange (16384 x 2048 bf16 24.7 us instead of 30.8, x 1536 22.6
+    // instead of 29.2, 4096 x 8192 26.6 instead of 39); fp32 rows are bound by memory with one
     constexpr int U = sizeof(T) == 4 ? 1 : 2, ROWS = sizeof(T) == 4 ? 4 : 6;      // rows in the ring: 128 KB, 96 KB
     constexpr int SMEM = ROWS * RING_THREADS * RING_COLUMNS * static_cast<int>(sizeof(T));
     const int warps = ring_warps(p.D), groups = MAX_WARPS / warps;

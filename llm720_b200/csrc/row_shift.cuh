@@ -11,7 +11,7 @@
 
 namespace peer {
 
-constexpr int RING_COLUMNS = 16, RING_THREADS = 512;      // columns per thread; one block per SM
+constexpr int RING_COLUMNS = 16, RING_THREADS = 512;      // columns per thread, threads of a block at most
 inline int ring_warps(int64_t D) { return static_cast<int>((D + 32 * RING_COLUMNS - 1) / (32 * RING_COLUMNS)); }
 
 // 16, 8 or 4 bytes of this thread's shared memory

@@ -22,5 +22,6 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x is fp32, bf16 or fp16, of any shape and strides; weight and bias [D] are fp32 (what the reference keeps)
     or of x's dtype, and either may be missing.  ``checkpoint="e4m3"`` keeps x in 8 bits for the backward pass
-    (a quarter to a half of the memory); y and the row statistics are those of the exact x.  Differentiable once."""
+    (a quarter to a half of the memory); y and the row statistics are those of the exact x.  Differentiable once,
+    backward; a tensor with a forward-mode tangent is refused."""
     return _ext.load().layer_norm(x, weight, bias, eps, checkpoint)

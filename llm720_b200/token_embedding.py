@@ -21,5 +21,6 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, pa
 
     An id outside [0, V) (-1 for a position without a token, say) reads nothing: its row is zero and takes no
     part in the gradient; ``dropped`` (int64 [1] on the device) is increased by the number of such ids.  The row
-    ``padding_idx`` is read like any other and receives a gradient of zero.  Differentiable once, in weight."""
+    ``padding_idx`` is read like any other and receives a gradient of zero.  Differentiable once, backward, in
+    weight; a table with a forward-mode tangent is refused."""
     return _ext.load().embedding(ids, weight, scale, padding_idx, dropped)
